@@ -604,6 +604,102 @@ AXM_API int axm_moe_ep_forward_host(const AxmEpLayout* layout, const AxmMoeDesc*
                                     void* d_out, void* workspace, size_t workspace_bytes, int32_t chunks,
                                     uint32_t* step, void* stream);
 
+/* ---- microscaled operands: 4-bit weights and activations, 8-bit checkpoints ----------
+ * No reference counterpart (the engine's weights are bf16 with fp32 masters,
+ * core/src/CUDA/util/gpu_types.cuh:148-168); the formats are the OCP microscaling ones.
+ * 32 neighbours along the reduction axis share one power of two 2^(s - 127), s a byte:
+ *   s = exponent of the largest magnitude - emax + 127, at least 0 (a block of zeros: 0);
+ *   a block with an infinity or a NaN: s = 255, and all of it reads as NaN.
+ * A value divided by that power is rounded to nearest, ties to even, and saturates:
+ *   4 bits  e2m1, magnitudes 0 0.5 1 1.5 2 3 4 6, emax 2, two a byte (lower index in the low half)
+ *   8 bits  e4m3, up to 448, emax 8
+ * 4-bit codes are [rows][K/2] (activations) or [E][N][K/2] (weights: K is the reduction axis,
+ * so they are the transposes of the engine's [E][K][N]).  Their scale bytes are kept in the
+ * tensor core's order: tiles of 128 rows, a tile = ceil(K/256) * 2 chunks of 512 bytes, the
+ * byte of (row r, block b) of a chunk at (r % 32) * 16 + (r / 32) * 4 + b % 4.  Rows of
+ * activations that a segment table divides start a new tile with every segment: those of
+ * segment s are in the tiles from out_row0 / 128 + s on.  8-bit codes are [rows][K], their
+ * scale bytes [rows][K/32].  K is a multiple of 32, N a multiple of 8; matrices, codes and
+ * tile-ordered scales are 16-byte aligned.  Tables must be ordered by out_row0, their rows
+ * disjoint and inside `rows`. */
+enum { AXM_DTYPE_BF16 = 0, AXM_DTYPE_FP32 = 1 };
+
+/* Bytes of the codes and of the tile-ordered scales.  num_segments 0: no table. */
+AXM_API int axm_mx4_rows_bytes(int32_t rows, int32_t num_segments, int32_t k, size_t* code_bytes,
+                               size_t* scale_bytes);
+AXM_API int axm_mx4_weights_bytes(int32_t experts, int32_t k, int32_t n, size_t* code_bytes,
+                                  size_t* scale_bytes);
+
+/* Rows of a matrix (row stride ld elements: a multiple of 16 bytes) to 4 bits.  Row r is read
+ * from source row row_src[r] / row_div (row_src NULL: r; row_src[r] < 0: zeros), so that the
+ * layer's permutation can be applied on the way (axm_moe_permute's row_src with row_div = k).
+ * segments NULL: all rows form one segment; rows outside every segment get no scale bytes. */
+AXM_API int axm_mx4_quantize_rows(const void* x, int32_t x_dtype, int64_t ld, const int32_t* row_src,
+                                  int32_t row_div, int32_t rows, int32_t k, const AxmSegment* segments,
+                                  int32_t num_segments, void* codes, void* scales, void* stream);
+/* ... and back to bf16 or fp32 (rows outside every segment are left as they are). */
+AXM_API int axm_mx4_dequantize_rows(const void* codes, const void* scales, int32_t rows, int32_t k,
+                                    const AxmSegment* segments, int32_t num_segments, void* out,
+                                    int32_t out_dtype, int64_t ld, void* stream);
+
+/* Expert weights [E][K][N] (bf16, or the fp32 master copies) to 4 bits, and back. */
+AXM_API int axm_mx4_quantize_weights(const void* w, int32_t w_dtype, int32_t experts, int32_t k, int32_t n,
+                                     void* codes, void* scales, void* stream);
+AXM_API int axm_mx4_dequantize_weights(const void* codes, const void* scales, int32_t experts, int32_t k,
+                                       int32_t n, void* w, int32_t w_dtype, void* stream);
+/* Scale bytes as checkpoints keep them, [E][N][K/32], to the tiles' order (once, after loading;
+ * the codes of such a checkpoint, [E][N][K/2], are used as they are). */
+AXM_API int axm_mx4_pack_scales(const void* plain, int32_t experts, int32_t k, int32_t n, void* scales,
+                                void* stream);
+
+/* Rows to 8 bits and back: activations laid aside between a forward and a backward pass. */
+AXM_API int axm_mx8_quantize_rows(const void* x, int32_t x_dtype, int64_t ld, int32_t rows, int32_t k,
+                                  void* codes, void* scales, void* stream);
+AXM_API int axm_mx8_dequantize_rows(const void* codes, const void* scales, int32_t rows, int32_t k,
+                                    void* out, int32_t out_dtype, int64_t ld, void* stream);
+
+/* out[t] = q4(x[t]) . W^T for one weight matrix [N][K] in 4 bits: x (bf16 or fp32, row stride ld)
+ * is quantised into the workspace, the product runs on the 4-bit tensor cores with fp32
+ * accumulators, out is [T][N] bf16 or fp32.  The first word of the workspace (256-byte aligned)
+ * is the status word: non-zero when a bounded wait inside a kernel gave up. */
+AXM_API int axm_mx4_linear_workspace_bytes(int32_t tokens, int32_t k, int32_t n, size_t* bytes);
+AXM_API int axm_mx4_linear(const void* x, int32_t x_dtype, int64_t ld, int32_t tokens, int32_t k, int32_t n,
+                           const void* w_codes, const void* w_scales, void* out, int32_t out_dtype,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Weights of a set of experts in 4 bits: gate and up [E][F][D/2], down [E][D][F/2], with their
+ * tile-ordered scales. */
+typedef struct AxmMx4Experts {
+  const void* gate_codes;
+  const void* gate_scales;
+  const void* up_codes;
+  const void* up_scales;
+  const void* down_codes;
+  const void* down_scales;
+} AxmMx4Experts;
+
+/* The expert feed-forward from 4-bit weights: o = q4(silu(g) u) . Wd[e]^T,
+ * g = q4(x) . Wg[e]^T, u = q4(x) . Wu[e]^T over the rows of each segment (a_row0 == out_row0; at
+ * most desc->tokens rows each).  x [rows][D] bf16, o [rows][D] bf16 or fp32; rows outside every
+ * segment of o are left as they are.  desc gives tokens, d_model and d_ff (multiples of 32) and
+ * num_experts.  Workspace as for axm_mx4_linear. */
+AXM_API int axm_mx4_expert_ffn_workspace_bytes(const AxmMoeDesc* desc, int32_t rows, int32_t num_segments,
+                                               size_t* bytes);
+AXM_API int axm_mx4_expert_ffn(const AxmMoeDesc* desc, const void* x, int32_t rows,
+                               const AxmSegment* segments, int32_t num_segments,
+                               const AxmMx4Experts* experts, void* o, int32_t o_dtype, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* axm_moe_forward with expert weights in 4 bits (and shared experts', when num_shared > 0):
+ * router, permutation and combine are the layer's own, the expert feed-forward is the one above,
+ * with the quantisation of x folded into the permutation's row copies.  tensors->w_* and shared_*
+ * are not looked at; AXM_FLAG_H_EXACT does not apply.  Workspace: 256-byte aligned, its first word
+ * the status word. */
+AXM_API int axm_moe_mx4_workspace_bytes(const AxmMoeDesc* desc, size_t* bytes);
+AXM_API int axm_moe_forward_mx4(const AxmMoeDesc* desc, const AxmMoeTensors* tensors,
+                                const AxmMx4Experts* experts, const AxmMx4Experts* shared, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 /* Number of token blocks the router splits T into (rows of block_counts). */
 #define AXM_ROUTE_BLOCKS 296
 

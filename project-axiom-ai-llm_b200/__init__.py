@@ -30,6 +30,8 @@ FLAG_HIST_ACCUMULATE = 2
 FLAG_H_EXACT = 4
 ROUTE_BLOCKS = 296
 SEG_ALT_A = 1 << 30
+DTYPE_BF16 = 0
+DTYPE_FP32 = 1
 NOALLOC_MAX_EXPERTS = 128
 
 
@@ -79,6 +81,11 @@ class MoeTrain(ctypes.Structure):
 class MoeCheckpoint(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("router_w", "router_bias", "w_gate", "w_up", "w_down",
                                                "shared_gate", "shared_up", "shared_down")]
+
+
+class Mx4ExpertWeights(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("gate_codes", "gate_scales", "up_codes", "up_scales",
+                                               "down_codes", "down_scales")]
 
 
 class Segment(ctypes.Structure):
@@ -155,6 +162,22 @@ def load():
     lib.axm_moe_checkpoint_probe.argtypes = [ctypes.c_char_p, dp, ctypes.POINTER(i32)]
     lib.axm_moe_checkpoint_load.argtypes = [ctypes.c_char_p, dp, cp]
     lib.axm_moe_cast_master.argtypes = [vp, vp, sz, vp]
+    szp, i64, mp = ctypes.POINTER(sz), ctypes.c_int64, ctypes.POINTER(Mx4ExpertWeights)
+    lib.axm_mx4_rows_bytes.argtypes = [i32, i32, i32, szp, szp]
+    lib.axm_mx4_weights_bytes.argtypes = [i32, i32, i32, szp, szp]
+    lib.axm_mx4_quantize_rows.argtypes = [vp, i32, i64, vp, i32, i32, i32, vp, i32, vp, vp, vp]
+    lib.axm_mx4_dequantize_rows.argtypes = [vp, vp, i32, i32, vp, i32, vp, i32, i64, vp]
+    lib.axm_mx4_quantize_weights.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp]
+    lib.axm_mx4_dequantize_weights.argtypes = [vp, vp, i32, i32, i32, vp, i32, vp]
+    lib.axm_mx4_pack_scales.argtypes = [vp, i32, i32, i32, vp, vp]
+    lib.axm_mx8_quantize_rows.argtypes = [vp, i32, i64, i32, i32, vp, vp, vp]
+    lib.axm_mx8_dequantize_rows.argtypes = [vp, vp, i32, i32, vp, i32, i64, vp]
+    lib.axm_mx4_linear_workspace_bytes.argtypes = [i32, i32, i32, szp]
+    lib.axm_mx4_linear.argtypes = [vp, i32, i64, i32, i32, i32, vp, vp, vp, i32, vp, sz, vp]
+    lib.axm_mx4_expert_ffn_workspace_bytes.argtypes = [dp, i32, i32, szp]
+    lib.axm_mx4_expert_ffn.argtypes = [dp, vp, i32, vp, i32, mp, vp, i32, vp, sz, vp]
+    lib.axm_moe_mx4_workspace_bytes.argtypes = [dp, szp]
+    lib.axm_moe_forward_mx4.argtypes = [dp, ctypes.POINTER(MoeTensors), mp, mp, vp, sz, vp]
     _lib = lib
     return lib
 

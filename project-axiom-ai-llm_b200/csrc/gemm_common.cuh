@@ -106,6 +106,13 @@ int encode_tensor_map_f32(CUtensorMap* m, const void* base, int rank, const uint
 int encode_tensor_map_sw64(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
                            const uint64_t* strides_bytes, const uint32_t* box);
 
+// Map of bytes with 128-byte swizzle (box inner extent 128): 4-bit codes, two a byte.
+int encode_tensor_map_bytes(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
+                            const uint64_t* strides_bytes, const uint32_t* box);
+// Map of 32-bit words without swizzle: the scale bytes of 4-bit operands, four a word.
+int encode_tensor_map_words(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
+                            const uint64_t* strides_bytes, const uint32_t* box);
+
 // Two-SM (cta_group::2) kernels are the default; AXM_GEMM_2SM=0 selects the one-SM kernels.
 bool use_2sm_kernels();
 // Input-gradient GEMM of the backward pass on CTA pairs (grouped_ffn_2sm.cu).

@@ -383,6 +383,17 @@ int encode_tensor_map_f32(CUtensorMap* m, const void* base, int rank, const uint
   return encode_tensor_map_typed(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, rank, dims, strides_bytes, box);
 }
 
+int encode_tensor_map_bytes(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
+                            const uint64_t* strides_bytes, const uint32_t* box) {
+  return encode_tensor_map_typed(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rank, dims, strides_bytes, box);
+}
+
+int encode_tensor_map_words(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
+                            const uint64_t* strides_bytes, const uint32_t* box) {
+  return encode_tensor_map_typed(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, rank, dims, strides_bytes, box,
+                                 CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 int launch_expert_ffn_2sm(const AxmMoeDesc* d, const void* x_perm, int32_t a_rows, const void* x_alt,
                           int32_t alt_rows, const AxmSegment* segments, int32_t num_segments,
                           const void* w_gate, const void* w_up, const void* w_down,

@@ -1,0 +1,152 @@
+// Microscaled blocks: 32 neighbours along the reduction axis share one power of two.
+//
+//   scale byte  s = max(exponent field of the block's largest magnitude (as fp32) - emax, 0),
+//               i.e. 2^(s - 127) with s - 127 = floor(log2(amax)) - emax, emax = 2 (e2m1) or 8 (e4m3);
+//               a block of zeros has s = 0, a block with an infinity or a NaN has s = 255 and
+//               stands for NaNs
+//   code        x * 2^(127 - s), a product that is exact, rounded to nearest even by the
+//               conversion instruction, saturating at 6 (e2m1) or 448 (e4m3)
+//
+// 4-bit operands of the matrix products (csrc/mx4_gemm.cu): two codes a byte, the lower index in
+// the low half; rows of K / 2 bytes.  Their scale bytes are kept in the order in which the tensor
+// core wants them in tensor memory: a tile is 128 rows, a chunk of a tile 128 rows x 128 elements
+// = 512 bytes with the byte of (row r, block b) at (r % 32) * 16 + (r / 32) * 4 + b.  A tile's
+// chunks follow one another, ceil(K / 256) * 2 of them (a pipeline stage is 256 elements); the
+// bytes of blocks beyond K are 0, those of rows that do not exist are never written.
+// Tiles of activations start at each segment's first row: rows of segment s are in the tiles from
+// out_row0 / 128 + s on (never two segments in one tile, whatever their lengths).
+#pragma once
+
+#include "common.cuh"
+
+namespace axm {
+
+constexpr int kMxBlock = 32;
+
+__host__ __device__ constexpr int mx4_chunks(int k) { return (k + 255) / 256 * 2; }
+__host__ __device__ constexpr long long mx4_row_tiles(long long rows, int num_segments) {
+  return rows / 128 + num_segments;
+}
+
+// The rows of a grouped 4-bit product: a segment table in device memory (its rows are out_row0 ..
+// of the operand and of the output; a_row0 is not looked at), or none: one segment of all rows.
+struct Mx4Rows {
+  const AxmSegment* segments;
+  int num_segments;
+  int rows;            // of the operand and of the output
+  int table_segments;  // segments of the whole table the scale tiles were laid out with
+  int seg_base;        // index of segments[0] in that table
+  int expert_base;     // expert id of the first weight matrix of this launch
+  int max_rows;        // most rows any segment can have (the number of tokens)
+  int32_t* status;
+};
+
+// q4 of the rows of a bf16 or fp32 matrix (microscale.cu).  Row r < tail_row0 comes from source row
+// row_src[r] / row_div (row_src null: r), rows from tail_row0 on from (r - tail_row0) % tail_mod.
+struct Mx4Gather {
+  const int32_t* row_src;
+  int row_div;
+  int tail_row0;
+  int tail_mod;
+};
+int launch_mx4_quantize_rows(const void* x, int32_t dtype, int64_t ld, const Mx4Gather& from, const Mx4Rows& rows, int k,
+                             void* codes, void* scales, cudaStream_t st);
+// The products (mx4_gemm.cu).
+int launch_mx4_linear(const Mx4Rows& r, const void* a_codes, const void* a_scales, const void* w_codes,
+                      const void* w_scales, int experts, int k, int n, void* out, bool out_bf16, cudaStream_t st);
+int launch_mx4_gated(const Mx4Rows& r, const void* a_codes, const void* a_scales, const AxmMx4Experts* w, int experts,
+                     int d, int f, void* h_codes, void* h_scales, cudaStream_t st);
+
+#if defined(__CUDACC__)
+
+// Scale byte of a block whose largest magnitude has these fp32 bits (sign cleared).
+template <int kEmax>
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {
+  const int e = (int)(amax_bits >> 23);
+  if (e == 255) return 255u;
+  return e > kEmax ? (uint32_t)(e - kEmax) : 0u;
+}
+// 2^(127 - s): what a block's values are multiplied with before the conversion.  (s <= 253 for
+// finite blocks; for s = 255 the result does not matter, the block reads as NaN.)
+__device__ __forceinline__ float mx_inverse_scale(uint32_t s) {
+  return __uint_as_float(s >= 254u ? 0x00800000u : (254u - s) << 23);
+}
+// 2^(s - 127); s = 0 is a subnormal, s = 255 a NaN.
+__device__ __forceinline__ float mx_scale_value(uint32_t s) {
+  return __uint_as_float(s == 255u ? 0x7fc00000u : (s == 0u ? 0x00400000u : s << 23));
+}
+
+// Eight values to eight e2m1 codes, value 0 in the lowest four bits.
+__device__ __forceinline__ uint32_t mx4_pack8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t"
+      ".reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t"
+      "}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+// The magnitude of an e2m1 code in fp32: 0 0.5 1 1.5 2 3 4 6 (with its sign).
+__device__ __forceinline__ float mx4_code_value(uint32_t code) {
+  const uint32_t m = code & 7u;
+  // exponent field and mantissa bit moved to fp32's places; the one subnormal (0.5) by hand
+  const uint32_t bits = m > 1u ? ((m << 22) + (126u << 23)) : (m ? 0x3f000000u : 0u);
+  return __uint_as_float(bits | ((code & 8u) << 28));
+}
+
+// Four values to four e4m3 codes, value 0 in the lowest byte.
+__device__ __forceinline__ uint32_t mx8_pack4(float a, float b, float c, float d) {
+  uint32_t r;
+  asm("{\n\t"
+      ".reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t"
+      "}"
+      : "=r"(r)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
+}
+// Two e4m3 codes (low half of the word first) to fp32.
+__device__ __forceinline__ float2 mx8_unpack2(uint32_t two) {
+  uint32_t h;
+  asm("{\n\t"
+      ".reg .b16 t;\n\t"
+      "cvt.u16.u32 t, %1;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, t;\n\t"
+      "}"
+      : "=r"(h)
+      : "r"(two));
+  float2 f;
+  asm("{\n\t"
+      ".reg .b16 lo, hi;\n\t"
+      "mov.b32 {lo, hi}, %2;\n\t"
+      "cvt.f32.f16 %0, lo;\n\t"
+      "cvt.f32.f16 %1, hi;\n\t"
+      "}"
+      : "=f"(f.x), "=f"(f.y)
+      : "r"(h));
+  return f;
+}
+
+// The segment that output row `row` belongs to (the last one that starts at or before it and has
+// rows); tables are ordered by out_row0.  -1: the row is behind its segment's end.
+__device__ __forceinline__ int segment_of_row(const AxmSegment* segments, int n, int row) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (__ldg(&segments[mid].out_row0) <= row) lo = mid; else hi = mid - 1;
+  }
+  // segments without rows share their start with the next one: the last of them was found
+  const int first = __ldg(&segments[lo].out_row0);
+  return (row >= first && row - first < __ldg(&segments[lo].rows)) ? lo : -1;
+}
+
+#endif
+
+}  // namespace axm

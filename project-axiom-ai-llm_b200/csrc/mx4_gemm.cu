@@ -1,0 +1,532 @@
+// Products of microscaled 4-bit matrices on the tensor cores (tcgen05.mma kind::mxf4, e2m1 codes,
+// one power-of-two scale byte per 32 elements of the reduction, fp32 accumulators in tensor
+// memory), grouped over the layer's segment table:
+//
+//   kModeLinear  out[r][n] = sum_k A[r][k] W[e][n][k]                      (fp32 or bf16 rows)
+//   kModeGated   h[r][f]   = q4( silu(g) u ),  g = A[r] . Wg[e][f],  u = A[r] . Wu[e][f]
+//
+// The second keeps the whole gate: both projections run in one accumulator (columns 0..127 gate,
+// 128..255 up), the epilogue thread that owns a row multiplies, finds each 32-block's largest
+// magnitude in its own registers and writes codes and scale bytes, so the intermediate of the
+// expert feed-forward touches memory at 4.25 bits a value and is the next product's A operand as
+// it lies.  The bf16 form of the same operator is grouped_ffn_2sm.cu
+// (core/src/CUDA/kernel/moe_router.cu:155-190 of the reference engine).
+//
+// Thread-block clusters of two CTAs, cta_group::2: M = 256 over the pair, N = 256, a stage of 256
+// reduction elements = 128 bytes of codes a row.  Each CTA loads its 128 rows of A, 128 of the 256
+// weight rows (Gated: the leader the gate rows, the peer the up rows) and the scale bytes of its
+// own A rows and of ALL 256 weight rows: 35 KB a stage, six stages.  At the 4-bit rate a stage
+// lasts about 520 cycles, so a single CTA's 128 x 256 tile (51 KB a stage) would ask more of L2
+// than it gives; the pair form asks 67 bytes a cycle and SM.
+// Scale bytes go from shared to tensor memory with tcgen05.cp (32 lanes x 16 bytes, repeated in
+// the four lane quarters), in order with the MMAs of the same issuing thread.
+//
+// Tensor memory: two 256-column accumulators and 24 columns of scales do not fit in 512 columns.
+// The accumulators overlap: the first is columns 0..255, the second 232..487, scales 488..511.
+// The epilogue takes the 32-column blocks that hold the shared columns first and then lets the
+// next tile's MMAs start; everything else of it runs under them.
+#include <mutex>
+
+#include "gemm_2sm.cuh"
+#include "microscale.cuh"
+
+namespace axm {
+
+namespace {
+
+enum { kModeLinear = 0, kModeGated = 1 };
+
+constexpr int kKStage = 256;                          // reduction elements a stage
+constexpr int kCodeBytes = 128 * kKStage / 2;         // 16 KiB: 128 rows of A, or of the weights
+constexpr int kScaleABytes = 2 * 512;                 // this CTA's 128 rows, two 128-element chunks
+constexpr int kScaleBBytes = 4 * 512;                 // 256 weight rows
+constexpr int kStageBytes4 = 2 * kCodeBytes + kScaleABytes + kScaleBBytes;
+constexpr int kStages4 = 6;
+constexpr int kThreads4 = 192;
+
+constexpr uint32_t kAcc1 = 232;   // first column of the second accumulator
+constexpr uint32_t kSfA = 488;    // 2 x 4 columns
+constexpr uint32_t kSfB = 496;    // 2 x 8 columns
+
+struct __align__(8) Mx4Shared {
+  uint64_t full[kStages4];   // used in the leader: bytes of both CTAs land here
+  uint64_t empty[kStages4];  // own: the leader's MMA commit arrives in both CTAs
+  uint64_t tmem_full[2];     // own
+  uint64_t overlap_free;     // used in the leader: 4 epilogue warps of each CTA, once a tile
+  uint32_t tmem_base;
+  int abort_flag;
+  int total_units;
+  int num_groups;
+  int tile_prefix[kMaxSegments + 1];
+  int group_first[kMaxSegments + 1];
+  int pair_prefix[kMaxSegments + 1];
+  AxmSegment seg[kMaxSegments];
+};
+constexpr size_t kMx4SmemBytes = 1024 + (size_t)kStages4 * kStageBytes4 + sizeof(Mx4Shared);
+static_assert(kMx4SmemBytes <= 227u * 1024u, "shared memory of the 4-bit pair kernel");
+
+struct Mx4Args {
+  const AxmSegment* segments;
+  int num_segments;
+  int n_total;       // Linear: columns of out; Gated: columns of h
+  int k_total;
+  int rows_total;    // without a segment table: the rows of the one segment, expert 0
+  int seg_base;      // index of segments[0] in the layer's whole table (scale tiles count from there)
+  int expert_base;   // expert id of the first weight matrix
+  int out_bf16;      // Linear
+  int wn_tiles;      // 128-row tiles of one expert's weights
+  void* out;         // Linear: rows of n_total; Gated: codes
+  uint8_t* out_scales;
+  int* status;
+};
+
+// Block-scaled kind::mxf4: A and B e2m1 (code 1), scale type ue8m0 (bit 23), M = 256 over the
+// pair, N = 256, both operands K-major.  Bits 29..30 and 4..5 pick the byte pair of the scale
+// words of A and B: the two 64-element steps of a 128-element chunk.
+constexpr uint32_t mx4_instr_desc(uint32_t step) {
+  return ((step * 2u) << 4) | (1u << 7) | (1u << 10) | ((256u >> 3) << 17) | (1u << 23) | ((256u >> 4) << 24) |
+         ((step * 2u) << 29);
+}
+
+__device__ __forceinline__ void tc_mma2_mx4(uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                            uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// 512 bytes of shared memory (32 rows of 16) to four columns of tensor memory, the same in all four
+// lane quarters, in both CTAs of the pair.
+__device__ __forceinline__ void tc_cp2_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Shared-memory descriptor of a 512-byte scale chunk: no swizzle, 8-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr >> 4) & 0x3fffu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+
+struct Unit4 {
+  int seg, m_tile, n_tile, seg0;
+  bool live;  // false: this half of the pair has no rows
+};
+
+// Units are ordered like those of the bf16 pair kernel: expert group by expert group, inside a
+// group column tile by column tile, and pairs of row tiles innermost, so that CTA pairs that run
+// together share a weight tile.
+__device__ __forceinline__ Unit4 decode4(const Mx4Shared* sh, int n_tiles, int unit, int rank) {
+  int lo = 0, hi = sh->num_groups - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (sh->pair_prefix[mid] * n_tiles <= unit) lo = mid; else hi = mid - 1;
+  }
+  const int s0 = sh->group_first[lo], s1 = sh->group_first[lo + 1];
+  const int base = sh->tile_prefix[s0];
+  const int mt = sh->tile_prefix[s1] - base;
+  const int pairs = sh->pair_prefix[lo + 1] - sh->pair_prefix[lo];
+  const int local = unit - sh->pair_prefix[lo] * n_tiles;
+  Unit4 u;
+  u.n_tile = local / pairs;
+  const int p = local - u.n_tile * pairs;
+  u.seg0 = s0;
+  u.live = 2 * p + rank < mt;
+  const int idx = base + 2 * p + (u.live ? rank : 0);
+  int a = s0, b = s1 - 1;
+  while (a < b) {
+    const int mid = (a + b + 1) >> 1;
+    if (sh->tile_prefix[mid] <= idx) a = mid; else b = mid - 1;
+  }
+  u.seg = a;
+  u.m_tile = idx - sh->tile_prefix[a];
+  return u;
+}
+
+// silu(g) u, and the block's codes and scale byte
+__device__ __forceinline__ uint4 gate_block(const uint32_t (&g)[32], const uint32_t (&u)[32], uint32_t& byte) {
+  float h[32];
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float gv = __uint_as_float(g[j]);
+    h[j] = __fdividef(gv, 1.0f + __expf(-gv)) * __uint_as_float(u[j]);
+    top = max(top, __float_as_uint(h[j]) & 0x7fffffffu);
+  }
+  byte = mx_scale_byte<2>(top);
+  const float inv = mx_inverse_scale(byte);
+  uint32_t q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = h[8 * i + j] * inv;
+    q[i] = mx4_pack8(t);
+  }
+  return make_uint4(q[0], q[1], q[2], q[3]);
+}
+
+template <int kMode>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads4, 1)
+mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a_sf,
+                     const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1,
+                     const __grid_constant__ CUtensorMap tm_b0_sf, const __grid_constant__ CUtensorMap tm_b1_sf,
+                     Mx4Args args) {
+  constexpr bool kGated = kMode == kModeGated;
+  constexpr int kCols = kGated ? 128 : 256;  // output columns a tile
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* tiles = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  // all codes first (1024-byte aligned stages of 32 KiB), then the scale bytes, then the control block
+  unsigned char* scales_s = tiles + (size_t)kStages4 * 2 * kCodeBytes;
+  Mx4Shared* sh = reinterpret_cast<Mx4Shared*>(scales_s + (size_t)kStages4 * (kScaleABytes + kScaleBBytes));
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t peer = rank ^ 1u;
+  const int cluster_id = blockIdx.x >> 1;
+  const int num_clusters = gridDim.x >> 1;
+  const int n_tiles = (args.n_total + kCols - 1) / kCols;
+  const int k_blocks = (args.k_total + kKStage - 1) / kKStage;
+  const int nseg = args.num_segments;
+
+  for (int s = threadIdx.x; s < nseg; s += kThreads4)
+    sh->seg[s] = args.segments != nullptr ? args.segments[s] : AxmSegment{0, 0, args.rows_total, 0};
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages4; ++i) {
+      mbar_init(&sh->full[i], 1);
+      mbar_init(&sh->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&sh->tmem_full[i], 1);
+    mbar_init(&sh->overlap_free, 8);
+    sh->abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_a_sf);
+    tma_prefetch_desc(&tm_b0);
+    tma_prefetch_desc(&tm_b0_sf);
+    if (kGated) {
+      tma_prefetch_desc(&tm_b1);
+      tma_prefetch_desc(&tm_b1_sf);
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc2(&sh->tmem_base, kTmemCols);
+    tmem_relinquish2();
+  }
+  if (threadIdx.x == 0) {
+    int acc = 0;
+    for (int s = 0; s < nseg; ++s) {
+      sh->tile_prefix[s] = acc;
+      const int rows = sh->seg[s].rows;
+      acc += rows > 0 ? (rows + 127) / 128 : 0;
+    }
+    sh->tile_prefix[nseg] = acc;
+    int ng = 0;
+    for (int s = 0; s < nseg; ++s)
+      if (s == 0 || sh->seg[s].expert != sh->seg[s - 1].expert) sh->group_first[ng++] = s;
+    sh->group_first[ng] = nseg;
+    sh->num_groups = ng;
+    int pairs = 0;
+    for (int g = 0; g < ng; ++g) {
+      sh->pair_prefix[g] = pairs;
+      pairs += (sh->tile_prefix[sh->group_first[g + 1]] - sh->tile_prefix[sh->group_first[g]] + 1) / 2;
+    }
+    sh->pair_prefix[ng] = pairs;
+    sh->total_units = pairs * n_tiles;
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+
+  const int total_units = sh->total_units;
+  const uint32_t tmem_base = sh->tmem_base;
+  volatile int* abort_flag = &sh->abort_flag;
+  auto raise_abort = [&]() { st_cluster_u32(map_to_cta(smem_u32(&sh->abort_flag), peer), 1u); };
+
+  if (warp == 0) {
+    // ---- TMA producer --------------------------------------------------------------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int unit = cluster_id; ok && unit < total_units; unit += num_clusters) {
+        const Unit4 uc = decode4(sh, n_tiles, unit, (int)rank);
+        const AxmSegment sg = sh->seg[uc.seg];
+        const int e = (sh->seg[uc.seg0].expert & 0xffff) - args.expert_base;
+        const int a_row = sg.out_row0 + uc.m_tile * 128;
+        const int a_tile = sg.out_row0 / 128 + args.seg_base + uc.seg + uc.m_tile;
+        const CUtensorMap* mb = kGated && rank == 1 ? &tm_b1 : &tm_b0;
+        const int n_row = uc.n_tile * kCols + (kGated ? 0 : (int)rank * 128);
+        const int b_tile = e * args.wn_tiles + (kGated ? uc.n_tile : 2 * uc.n_tile);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&sh->empty[stage], phase ^ 1u, abort_flag)) {
+            raise_abort();
+            ok = false;
+            break;
+          }
+          unsigned char* sa = tiles + (size_t)stage * 2 * kCodeBytes;
+          unsigned char* ssf = scales_s + (size_t)stage * (kScaleABytes + kScaleBBytes);
+          if (rank == 0) mbar_expect_tx(&sh->full[stage], 2 * kStageBytes4);
+          const uint32_t bar = map_to_cta(smem_u32(&sh->full[stage]), 0);
+          tma2_load_3d(sa, &tm_a, bar, kb * (kKStage / 2), a_row, 0);
+          tma2_load_3d(sa + kCodeBytes, mb, bar, kb * (kKStage / 2), n_row, e);
+          tma2_load_3d(ssf, &tm_a_sf, bar, 0, kb * 2, a_tile);
+          if constexpr (kGated) {
+            tma2_load_3d(ssf + kScaleABytes, &tm_b0_sf, bar, 0, kb * 2, b_tile);
+            tma2_load_3d(ssf + kScaleABytes + 1024, &tm_b1_sf, bar, 0, kb * 2, b_tile);
+          } else {
+            tma2_load_3d(ssf + kScaleABytes, &tm_b0_sf, bar, 0, kb * 2, b_tile);
+            // a weight matrix with an odd number of tiles: the next expert's bytes, or the fill
+            // value behind the last one; they scale columns that are not stored
+            tma2_load_3d(ssf + kScaleABytes + 1024, &tm_b0_sf, bar, 0, kb * 2, b_tile + 1);
+          }
+          if (++stage == kStages4) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer: the leader CTA only -----------------------------------------------------
+    if (lane == 0 && rank == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int tile = 0;
+      bool ok = true;
+      for (int unit = cluster_id; ok && unit < total_units; unit += num_clusters, ++tile) {
+        // the previous tile's epilogue has taken the columns both accumulators share (and, as it
+        // works tile by tile, has finished the tile before)
+        if (!mbar_wait(&sh->overlap_free, (uint32_t)(tile & 1) ^ 1u, abort_flag)) {
+          raise_abort();
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + ((tile & 1) ? kAcc1 : 0u);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&sh->full[stage], phase, abort_flag)) {
+            raise_abort();
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(tiles + (size_t)stage * 2 * kCodeBytes);
+          const uint32_t ssf = smem_u32(scales_s + (size_t)stage * (kScaleABytes + kScaleBBytes));
+          const uint64_t da = make_smem_desc(sa, 16, 1024);
+          const uint64_t db = make_smem_desc(sa + kCodeBytes, 16, 1024);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            tc_cp2_scales(tmem_base + kSfA + 4 * c, scale_desc(ssf + 512 * c));
+            tc_cp2_scales(tmem_base + kSfB + 8 * c, scale_desc(ssf + kScaleABytes + 512 * c));
+            tc_cp2_scales(tmem_base + kSfB + 8 * c + 4, scale_desc(ssf + kScaleABytes + 1024 + 512 * c));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // 64 elements = 32 bytes a step
+            tc_mma2_mx4(d_tmem, da + (uint64_t)(j * 2), db + (uint64_t)(j * 2), mx4_instr_desc(j & 1),
+                        tmem_base + kSfA + 4 * (j >> 1), tmem_base + kSfB + 8 * (j >> 1), (kb > 0 || j > 0) ? 1u : 0u);
+          tc_commit2(map_to_cta(smem_u32(&sh->empty[stage]), 0));
+          tc_commit2(map_to_cta(smem_u32(&sh->empty[stage]), 1));
+          if (++stage == kStages4) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit2(map_to_cta(smem_u32(&sh->tmem_full[tile & 1]), 0));
+        tc_commit2(map_to_cta(smem_u32(&sh->tmem_full[tile & 1]), 1));
+      }
+    }
+  } else {
+    // ---- epilogue: every CTA drains its own 128 accumulator rows --------------------------------
+    const int quad = warp & 3;
+    const uint32_t leader_free = map_to_cta(smem_u32(&sh->overlap_free), 0);
+    int tile = 0;
+    for (int unit = cluster_id; unit < total_units; unit += num_clusters, ++tile) {
+      const Unit4 uc = decode4(sh, n_tiles, unit, (int)rank);
+      const AxmSegment sg = sh->seg[uc.seg];
+      const int acc = tile & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&sh->tmem_full[acc], (uint32_t)((tile >> 1) & 1), abort_flag))) break;
+      tc_fence_after();
+      const int row_in_seg = uc.m_tile * 128 + quad * 32 + lane;
+      const bool row_ok = uc.live && row_in_seg < sg.rows;
+      const size_t row = (size_t)sg.out_row0 + (row_ok ? row_in_seg : 0);
+      const uint32_t t_addr = tmem_base + ((uint32_t)(quad * 32) << 16) + (acc ? kAcc1 : 0u);
+      const int n0 = uc.n_tile * kCols;
+      // blocks of 32 columns; the shared columns are the last 24 of accumulator 0 and the first
+      // 24 of accumulator 1
+      constexpr int kBlocks = kCols / 32;
+      uint32_t sf_word = 0;
+#pragma unroll 1
+      for (int i = 0; i < kBlocks; ++i) {
+        const int jb = acc ? i : kBlocks - 1 - i;
+        const int c0 = jb * 32;
+        uint32_t v[32];
+        __syncwarp();
+        tmem_ld32(t_addr + c0, v);
+        if constexpr (kGated) {
+          uint32_t u[32];
+          tmem_ld32(t_addr + 128 + c0, u);
+          tmem_ld_wait();
+          if (i == 0) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(leader_free);
+          }
+          if (uc.live && n0 + c0 < args.n_total) {  // n_total is a multiple of 32
+            uint32_t byte;
+            const uint4 q = gate_block(v, u, byte);
+            sf_word |= byte << (8 * jb);
+            if (row_ok)
+              __stcs(reinterpret_cast<uint4*>(static_cast<uint8_t*>(args.out) + row * (size_t)(args.n_total >> 1) +
+                                              ((n0 + c0) >> 1)), q);
+          }
+        } else {
+          tmem_ld_wait();
+          if (i == 0) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(leader_free);
+          }
+          if (row_ok) {
+            if (args.out_bf16) {
+              __nv_bfloat16* p = static_cast<__nv_bfloat16*>(args.out) + row * args.n_total + n0 + c0;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (n0 + c0 + q * 8 < args.n_total) {
+                  uint32_t w[4];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    w[j] = pack_bf16(__uint_as_float(v[8 * q + 2 * j]), __uint_as_float(v[8 * q + 2 * j + 1]));
+                  __stcs(reinterpret_cast<uint4*>(p + q * 8), make_uint4(w[0], w[1], w[2], w[3]));
+                }
+            } else {
+              float* p = static_cast<float*>(args.out) + row * args.n_total + n0 + c0;
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                if (n0 + c0 + q * 4 < args.n_total)
+                  __stcs(reinterpret_cast<uint4*>(p + q * 4), make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+            }
+          }
+        }
+      }
+      if constexpr (kGated) {
+        // one chunk of scale bytes a tile (128 columns); behind the last one of an odd number, zeros
+        if (row_ok) {
+          const int r = row_in_seg & 127;
+          const size_t t = (size_t)(sg.out_row0 / 128 + args.seg_base + uc.seg + uc.m_tile);
+          const int chunks = mx4_chunks(args.n_total);
+          uint8_t* p = args.out_scales + (t * chunks + uc.n_tile) * 512 + (r & 31) * 16 + (r >> 5) * 4;
+          *reinterpret_cast<uint32_t*>(p) = sf_word;
+          if (uc.n_tile == n_tiles - 1 && n_tiles < chunks) *reinterpret_cast<uint32_t*>(p + 512) = 0u;
+        }
+      }
+    }
+  }
+
+  // ---- drain: nobody leaves while the peer may still touch its shared memory or TMEM -----------
+  tc_fence_before();
+  __syncthreads();
+  if (sh->abort_flag != 0) {
+    long long t0 = clock64();
+    while (clock64() - t0 < 4000000LL) {
+    }
+    if (threadIdx.x == 0 && args.status != nullptr) atomicExch(args.status, kGated ? 11 : 12);
+  }
+  cluster_sync_all();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc2(tmem_base, kTmemCols);
+  }
+}
+
+// ---- host side -----------------------------------------------------------------------------
+
+// Codes: rows of k / 2 bytes, a box of 128 bytes x 128 rows, 128-byte swizzle.
+int map_codes(CUtensorMap* m, const void* base, uint64_t experts, uint64_t rows, uint64_t k) {
+  const uint64_t dims[3] = {k / 2, rows, experts};
+  const uint64_t strides[2] = {k / 2, k / 2 * rows};
+  const uint32_t box[3] = {128, 128, 1};
+  return encode_tensor_map_bytes(m, base, 3, dims, strides, box);
+}
+// Scale chunks: words [tiles][chunks][128], a box of two chunks of one tile.
+int map_scales(CUtensorMap* m, const void* base, uint64_t tiles, int k) {
+  const uint64_t dims[3] = {128, (uint64_t)mx4_chunks(k), tiles};
+  const uint64_t strides[2] = {512, 512ull * mx4_chunks(k)};
+  const uint32_t box[3] = {128, 2, 1};
+  return encode_tensor_map_words(m, base, 3, dims, strides, box);
+}
+
+template <int kMode>
+int launch_pair(const CUtensorMap& a, const CUtensorMap& a_sf, const CUtensorMap& b0, const CUtensorMap& b1,
+                const CUtensorMap& b0_sf, const CUtensorMap& b1_sf, const Mx4Args& args, cudaStream_t st) {
+  static SmemLimitCache smem = {};
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(mx4_gemm_pair_kernel<kMode>), kMx4SmemBytes, &smem,
+                                   "mx4_gemm_pair_kernel"))
+    return rc;
+  const int grid = grid_2sm();
+  if (grid < 0) return grid;
+  if (grid < 2) return fail(AXM_ERR_DEVICE, "two-SM clusters cannot be scheduled on this device");
+  mx4_gemm_pair_kernel<kMode><<<grid, kThreads4, kMx4SmemBytes, st>>>(a, a_sf, b0, b1, b0_sf, b1_sf, args);
+  return check_launch("mx4_gemm_pair_kernel");
+}
+
+}  // namespace
+
+// The tables' rows are out_row0 .. of A, of its scale tiles and of the output alike.
+static Mx4Args mx4_args(const Mx4Rows& r) {
+  Mx4Args ga = {};
+  ga.segments = r.segments;
+  ga.num_segments = r.segments != nullptr ? r.num_segments : 1;
+  ga.rows_total = r.rows;
+  ga.seg_base = r.seg_base;
+  ga.expert_base = r.expert_base;
+  ga.status = r.status;
+  return ga;
+}
+
+int launch_mx4_linear(const Mx4Rows& r, const void* a_codes, const void* a_scales, const void* w_codes,
+                      const void* w_scales, int experts, int k, int n, void* out, bool out_bf16, cudaStream_t st) {
+  CUtensorMap a, a_sf, b, b_sf;
+  int rc;
+  const int wn = (n + 127) / 128;
+  if ((rc = map_codes(&a, a_codes, 1, r.rows, k))) return rc;
+  if ((rc = map_scales(&a_sf, a_scales, mx4_row_tiles(r.rows, r.table_segments), k))) return rc;
+  if ((rc = map_codes(&b, w_codes, experts, n, k))) return rc;
+  if ((rc = map_scales(&b_sf, w_scales, (uint64_t)experts * wn, k))) return rc;
+  Mx4Args ga = mx4_args(r);
+  ga.n_total = n;
+  ga.k_total = k;
+  ga.out_bf16 = out_bf16 ? 1 : 0;
+  ga.wn_tiles = wn;
+  ga.out = out;
+  return launch_pair<kModeLinear>(a, a_sf, b, b, b_sf, b_sf, ga, st);
+}
+
+int launch_mx4_gated(const Mx4Rows& r, const void* a_codes, const void* a_scales, const AxmMx4Experts* w, int experts,
+                     int d, int f, void* h_codes, void* h_scales, cudaStream_t st) {
+  CUtensorMap a, a_sf, g, u, g_sf, u_sf;
+  int rc;
+  const int wn = (f + 127) / 128;
+  if ((rc = map_codes(&a, a_codes, 1, r.rows, d))) return rc;
+  if ((rc = map_scales(&a_sf, a_scales, mx4_row_tiles(r.rows, r.table_segments), d))) return rc;
+  if ((rc = map_codes(&g, w->gate_codes, experts, f, d))) return rc;
+  if ((rc = map_codes(&u, w->up_codes, experts, f, d))) return rc;
+  if ((rc = map_scales(&g_sf, w->gate_scales, (uint64_t)experts * wn, d))) return rc;
+  if ((rc = map_scales(&u_sf, w->up_scales, (uint64_t)experts * wn, d))) return rc;
+  Mx4Args ga = mx4_args(r);
+  ga.n_total = f;
+  ga.k_total = d;
+  ga.wn_tiles = wn;
+  ga.out = h_codes;
+  ga.out_scales = static_cast<uint8_t*>(h_scales);
+  return launch_pair<kModeGated>(a, a_sf, g, u, g_sf, u_sf, ga, st);
+}
+
+}  // namespace axm

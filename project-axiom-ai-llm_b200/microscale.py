@@ -1,0 +1,284 @@
+"""Microscaled operands from Python: expert weights and activations in 4 bits, activation
+checkpoints in 8 bits (formats in include/axm_moe.h).
+
+    quantize_rows(x) -> Mx4Rows             dequantize_rows(q) -> x
+    quantize_weights(w) -> Mx4Weights       dequantize_weights(q) -> w
+    quantize_rows8(x) -> (codes, scales)    dequantize_rows8(codes, scales) -> x
+    Mx4Linear        y = q4(x) . W^T for one weight matrix
+    Mx4ExpertFfn     the expert feed-forward over a segment table
+    Mx4MoeLayer      the whole layer (MoeLayer's call) with expert weights in 4 bits
+
+Like the rest of the package these are thin callers of the C ABI: tensors are device memory,
+work goes to the current stream, nothing synchronises.  The engine keeps its weights in bf16
+with fp32 masters (core/src/CUDA/util/gpu_types.cuh:148-168); either is a source here.
+"""
+import ctypes
+import importlib
+
+import torch
+
+_pkg = importlib.import_module(__package__)
+
+_DTYPES = {torch.bfloat16: _pkg.DTYPE_BF16, torch.float32: _pkg.DTYPE_FP32}
+
+
+def _dtype(t):
+    if t not in _DTYPES:
+        raise TypeError(f"bf16 or fp32 is needed, not {t}")
+    return _DTYPES[t]
+
+
+def _on(device):
+    """The library enqueues on the current device: make it the tensors'."""
+    return torch.cuda.device(device)
+
+
+def _rows_of(x):
+    if not x.is_cuda or x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError("a CUDA matrix with contiguous rows is needed")
+    return x.shape[0], x.shape[1], x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
+
+
+def _bytes(call, *args):
+    a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    _pkg.check(call(*args, ctypes.byref(a), ctypes.byref(b)))
+    return a.value, b.value
+
+
+class Mx4Rows:
+    """Rows in 4 bits: codes [rows][K/2], tile-ordered scales, the segment table they follow."""
+
+    def __init__(self, codes, scales, rows, k, segments=None):
+        self.codes, self.scales, self.rows, self.k, self.segments = codes, scales, rows, k, segments
+
+
+class Mx4Weights:
+    """Weights in 4 bits: codes [E][N][K/2], tile-ordered scales."""
+
+    def __init__(self, codes, scales, experts, k, n):
+        self.codes, self.scales, self.experts, self.k, self.n = codes, scales, experts, k, n
+
+    @classmethod
+    def from_checkpoint(cls, codes, scales):
+        """From codes [E][N][K/2] and scale bytes [E][N][K/32], as 4-bit checkpoints keep them.
+        The codes are used as they are, the scale bytes are brought into the tiles' order."""
+        lib = _pkg.load()
+        if not (codes.is_cuda and scales.is_cuda and codes.device == scales.device and
+                codes.is_contiguous() and scales.is_contiguous() and
+                codes.dtype == torch.uint8 and scales.dtype == torch.uint8 and codes.dim() == 3):
+            raise ValueError("contiguous uint8 CUDA tensors [E][N][K/2] and [E][N][K/32] on one device are needed")
+        e, n, k = codes.shape[0], codes.shape[1], 2 * codes.shape[2]
+        if scales.shape != (e, n, k // 32):
+            raise ValueError(f"scales {tuple(scales.shape)} do not belong to codes {tuple(codes.shape)}")
+        _, size = _bytes(lib.axm_mx4_weights_bytes, e, k, n)
+        with _on(codes.device):
+            packed = torch.empty(size, dtype=torch.uint8, device=codes.device)
+            _pkg.check(lib.axm_mx4_pack_scales(_pkg.ptr(scales), e, k, n, _pkg.ptr(packed), _pkg.current_stream()))
+        return cls(codes, packed, e, k, n)
+
+
+def quantize_rows(x, segments=None, row_src=None, row_div=1):
+    """x [rows][K] bf16 or fp32 to 4 bits; row_src: row r is read from x[row_src[r] // row_div]."""
+    lib = _pkg.load()
+    src_rows, k, ld = _rows_of(x)
+    rows = src_rows if row_src is None else row_src.numel()
+    nseg = 0 if segments is None else segments.shape[0]
+    n_codes, n_scales = _bytes(lib.axm_mx4_rows_bytes, rows, nseg, k)
+    with _on(x.device):
+        codes = torch.empty(rows, k // 2, dtype=torch.uint8, device=x.device)
+        scales = torch.empty(n_scales, dtype=torch.uint8, device=x.device)
+        _pkg.check(lib.axm_mx4_quantize_rows(_pkg.ptr(x), _dtype(x.dtype), ld, _pkg.ptr(row_src), row_div, rows, k,
+                                             _pkg.ptr(segments), nseg, _pkg.ptr(codes), _pkg.ptr(scales),
+                                             _pkg.current_stream()))
+    return Mx4Rows(codes, scales, rows, k, segments)
+
+
+def dequantize_rows(q, dtype=torch.bfloat16, out=None):
+    lib = _pkg.load()
+    with _on(q.codes.device):
+        if out is None:
+            out = torch.empty(q.rows, q.k, dtype=dtype, device=q.codes.device)
+        rows, k, ld = _rows_of(out)
+        if (rows, k) != (q.rows, q.k):
+            raise ValueError(f"out is {tuple(out.shape)}, the rows are {(q.rows, q.k)}")
+        nseg = 0 if q.segments is None else q.segments.shape[0]
+        _pkg.check(lib.axm_mx4_dequantize_rows(_pkg.ptr(q.codes), _pkg.ptr(q.scales), rows, k, _pkg.ptr(q.segments), nseg,
+                                               _pkg.ptr(out), _dtype(out.dtype), ld, _pkg.current_stream()))
+    return out
+
+
+def quantize_rows8(x):
+    """x [rows][K] to 8 bits: codes [rows][K] (e4m3), scale bytes [rows][K/32]."""
+    lib = _pkg.load()
+    rows, k, ld = _rows_of(x)
+    with _on(x.device):
+        codes = torch.empty(rows, k, dtype=torch.uint8, device=x.device)
+        scales = torch.empty(rows, k // 32, dtype=torch.uint8, device=x.device)
+        _pkg.check(lib.axm_mx8_quantize_rows(_pkg.ptr(x), _dtype(x.dtype), ld, rows, k, _pkg.ptr(codes), _pkg.ptr(scales),
+                                             _pkg.current_stream()))
+    return codes, scales
+
+
+def dequantize_rows8(codes, scales, dtype=torch.bfloat16):
+    lib = _pkg.load()
+    rows, k = codes.shape
+    with _on(codes.device):
+        out = torch.empty(rows, k, dtype=dtype, device=codes.device)
+        _pkg.check(lib.axm_mx8_dequantize_rows(_pkg.ptr(codes), _pkg.ptr(scales), rows, k, _pkg.ptr(out), _dtype(dtype), k,
+                                               _pkg.current_stream()))
+    return out
+
+
+def quantize_weights(w):
+    """w [E][K][N] bf16 or fp32 (the engine's layout, K is summed over) to 4 bits."""
+    lib = _pkg.load()
+    if not (w.is_cuda and w.dim() == 3 and w.is_contiguous()):
+        raise ValueError("a contiguous CUDA tensor [E][K][N] is needed")
+    e, k, n = w.shape
+    n_codes, n_scales = _bytes(lib.axm_mx4_weights_bytes, e, k, n)
+    with _on(w.device):
+        codes = torch.empty(e, n, k // 2, dtype=torch.uint8, device=w.device)
+        scales = torch.empty(n_scales, dtype=torch.uint8, device=w.device)
+        _pkg.check(lib.axm_mx4_quantize_weights(_pkg.ptr(w), _dtype(w.dtype), e, k, n, _pkg.ptr(codes), _pkg.ptr(scales),
+                                                _pkg.current_stream()))
+    return Mx4Weights(codes, scales, e, k, n)
+
+
+def dequantize_weights(q, dtype=torch.bfloat16):
+    lib = _pkg.load()
+    with _on(q.codes.device):
+        w = torch.empty(q.experts, q.k, q.n, dtype=dtype, device=q.codes.device)
+        _pkg.check(lib.axm_mx4_dequantize_weights(_pkg.ptr(q.codes), _pkg.ptr(q.scales), q.experts, q.k, q.n, _pkg.ptr(w),
+                                                  _dtype(dtype), _pkg.current_stream()))
+    return w
+
+
+class _Workspace:
+    """Scratch of one object; its first word is the status word."""
+
+    def _scratch(self, size, device):
+        self.workspace = torch.empty(max(size, 256), dtype=torch.uint8, device=device)
+
+    def status(self):
+        """Reads the status word of the last call (synchronises): 0, or the code of a kernel whose
+        bounded wait gave up."""
+        torch.cuda.synchronize(self.workspace.device)
+        return int(self.workspace[:4].view(torch.int32).item())
+
+
+class Mx4Linear(_Workspace):
+    """y = q4(x) . W^T with W ([1][N][K/2] in 4 bits) and scratch for up to `tokens` rows."""
+
+    def __init__(self, weights, tokens):
+        if weights.experts != 1:
+            raise ValueError("one weight matrix is needed")
+        self.lib, self.w, self.tokens = _pkg.load(), weights, tokens
+        n = ctypes.c_size_t(0)
+        _pkg.check(self.lib.axm_mx4_linear_workspace_bytes(tokens, weights.k, weights.n, ctypes.byref(n)))
+        self._scratch(n.value, weights.codes.device)
+
+    def forward(self, x, out=None, dtype=torch.bfloat16):
+        w = self.w
+        rows, k, ld = _rows_of(x)
+        if rows > self.tokens or k != w.k or x.device != w.codes.device:
+            raise ValueError(f"x {tuple(x.shape)} on {x.device}: up to {self.tokens} rows of {w.k} on {w.codes.device}")
+        if out is None:
+            out = torch.empty(rows, w.n, dtype=dtype, device=x.device)
+        elif out.shape != (rows, w.n) or not out.is_contiguous() or out.device != x.device:
+            raise ValueError("out must be a contiguous [rows][N] matrix beside x")
+        with _on(x.device):
+            _pkg.check(self.lib.axm_mx4_linear(_pkg.ptr(x), _dtype(x.dtype), ld, rows, k, w.n, _pkg.ptr(w.codes),
+                                               _pkg.ptr(w.scales), _pkg.ptr(out), _dtype(out.dtype),
+                                               _pkg.ptr(self.workspace), self.workspace.numel(), _pkg.current_stream()))
+        return out
+
+
+def _expert_table(gate, up, down):
+    if (gate.experts, gate.k, gate.n) != (up.experts, up.k, up.n) or \
+            (down.experts, down.k, down.n) != (gate.experts, gate.n, gate.k):
+        raise ValueError("gate and up are [E][F][D/2], down is [E][D][F/2]")
+    return _pkg.Mx4ExpertWeights(*(t.data_ptr() for w in (gate, up, down) for t in (w.codes, w.scales)))
+
+
+class Mx4ExpertFfn(_Workspace):
+    """The expert feed-forward from 4-bit weights over up to `rows` rows in up to `segments`
+    segments (default: one per expert) of at most `tokens` rows each."""
+
+    def __init__(self, gate, up, down, rows, tokens, segments=None):
+        self.lib = _pkg.load()
+        self.weights = (gate, up, down)
+        self.table = _expert_table(gate, up, down)
+        self.rows, self.segments = rows, gate.experts if segments is None else segments
+        self.desc = _pkg.make_desc(tokens, gate.k, gate.n, gate.experts, 1, flags=0)
+        n = ctypes.c_size_t(0)
+        _pkg.check(self.lib.axm_mx4_expert_ffn_workspace_bytes(ctypes.byref(self.desc), rows, self.segments,
+                                                               ctypes.byref(n)))
+        self._scratch(n.value, gate.codes.device)
+
+    def forward(self, x, segments, out=None, dtype=torch.bfloat16):
+        """x [rows][D] bf16, segments int32 [n][4] {a_row0, out_row0, rows, expert} (device)."""
+        rows, d, _ = _rows_of(x)
+        dev = self.workspace.device
+        if rows > self.rows or d != self.desc.d_model or not x.is_contiguous() or x.dtype != torch.bfloat16 or x.device != dev:
+            raise ValueError(f"x: up to {self.rows} contiguous bf16 rows of {self.desc.d_model} on {dev}")
+        if segments.dtype != torch.int32 or segments.shape[1:] != (4,) or not segments.is_contiguous() or \
+                segments.device != dev or segments.shape[0] > self.segments:
+            raise ValueError(f"segments: a contiguous int32 table of up to {self.segments} x 4 on {dev}")
+        if out is None:
+            out = torch.empty(rows, d, dtype=dtype, device=dev)
+        elif out.shape != x.shape or not out.is_contiguous() or out.device != dev:
+            raise ValueError("out must be a contiguous matrix like x")
+        with _on(dev):
+            _pkg.check(self.lib.axm_mx4_expert_ffn(ctypes.byref(self.desc), _pkg.ptr(x), rows, _pkg.ptr(segments),
+                                                   segments.shape[0], ctypes.byref(self.table), _pkg.ptr(out),
+                                                   _dtype(out.dtype), _pkg.ptr(self.workspace), self.workspace.numel(),
+                                                   _pkg.current_stream()))
+        return out
+
+
+class Mx4MoeLayer(_Workspace):
+    """MoeLayer with expert weights in 4 bits.  weights: router_w (and router_bias) as for MoeLayer;
+    gate, up, down (and shared_gate, shared_up, shared_down) Mx4Weights."""
+
+    def __init__(self, weights, tokens, top_k, residual=True, hist_accumulate=False):
+        self.lib, self.w = _pkg.load(), weights
+        wr, gate = weights["router_w"], weights["gate"]
+        self.experts = _expert_table(gate, weights["up"], weights["down"])
+        self.shared = None
+        shared = 0
+        if weights.get("shared_gate") is not None:
+            self.shared = _expert_table(weights["shared_gate"], weights["shared_up"], weights["shared_down"])
+            shared = weights["shared_gate"].experts
+        if wr.shape != (gate.k, gate.experts):
+            raise ValueError(f"router_w {tuple(wr.shape)}: [D][E] = {(gate.k, gate.experts)} is needed")
+        flags = (_pkg.FLAG_RESIDUAL if residual else 0) | (_pkg.FLAG_HIST_ACCUMULATE if hist_accumulate else 0)
+        self.desc = _pkg.make_desc(tokens, gate.k, gate.n, gate.experts, top_k, shared,
+                                   _pkg.ROUTER_FP32 if wr.dtype == torch.float32 else _pkg.ROUTER_BF16, flags)
+        n = ctypes.c_size_t(0)
+        _pkg.check(self.lib.axm_moe_mx4_workspace_bytes(ctypes.byref(self.desc), ctypes.byref(n)))
+        dev = wr.device
+        self._scratch(n.value, dev)
+        self.T, self.D, self.k = tokens, gate.k, top_k
+        self.topk_idx = torch.empty(tokens, top_k, dtype=torch.int32, device=dev)
+        self.topk_gate = torch.empty(tokens, top_k, dtype=torch.float32, device=dev)
+        self.histogram = torch.zeros(gate.experts, dtype=torch.int32, device=dev)
+
+    def forward(self, x, out=None):
+        """out = x + sum of the chosen experts' outputs (without residual: the sum), histogram."""
+        dev = self.workspace.device
+        if x.shape != (self.T, self.D) or x.dtype != torch.bfloat16 or not x.is_contiguous() or x.device != dev:
+            raise ValueError(f"x: contiguous bf16 {(self.T, self.D)} on {dev}")
+        if out is None:
+            out = torch.empty_like(x)
+        t = _pkg.MoeTensors()
+        t.x, t.out, t.router_w = x.data_ptr(), out.data_ptr(), self.w["router_w"].data_ptr()
+        if self.w.get("router_bias") is not None:
+            t.router_bias = self.w["router_bias"].data_ptr()
+        t.topk_idx, t.topk_gate = self.topk_idx.data_ptr(), self.topk_gate.data_ptr()
+        t.histogram = self.histogram.data_ptr()
+        with _on(dev):
+            _pkg.check(self.lib.axm_moe_forward_mx4(ctypes.byref(self.desc), ctypes.byref(t), ctypes.byref(self.experts),
+                                                    None if self.shared is None else ctypes.byref(self.shared),
+                                                    _pkg.ptr(self.workspace), self.workspace.numel(),
+                                                    _pkg.current_stream()))
+        return out, self.histogram

@@ -1,0 +1,370 @@
+"""Microscaled operands on the GPU against 64-bit references: codes and scale bytes exactly, products
+exactly where their sums provably fit 24 bits, else within the error of a sum in 32 bits."""
+import importlib
+
+import pytest
+import torch
+
+import microscale_ref as ref
+
+pytestmark = pytest.mark.gpu
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ms(axm):
+    return importlib.import_module("project_axiom_ai_llm_b200.microscale")
+
+
+def generator(dev, seed):
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    return g
+
+
+def awkward(rows, k, dtype, dev, seed):
+    """Normal rows with every block of another size, zeros, ties, subnormals, the largest values,
+    infinities and NaNs among them."""
+    g = generator(dev, seed)
+    x = torch.empty(rows, k, device=dev).normal_(generator=g)
+    power = torch.randint(-40, 40, (rows, k // 32), generator=g, device=dev).float()
+    x = x * torch.exp2(power).repeat_interleave(32, 1)
+    b = x.view(rows, -1, 32)
+    ties = torch.tensor([0.25, -.75, 1.25, -1.75, 2.5, -3.5, 5.0, 4.0], device=dev).repeat(4)
+    n = b.shape[0] * b.shape[1]
+    flat = b.view(n, 32)
+    flat[0::11] = ties * torch.exp2(torch.randint(-100, 100, (flat[0::11].shape[0], 1), generator=g, device=dev).float())
+    flat[1::13] = 0.0
+    flat[2::17] = torch.finfo(dtype).max
+    flat[3::19] = 1e-39
+    flat[4::23, 5] = float("nan")
+    flat[5::29, 31] = -float("inf")
+    flat[6::31] = 2.0 ** -126
+    return x.to(dtype)
+
+
+def table(counts, dev, align=1):
+    rows, at = [], 0
+    for e, c in enumerate(counts):
+        n = -(-c // align) * align
+        rows.append((at, at, n, e))
+        at += n
+    return torch.tensor(rows, dtype=torch.int32, device=dev), at
+
+
+def same(a, b):
+    """Equal, NaN in the same places."""
+    return torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.nan_to_num(a), torch.nan_to_num(b))
+
+
+def held_float(x, bits, dtype):
+    """Blocks as held, rounded to dtype (exact but for the smallest subnormals)."""
+    return (ref.held4(x) if bits == 4 else ref.held8(x)).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("rows,k", [(1, 32), (1, 4096), (7, 96), (129, 288), (300, 544), (1031, 2048)])
+def test_rows_4_bits(ms, cuda_device, rows, k, dtype):
+    x = awkward(rows, k, dtype, cuda_device, rows + k)
+    q = ms.quantize_rows(x)
+    code, s = ref.quantize4(x)
+    got = ref.unpack4(q.codes)
+    fine = (s != 255).repeat_interleave(32, 1)
+    assert torch.equal(got[fine], code[fine])
+    tiles = ref.tile_order(s)
+    there = ref.tile_order(torch.ones_like(s)) != 0
+    packed = q.scales.view(-1, tiles.shape[1], 512)[:tiles.shape[0]]
+    assert torch.equal(packed[there], tiles[there])
+    # bytes of blocks behind K are 0 in every row that exists
+    if k % 256:
+        rows_of = ref.tile_order(torch.ones(rows, (k + 255) // 256 * 8, dtype=torch.uint8, device=cuda_device)) != 0
+        assert (packed[rows_of & ~there] == 0).all()
+    for out in (BF16, FP32):
+        assert same(ms.dequantize_rows(q, out), held_float(x, 4, out))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("rows,k", [(1, 32), (3, 4096), (129, 288), (1031, 416)])
+def test_rows_8_bits(ms, cuda_device, rows, k, dtype):
+    x = awkward(rows, k, dtype, cuda_device, rows * k)
+    codes, s = ms.quantize_rows8(x)
+    assert torch.equal(s, ref.scale_bytes(x, 8))
+    for out in (BF16, FP32):
+        assert same(ms.dequantize_rows8(codes, s, out), held_float(x, 8, out))
+
+
+def test_rows_with_strides_and_sources(ms, cuda_device):
+    wide = awkward(40, 640, BF16, cuda_device, 4)
+    x = wide[:, 64:64 + 288]  # row stride 640, 16-byte aligned
+    assert same(ms.dequantize_rows(ms.quantize_rows(x)), held_float(x, 4, BF16))
+    out = torch.full((40, 640), 3.0, dtype=BF16, device=cuda_device)
+    ms.dequantize_rows(ms.quantize_rows(x), out=out[:, 64:64 + 288])
+    assert same(out[:, 64:64 + 288], held_float(x, 4, BF16))
+    assert (out[:, :64] == 3).all() and (out[:, 352:] == 3).all()
+    # rows gathered on the way, two slots a source row, one of them empty
+    src = torch.tensor([3, 79, -1, 0, 3, 42], dtype=torch.int32, device=cuda_device)
+    want = held_float(x, 4, BF16)[(src.long() // 2).clamp(min=0)]
+    want[2] = 0
+    assert same(ms.dequantize_rows(ms.quantize_rows(x, row_src=src, row_div=2)), want)
+    with pytest.raises(Exception):
+        ms.quantize_rows(wide[:, 4:4 + 288])  # not 16-byte aligned
+
+
+@pytest.mark.parametrize("counts", [[5], [0, 3, 0, 0, 200, 1, 0], [128, 128, 127, 129, 0], [1] * 70, [300, 0, 0]])
+def test_rows_by_segments(ms, cuda_device, counts):
+    segs, rows = table(counts, cuda_device)
+    k = 160
+    x = awkward(rows + 9, k, FP32, cuda_device, sum(counts))  # nine rows behind the last segment
+    q = ms.quantize_rows(x, segments=segs)
+    s = ref.scale_bytes(x, 2)
+    got = q.scales.view(-1, 2, 512)
+    at = 0
+    for e, c in enumerate(counts):
+        if c:
+            tiles = ref.tile_order(s[at:at + c])
+            there = ref.tile_order(torch.ones_like(s[at:at + c])) != 0
+            first = at // 128 + e
+            assert torch.equal(got[first:first + tiles.shape[0]][there], tiles[there])
+        at += c
+    out = torch.full((rows + 9, k), 7.0, device=cuda_device)
+    ms.dequantize_rows(q, out=out)
+    assert same(out[:rows], held_float(x, 4, FP32)[:rows])
+    assert (out[rows:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("e,k,n", [(1, 32, 8), (3, 96, 72), (2, 288, 136), (1, 544, 1000), (2, 2048, 64)])
+def test_weights(ms, cuda_device, e, k, n, dtype):
+    w = awkward(e * n, k, dtype, cuda_device, e + k + n).view(e, n, k).transpose(1, 2).contiguous()
+    q = ms.quantize_weights(w)
+    wt = w.transpose(1, 2).contiguous()
+    code, s = ref.quantize4(wt)
+    fine = (s != 255).repeat_interleave(32, -1)
+    assert torch.equal(ref.unpack4(q.codes)[fine], code[fine])
+    want = torch.stack([ref.tile_order(s[i]) for i in range(e)])
+    there = torch.stack([ref.tile_order(torch.ones_like(s[i])) for i in range(e)]) != 0
+    assert torch.equal(q.scales.view(want.shape)[there], want[there])
+    for out in (BF16, FP32):
+        assert same(ms.dequantize_weights(q, out), ref.held4(wt).to(out).transpose(1, 2))
+    p = ms.Mx4Weights.from_checkpoint(ref.pack4(code), s)
+    assert torch.equal(p.scales.view(want.shape)[there], want[there])
+
+
+def held_operand(rows, k, dev, seed, spread):
+    """Random 4-bit rows: packed codes, scale bytes and values; scales of 2^0 .. 2^spread.  Every
+    block begins with the largest code, so that its values quantise to themselves."""
+    g = generator(dev, seed)
+    code = torch.randint(0, 16, (rows, k), generator=g, device=dev, dtype=torch.uint8)
+    code[:, ::32] = 7
+    s = torch.randint(127, 128 + spread, (rows, k // 32), generator=g, device=dev, dtype=torch.uint8)
+    return ref.pack4(code), s, ref.values4(code, s)
+
+
+LINEAR = [(1, 32, 8), (1, 4096, 264), (2, 256, 136), (3, 64, 256), (16, 544, 1000), (17, 288, 512), (33, 96, 40),
+          (64, 1024, 384), (100, 512, 248), (127, 256, 128), (128, 320, 264), (129, 64, 520), (257, 736, 1288),
+          (700, 128, 2048)]
+
+
+@pytest.mark.parametrize("t,k,n", LINEAR)
+def test_linear_exact(ms, cuda_device, t, k, n):
+    """x is made of values that quantise to themselves; every sum of magnitudes fits 24 bits of the
+    smallest product, so whatever the order of additions the result is the exact one."""
+    _, _, x = held_operand(t, k, cuda_device, t + k, 1)
+    assert torch.equal(ref.held4(x), x)
+    codes, s, w = held_operand(n, k, cuda_device, n, 1)
+    want = x @ w.T
+    assert float((x.abs() @ w.abs().T).max()) < 2 ** 24 * 0.25 and float((want * 4 - torch.round(want * 4)).abs().max()) == 0
+    plan = ms.Mx4Linear(ms.Mx4Weights.from_checkpoint(codes.unsqueeze(0), s.unsqueeze(0)), t + 3)
+    for dt in (FP32, BF16):
+        for x_dt in (FP32, BF16):
+            out = torch.full((t + 1, n), float("nan"), dtype=dt, device=cuda_device)
+            plan.forward(x.to(x_dt), out=out[:t])
+            assert torch.equal(out[:t], want.to(dt)), (dt, x_dt)
+            assert torch.isnan(out[t]).all()
+    assert plan.status() == 0
+
+
+@pytest.mark.parametrize("t,k,n", [(1, 4096, 1024), (5, 2048, 392), (40, 1056, 640), (200, 4096, 512), (513, 1408, 1032)])
+def test_linear_wide_scales(ms, cuda_device, t, k, n):
+    g = generator(cuda_device, t)
+    x = torch.empty(t, k, device=cuda_device).normal_(generator=g) * torch.exp2(
+        torch.randint(-20, 20, (t, k // 32), generator=g, device=cuda_device).float()).repeat_interleave(32, 1)
+    codes, s, w = held_operand(n, k, cuda_device, n, 20)
+    plan = ms.Mx4Linear(ms.Mx4Weights.from_checkpoint(codes.unsqueeze(0), s.unsqueeze(0)), t)
+    y = plan.forward(x, dtype=FP32)
+    a = ref.held4(x)
+    # each of k additions rounds (or cuts) at 2^-23 of a partial sum of at most sum |a w|
+    bound = k * 2.0 ** -23 * (a.abs() @ w.abs().T)
+    assert ((y.double() - a @ w.T).abs() <= bound).all()
+    assert plan.status() == 0
+
+
+def test_linear_not_finite(ms, cuda_device):
+    x = torch.ones(4, 64, device=cuda_device)
+    x[1, 3], x[2, 40] = float("nan"), float("inf")
+    codes, s, w = held_operand(16, 64, cuda_device, 2, 1)
+    s[5, 1] = 255
+    y = ms.Mx4Linear(ms.Mx4Weights.from_checkpoint(codes.unsqueeze(0), s.unsqueeze(0)), 4).forward(x)
+    bad = torch.isnan(y)
+    assert bad[1].all() and bad[2].all() and bad[:, 5].all()
+    assert not bad[[0, 3]][:, [c for c in range(16) if c != 5]].any()
+
+
+FFN = [([1], 64, 32), ([0, 1, 0, 1], 256, 512), ([3, 0, 2, 0, 0, 11], 96, 160), ([16, 1, 0, 15], 288, 416),
+       ([40, 17, 0, 64], 544, 224), ([129, 0, 1, 300, 128], 160, 352), ([1] * 40 + [0] * 24 + [90], 128, 96),
+       ([260, 255], 1024, 1408)]
+
+
+def exact_expert_weights(ms, e, k, n, dev, seed, shift):
+    """[E][N][K] 4-bit weights of two neighbouring scales around 2^-shift, and their values."""
+    code, s, v = held_operand(e * n, k, dev, seed, 1)
+    s = s - shift
+    return ms.Mx4Weights.from_checkpoint(code.view(e, n, -1), s.view(e, n, -1)), (v * 2.0 ** -shift).view(e, n, k)
+
+
+def ffn_reference(x, segs, gate, up, down):
+    """(o, bound on its error).  x, gate and up are such that g and u are exact in 32 bits; silu(g) u
+    then carries the errors of e^-g (2 + 1.173 |g| ulp), a division (2 ulp), a sum and a product."""
+    o, slack = torch.zeros_like(x, dtype=torch.float64), torch.zeros_like(x, dtype=torch.float64)
+    for _, at, n, e in segs.tolist():
+        if n == 0:
+            continue
+        a = ref.held4(x[at:at + n])
+        for w in (gate[e], up[e]):
+            unit = 0.25 * float(2.0 ** (torch.frexp(w.abs().max())[1] - 4))  # scales of two neighbouring powers
+            assert float((a.abs() @ w.abs().T).max()) < 2 ** 24 * unit
+        g, u = a @ gate[e].T, a @ up[e].T
+        h = g * torch.sigmoid(g) * u
+        rel = (6 + 1.2 * float(g.abs().max())) * 2.0 ** -23
+        lo, hi = ref.candidates(h, rel, ref.held4, 2)
+        held = ref.held4(h)
+        o[at:at + n] = held @ down[e].T
+        slack[at:at + n] = (torch.maximum(hi - held, held - lo) @ down[e].abs().T +
+                            h.shape[1] * 2.0 ** -23 * (torch.maximum(lo.abs(), hi.abs()) @ down[e].abs().T))
+    return o, slack
+
+
+@pytest.mark.parametrize("counts,d,f", FFN)
+def test_expert_ffn(ms, cuda_device, counts, d, f):
+    segs, rows = table(counts, cuda_device)
+    e = len(counts)
+    _, _, x = held_operand(rows + 5, d, cuda_device, rows, 1)
+    x = x.to(BF16)
+    assert torch.equal(ref.held4(x), x.double())
+    shift = (d.bit_length() + 7) // 2  # g of a few units
+    qg, gate = exact_expert_weights(ms, e, d, f, cuda_device, 1, shift)
+    qu, up = exact_expert_weights(ms, e, d, f, cuda_device, 2, shift)
+    qd, down = exact_expert_weights(ms, e, f, d, cuda_device, 3, shift)
+    plan = ms.Mx4ExpertFfn(qg, qu, qd, rows=rows + 5, tokens=max(counts))
+    o, slack = ffn_reference(x, segs, gate, up, down)
+    for dt in (FP32, BF16):
+        out = torch.full((rows + 5, d), float("nan"), dtype=dt, device=cuda_device)
+        plan.forward(x, segs, out=out)
+        assert plan.status() == 0
+        half = 0.0 if dt == FP32 else 2.0 ** -8
+        err = (out[:rows].double() - o[:rows]).abs()
+        assert (err <= slack[:rows] + half * (o[:rows].abs() + slack[:rows])).all(), float((err - slack[:rows]).max())
+        assert torch.isnan(out[rows:].float()).all()  # rows behind the last segment are left as they were
+    assert float(slack[:rows].norm()) < 0.02 * float(o.norm())  # the bound says something
+
+
+def layer_weights(ms, axm, cfg, dev, seed=0):
+    """4-bit weights of a layer, and the same layer's values in the engine's layout in bf16."""
+    D, F, E, S = cfg["d"], cfg["f"], cfg["e"], cfg.get("shared", 0)
+    g = generator(dev, seed)
+    q, v = {}, {}
+
+    def draw(*shape):
+        return torch.empty(*shape, device=dev).normal_(0, 0.05, generator=g)
+
+    q["router_w"] = v["router_w"] = draw(D, E)
+    for name, n, (k, m) in [("gate", E, (D, F)), ("up", E, (D, F)), ("down", E, (F, D)), ("shared_gate", S, (D, F)),
+                            ("shared_up", S, (D, F)), ("shared_down", S, (F, D))]:
+        if n:
+            q[name] = ms.quantize_weights(draw(n, k, m))
+            v[name] = ms.dequantize_weights(q[name], FP32).double()
+    return q, v
+
+
+LAYER = [dict(t=1, d=64, f=96, e=4, k=2), dict(t=5, d=256, f=512, e=8, k=2, shared=1), dict(t=64, d=256, f=512, e=8, k=2),
+         dict(t=130, d=96, f=160, e=12, k=4, shared=2), dict(t=700, d=256, f=352, e=64, k=6, shared=2)]
+
+
+@pytest.mark.parametrize("cfg", LAYER, ids=lambda c: "-".join(str(v) for v in c.values()))
+def test_layer(ms, axm, cuda_device, cfg):
+    """The layer's output from its own routing (whose exactness the layer's other tests show): the
+    chosen experts' feed-forwards by the stage's own call, combined in 64 bits."""
+    q, _ = layer_weights(ms, axm, cfg, cuda_device)
+    T, D, E, k, S = cfg["t"], cfg["d"], cfg["e"], cfg["k"], cfg.get("shared", 0)
+    x = torch.empty(T, D, device=cuda_device).normal_(generator=generator(cuda_device, 9)).to(BF16)
+    layer = ms.Mx4MoeLayer(q, T, k)
+    out, hist = layer.forward(x)
+    assert layer.status() == 0
+    idx, gate = layer.topk_idx.long(), layer.topk_gate.double()
+    assert torch.equal(hist.long(), torch.bincount(idx.reshape(-1), minlength=E))
+    logits = x.double() @ q["router_w"].double()
+    assert torch.equal(logits.gather(1, idx).sum(1) >= logits.topk(k).values.sum(1) - 1e-3, torch.ones(T, dtype=torch.bool, device=cuda_device))
+
+    def stage(w, counts, rows):
+        segs, n = table(counts, cuda_device)
+        plan = ms.Mx4ExpertFfn(*w, rows=n, tokens=T)
+        return plan.forward(rows, segs, dtype=FP32).double()
+
+    order = torch.argsort(idx.reshape(-1), stable=True)
+    o = torch.empty(T * k, D, dtype=torch.float64, device=cuda_device)
+    o[order] = stage((q["gate"], q["up"], q["down"]), hist.tolist(), x[order // k].contiguous())
+    y = (o.view(T, k, D) * gate.unsqueeze(-1)).sum(1)
+    size = (o.view(T, k, D) * gate.unsqueeze(-1)).abs().sum(1)
+    for i in range(S):
+        one = [ms.Mx4Weights.from_checkpoint(q[n].codes[i:i + 1].contiguous(), ref.scale_bytes(
+            ms.dequantize_weights(q[n], FP32)[i].T, 2).unsqueeze(0)) for n in ("shared_gate", "shared_up", "shared_down")]
+        add = stage(one, [T], x)
+        y, size = y + add, size + add.abs()
+    # y in 32 bits (k + S products and sums), rounded to bf16, then x + y rounded again
+    bound = (k + S + 1) * 2.0 ** -23 * size + 2.0 ** -8 * (y.abs() + size * 2.0 ** -20) + 2.0 ** -8 * ((x.double() + y).abs() + 2.0 ** -8 * y.abs()) + 1e-30
+    assert ((out.double() - (x.double() + y)).abs() <= bound).all()
+    # in place, without the residual, and accumulating the histogram
+    z = x.clone()
+    layer.forward(z, out=z)
+    assert torch.equal(z, out)
+
+
+def test_captured_calls_and_streams(ms, axm, cuda_device):
+    """A captured call replays with new inputs; another stream gives the same bits; two objects'
+    workspaces do not meet."""
+    cfg = dict(t=33, d=256, f=160, e=8, k=2)
+    q, _ = layer_weights(ms, axm, cfg, cuda_device)
+    x = [torch.empty(33, 256, device=cuda_device).normal_(generator=generator(cuda_device, i)).to(BF16) for i in range(2)]
+    a, b = ms.Mx4MoeLayer(q, 33, 2), ms.Mx4MoeLayer(q, 33, 2)
+    want = [a.forward(v)[0].clone() for v in x]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [b.forward(v)[0] for v in x]
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, r) for p, r in zip(want, got))
+    held, out = x[0].clone(), torch.empty_like(x[0])
+    lin = ms.Mx4Linear(ms.quantize_weights(torch.randn(1, 256, 72, device=cuda_device)), 33)
+    y = torch.empty(33, 72, dtype=BF16, device=cuda_device)
+    want_y = [lin.forward(v).clone() for v in x]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.forward(held, out=out)
+        lin.forward(held, out=y)
+    for v, w, wy in list(zip(x, want, want_y)) * 2:
+        held.copy_(v)
+        out.zero_()
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, w) and torch.equal(y, wy)
+
+
+def test_same_bits_again(ms, cuda_device):
+    """A call gives the same bits every time."""
+    w = ms.quantize_weights(torch.randn(1, 1056, 520, device=cuda_device))
+    for t in (1, 7, 300):
+        x = torch.randn(t, 1056, device=cuda_device).to(BF16)
+        plan = ms.Mx4Linear(w, t)
+        first = plan.forward(x, dtype=FP32).clone()
+        assert all(torch.equal(first, plan.forward(x, dtype=FP32)) for _ in range(5))
