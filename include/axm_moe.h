@@ -700,6 +700,40 @@ AXM_API int axm_moe_forward_mx4(const AxmMoeDesc* desc, const AxmMoeTensors* ten
                                 const AxmMx4Experts* experts, const AxmMx4Experts* shared, void* workspace,
                                 size_t workspace_bytes, void* stream);
 
+/* What the expert feed-forward's training step keeps between its two passes when it keeps it in
+ * 8 bits: the gate's and the up projection's outputs, [rows][F] e4m3 codes and [rows][F/32] scale
+ * bytes each (axm_mx8_checkpoint_bytes).  2 F (1 + 1/32) bytes a row where the bf16 form
+ * (axm_moe_expert_ffn_backward) keeps g, u and h: 6 F. */
+typedef struct AxmMx8Checkpoint {
+  void* gate_codes;
+  void* gate_scales;
+  void* up_codes;
+  void* up_scales;
+} AxmMx8Checkpoint;
+AXM_API int axm_mx8_checkpoint_bytes(int32_t rows, int32_t d_ff, size_t* code_bytes, size_t* scale_bytes);
+
+/* Forward: g = x . Wg[e], u = x . Wu[e], o = bf16(silu(g) u) . Wd[e] over the segments' rows, weights
+ * in the engine's layouts (bf16); g and u are kept as q8(g), q8(u).  h [rows][F] bf16 is scratch of
+ * this call, o [rows][D] bf16 or fp32.
+ * Backward, from d_o [rows][D] bf16 and the kept g^, u^, with s = sigmoid(g^):
+ *   dH = d_o . Wd[e]^T, dG = dH u^ s (1 + g^ (1 - s)), dU = dH g^ s, h^ = g^ s u^      (bf16)
+ *   d_x = dG . Wg[e]^T + dU . Wu[e]^T, dWd[e] = h^T d_o, dWg[e] = x^T dG, dWu[e] = x^T dU
+ * Gradients are bf16 or fp32 (grad_dtype, all of them alike), in the layouts of what they belong to;
+ * the three weight gradients may all be NULL.  h, d_g, d_u [rows][F] bf16 are scratch of the call.
+ * Tables as for axm_moe_expert_ffn_backward: a_row0 == out_row0, every expert once, segments
+ * padded to multiples of 64 rows with zero rows of x and d_o.  d_ff is a multiple of 32, d_model of 8.
+ * status: an optional int32 device word that receives a non-zero code when a bounded wait gave up. */
+AXM_API int axm_mx8_expert_ffn_train(const AxmMoeDesc* desc, const void* x, int32_t rows,
+                                     const AxmSegment* segments, int32_t num_segments, const void* w_gate,
+                                     const void* w_up, const void* w_down, const AxmMx8Checkpoint* keep,
+                                     void* h, void* o, int32_t o_dtype, int32_t* status, void* stream);
+AXM_API int axm_mx8_expert_ffn_backward(const AxmMoeDesc* desc, const void* x, int32_t rows,
+                                        const AxmSegment* segments, int32_t num_segments,
+                                        const AxmMx8Checkpoint* keep, const void* d_o, const void* w_gate,
+                                        const void* w_up, const void* w_down, void* h, void* d_g, void* d_u,
+                                        void* d_x, void* d_w_gate, void* d_w_up, void* d_w_down,
+                                        int32_t grad_dtype, int32_t* status, void* stream);
+
 /* Number of token blocks the router splits T into (rows of block_counts). */
 #define AXM_ROUTE_BLOCKS 296
 

@@ -88,6 +88,10 @@ class Mx4ExpertWeights(ctypes.Structure):
                                                "down_codes", "down_scales")]
 
 
+class Mx8Checkpoint(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("gate_codes", "gate_scales", "up_codes", "up_scales")]
+
+
 class Segment(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("a_row0", "out_row0", "rows", "expert")]
 
@@ -178,6 +182,10 @@ def load():
     lib.axm_mx4_expert_ffn.argtypes = [dp, vp, i32, vp, i32, mp, vp, i32, vp, sz, vp]
     lib.axm_moe_mx4_workspace_bytes.argtypes = [dp, szp]
     lib.axm_moe_forward_mx4.argtypes = [dp, ctypes.POINTER(MoeTensors), mp, mp, vp, sz, vp]
+    kp = ctypes.POINTER(Mx8Checkpoint)
+    lib.axm_mx8_checkpoint_bytes.argtypes = [i32, i32, szp, szp]
+    lib.axm_mx8_expert_ffn_train.argtypes = [dp, vp, i32, vp, i32, vp, vp, vp, kp, vp, vp, i32, vp, vp]
+    lib.axm_mx8_expert_ffn_backward.argtypes = [dp, vp, i32, vp, i32, kp] + [vp] * 11 + [i32, vp, vp]
     _lib = lib
     return lib
 

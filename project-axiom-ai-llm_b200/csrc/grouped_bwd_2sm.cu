@@ -65,6 +65,9 @@ __device__ __forceinline__ WgradUnit decode_wgrad(int unit, int pairs_w, int n_t
   return u;
 }
 
+// kBf16: the gradient leaves as bf16 (rounded once from the fp32 accumulator): half the bytes of
+// the largest outputs of a training step.
+template <bool kBf16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                          const __grid_constant__ CUtensorMap tm_out, Wgrad2Args args) {
@@ -234,10 +237,22 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
           if (lane == 0) bulk_wait_read();  // the previous block's store has read the buffer
           __syncwarp();
           if (n0 + c0 < args.n_total && block_row0 < args.m_total) {
+            if constexpr (kBf16) {  // rows of 64 bytes, the 64-byte swizzle of the bf16 output map
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              *reinterpret_cast<uint4*>(stage_w + lane * 128 + ((q ^ (lane & 7)) << 4)) =
-                  make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+              for (int q = 0; q < 4; ++q) {
+                uint32_t w4[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  w4[j] = pack_bf16(__uint_as_float(v[8 * q + 2 * j]), __uint_as_float(v[8 * q + 2 * j + 1]));
+                *reinterpret_cast<uint4*>(stage_w + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
+                    make_uint4(w4[0], w4[1], w4[2], w4[3]);
+              }
+            } else {
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                *reinterpret_cast<uint4*>(stage_w + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+                    make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
@@ -283,14 +298,12 @@ int map_kbox(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols) {
 
 }  // namespace
 
-// dW[e] = A^T . B over each segment's rows: A [rows_total][m_total], B [rows_total][n_total]
-// (bf16), dW [experts][m_total][n_total] fp32.  AXM_ERR_DEVICE when pairs cannot be
-// scheduled, so that the caller can fall back to the one-SM kernel.
-int launch_wgrad_2sm(const AxmSegment* segments, int32_t num_segments, int32_t rows_total, int32_t experts,
-                     const void* a, int32_t m_total, const void* b, int32_t n_total, void* d_w,
-                     int32_t* status, cudaStream_t st) {
+template <bool kBf16>
+static int launch_wgrad_as(const AxmSegment* segments, int32_t num_segments, int32_t rows_total, int32_t experts,
+                           const void* a, int32_t m_total, const void* b, int32_t n_total, void* d_w, int32_t* status,
+                           cudaStream_t st) {
   static SmemLimitCache smem = {};
-  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(grouped_wgrad_2sm_kernel), kWgrad2SmemBytes,
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(grouped_wgrad_2sm_kernel<kBf16>), kWgrad2SmemBytes,
                                    &smem, "grouped_wgrad_2sm_kernel"))
     return rc;
   const int grid = grid_2sm();
@@ -301,17 +314,32 @@ int launch_wgrad_2sm(const AxmSegment* segments, int32_t num_segments, int32_t r
   if ((rc = map_kbox(&ma, a, (uint64_t)rows_total, (uint64_t)m_total))) return rc;
   if ((rc = map_kbox(&mb, b, (uint64_t)rows_total, (uint64_t)n_total))) return rc;
   const uint64_t dims[3] = {(uint64_t)n_total, (uint64_t)m_total, (uint64_t)experts};
-  const uint64_t strides[2] = {(uint64_t)n_total * 4, (uint64_t)n_total * (uint64_t)m_total * 4};
+  const uint64_t size = kBf16 ? 2 : 4;
+  const uint64_t strides[2] = {(uint64_t)n_total * size, (uint64_t)n_total * (uint64_t)m_total * size};
   const uint32_t box[3] = {32, 32, 1};
-  if ((rc = encode_tensor_map_f32(&mo, d_w, 3, dims, strides, box))) return rc;
+  if constexpr (kBf16) {
+    if ((rc = encode_tensor_map_sw64(&mo, d_w, 3, dims, strides, box))) return rc;
+  } else {
+    if ((rc = encode_tensor_map_f32(&mo, d_w, 3, dims, strides, box))) return rc;
+  }
   Wgrad2Args wa;
   wa.segments = segments;
   wa.num_segments = num_segments;
   wa.m_total = m_total;
   wa.n_total = n_total;
   wa.status = status;
-  grouped_wgrad_2sm_kernel<<<grid, kGemmThreads, kWgrad2SmemBytes, st>>>(ma, mb, mo, wa);
+  grouped_wgrad_2sm_kernel<kBf16><<<grid, kGemmThreads, kWgrad2SmemBytes, st>>>(ma, mb, mo, wa);
   return check_launch("grouped_wgrad_2sm_kernel");
+}
+
+// dW[e] = A^T . B over each segment's rows: A [rows_total][m_total], B [rows_total][n_total]
+// (bf16), dW [experts][m_total][n_total] fp32 or bf16.  AXM_ERR_DEVICE when pairs cannot be
+// scheduled, so that the caller can fall back to the one-SM kernel.
+int launch_wgrad_2sm(const AxmSegment* segments, int32_t num_segments, int32_t rows_total, int32_t experts,
+                     const void* a, int32_t m_total, const void* b, int32_t n_total, void* d_w,
+                     int32_t* status, cudaStream_t st, bool out_bf16) {
+  return out_bf16 ? launch_wgrad_as<true>(segments, num_segments, rows_total, experts, a, m_total, b, n_total, d_w, status, st)
+                  : launch_wgrad_as<false>(segments, num_segments, rows_total, experts, a, m_total, b, n_total, d_w, status, st);
 }
 
 }  // namespace axm

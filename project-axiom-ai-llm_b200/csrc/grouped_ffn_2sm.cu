@@ -24,10 +24,15 @@
 #include <mutex>
 
 #include "gemm_2sm.cuh"
+#include "microscale.cuh"
 
 namespace axm {
 
-enum { kModeDown = 0, kModeSwiGLU = 1, kModeDX = 2, kModeDH = 3 };
+// kModeSwiGLU8 / kModeDH8: the training step that keeps g and u in 8 bits (microscale.cuh): the
+// forward epilogue quantises them where it would store bf16, the backward epilogue reads them,
+// and also writes h = silu(g) u of what it read, which the weight gradient of the down
+// projection multiplies (so h is not kept either).
+enum { kModeDown = 0, kModeSwiGLU = 1, kModeDX = 2, kModeDH = 3, kModeSwiGLU8 = 4, kModeDH8 = 5 };
 
 struct Gemm2Args {
   const AxmSegment* segments;
@@ -54,10 +59,19 @@ struct Gemm2Args {
   // them in range order).  1: the whole reduction in one unit, stored at out.
   int k_splits;
   long long split_stride;
+  int out_bf16;  // kModeDown, kModeDX: bf16 rows instead of fp32
+  // kModeSwiGLU8 (written) and kModeDH8 (read): e4m3 codes [rows][F], scale bytes [rows][F / 32]
+  uint8_t* codes_g;
+  uint8_t* codes_u;
+  uint8_t* scales_g;
+  uint8_t* scales_u;
+  void* out2;    // kModeDH8: h
 };
 
 constexpr int kStagesDh = 5;  // operand stages of kModeDH (one stage's room goes to its epilogue blocks)
 constexpr int kDhSlots = 3;   // 4 KiB slots (g / dG block + u / dU block) per epilogue warp
+constexpr int kDh8Slots = 2;  // kModeDH8: 6 KiB slots (dG, dU and h blocks; nothing comes in through them)
+static_assert(kDh8Slots * 6144 == kDhSlots * 4096, "both forms use the same room");
 
 // fp32 accumulate, bf16 A (K-major) and B (MN-major), N = 256, M = 256 over the pair
 constexpr uint32_t kInstrDesc2 = (1u << 4) | (1u << 7) | (1u << 10) | (0u << 15) | (1u << 16) |
@@ -114,6 +128,23 @@ __device__ __forceinline__ UnitCoord decode_unit(const GemmShared2* sh, int n_ti
   return uc;
 }
 
+// Quantises a row's 32 fp32 values to 8 bits, stores the codes, returns the scale byte.
+__device__ __forceinline__ uint32_t store_block8(const uint32_t (&v)[32], uint8_t* codes) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) top = max(top, v[j] & 0x7fffffffu);
+  const uint32_t s = mx_scale_byte<8>(top);
+  const float inv = mx_inverse_scale(s);
+  uint32_t c[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    c[j] = mx8_pack4(__uint_as_float(v[4 * j]) * inv, __uint_as_float(v[4 * j + 1]) * inv,
+                     __uint_as_float(v[4 * j + 2]) * inv, __uint_as_float(v[4 * j + 3]) * inv);
+  __stcs(reinterpret_cast<uint4*>(codes), make_uint4(c[0], c[1], c[2], c[3]));
+  __stcs(reinterpret_cast<uint4*>(codes) + 1, make_uint4(c[4], c[5], c[6], c[7]));
+  return s;
+}
+
 template <int kMode>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a_alt,
@@ -122,9 +153,11 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
                         const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ CUtensorMap tm_u,
                         const __grid_constant__ CUtensorMap tm_dg, const __grid_constant__ CUtensorMap tm_du,
                         Gemm2Args args) {
-  constexpr bool kSwiGLU = kMode == kModeSwiGLU;
+  constexpr bool kSave8 = kMode == kModeSwiGLU8;
+  constexpr bool kRead8 = kMode == kModeDH8;
+  constexpr bool kSwiGLU = kMode == kModeSwiGLU || kSave8;
   constexpr bool kDX = kMode == kModeDX;
-  constexpr bool kDH = kMode == kModeDH;
+  constexpr bool kDH = kMode == kModeDH || kRead8;
   constexpr bool kBKmajor = kDX || kDH;  // weights read K-major: one box of 64 k x 128 columns per CTA
   // kModeDH gives one operand stage to the epilogue's g / u / dG / dU blocks
   constexpr int kSt = kDH ? kStagesDh : kStages2;
@@ -357,7 +390,7 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
         tma_load_2d(dst + 2048, &tm_u, bar, dh_n0 + jb * 32, dh_row0);
         ++dh_issued;
       };
-      if constexpr (kDH) {
+      if constexpr (kDH && !kRead8) {
         if (dh_full && lane == 0) {
           bulk_wait_read();  // the previous tile's last stores have read their slots
           if (dh_valid(0)) dh_issue(0);
@@ -373,7 +406,94 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
       const size_t out_elem = (size_t)(sg.out_row0 + (row_ok ? row_in_seg : 0)) * args.n_total + n0 +
                               (k_splits > 1 ? (size_t)(uc.n_tile % k_splits) * (size_t)args.split_stride : 0);
       const uint32_t t_addr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)acc * UMMA_N;
-      if constexpr (kDH) {
+      if constexpr (kRead8) {
+        // The same derivative from g and u in 8 bits.  A lane reads its own row: 32 codes of each
+        // (two 16-byte pieces, a whole sector) and a scale byte a block, one block ahead of their
+        // use.  dG, dU and h leave as in the bf16 form, through two slots of three blocks.
+        unsigned char* slots = staging + (size_t)((warp - 2) & 3) * kDh8Slots * 6144;
+        auto piece_smem = [&](int row, int piece) { return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); };
+        const bool mine = lane < dh_rows_left;
+        const size_t row_at = (size_t)(dh_row0 + (mine ? lane : 0));
+        uint4 gc[2] = {}, uc8[2] = {};
+        uint32_t gs = 0, us = 0;
+        auto fetch = [&](int jb) {
+          if (!mine || !dh_valid(jb)) return;
+          const size_t el = row_at * args.n_total + dh_n0 + jb * 32;
+          const size_t sc = row_at * (args.n_total >> 5) + (dh_n0 >> 5) + jb;
+          gc[0] = __ldg(reinterpret_cast<const uint4*>(args.codes_g + el));
+          gc[1] = __ldg(reinterpret_cast<const uint4*>(args.codes_g + el) + 1);
+          uc8[0] = __ldg(reinterpret_cast<const uint4*>(args.codes_u + el));
+          uc8[1] = __ldg(reinterpret_cast<const uint4*>(args.codes_u + el) + 1);
+          gs = __ldg(args.scales_g + sc);
+          us = __ldg(args.scales_u + sc);
+        };
+        fetch(0);
+#pragma unroll 1
+        for (int jb = 0; jb < BN_OUT / 32; ++jb) {
+          if (!dh_valid(jb)) break;
+          unsigned char* dg_s = slots + (size_t)(dh_used % kDh8Slots) * 6144;
+          const int c0 = jb * 32;
+          uint32_t v[32];
+          __syncwarp();
+          tmem_ld32(t_addr + c0, v);
+          const uint32_t gw[8] = {gc[0].x, gc[0].y, gc[0].z, gc[0].w, gc[1].x, gc[1].y, gc[1].z, gc[1].w};
+          const uint32_t uw[8] = {uc8[0].x, uc8[0].y, uc8[0].z, uc8[0].w, uc8[1].x, uc8[1].y, uc8[1].z, uc8[1].w};
+          const float g_scale = mx_scale_value(gs), u_scale = mx_scale_value(us);
+          fetch(jb + 1);
+          tmem_ld_wait();
+          if (dh_full && lane == 0) bulk_wait_read_but_one();  // this slot's stores, a block before the last ones
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t dgw[4], duw[4], hw[4];
+#pragma unroll
+            for (int pp = 0; pp < 4; ++pp) {
+              const int i = q * 8 + pp * 2;  // elements i, i + 1 of the block
+              const uint32_t sh16 = (pp & 1) * 16;
+              const float2 gf = mx8_unpack2((gw[i >> 2] >> sh16) & 0xffffu);
+              const float2 uf = mx8_unpack2((uw[i >> 2] >> sh16) & 0xffffu);
+              float r0[2], r1[2], r2[2];
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                const float gval = (hh ? gf.y : gf.x) * g_scale;
+                const float uval = (hh ? uf.y : uf.x) * u_scale;
+                const float dh = __uint_as_float(v[i + hh]);
+                const float sg_ = __fdividef(1.0f, 1.0f + __expf(-gval));
+                const float silu = gval * sg_;
+                r0[hh] = dh * uval * (sg_ + silu * (1.0f - sg_));  // dG
+                r1[hh] = dh * silu;                                // dU
+                r2[hh] = silu * uval;                              // h
+              }
+              dgw[pp] = pack_bf16(r0[0], r0[1]);
+              duw[pp] = pack_bf16(r1[0], r1[1]);
+              hw[pp] = pack_bf16(r2[0], r2[1]);
+            }
+            const uint4 dgv = make_uint4(dgw[0], dgw[1], dgw[2], dgw[3]), duv = make_uint4(duw[0], duw[1], duw[2], duw[3]),
+                        hv = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+            if (dh_full) {
+              *reinterpret_cast<uint4*>(dg_s + piece_smem(lane, q)) = dgv;
+              *reinterpret_cast<uint4*>(dg_s + 2048 + piece_smem(lane, q)) = duv;
+              *reinterpret_cast<uint4*>(dg_s + 4096 + piece_smem(lane, q)) = hv;
+            } else if (mine) {
+              const size_t el = row_at * args.n_total + n0 + c0 + q * 8;
+              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(args.out) + el) = dgv;
+              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(args.out1) + el) = duv;
+              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(args.out2) + el) = hv;
+            }
+          }
+          if (dh_full) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tm_dg, dg_s, n0 + c0, dh_row0);
+              tma_store_2d(&tm_du, dg_s + 2048, n0 + c0, dh_row0);
+              tma_store_2d(&tm_g, dg_s + 4096, n0 + c0, dh_row0);  // the map of h
+              bulk_commit_group();
+            }
+            ++dh_used;
+          }
+        }
+      } else if constexpr (kDH) {
         // The SwiGLU derivative with the saved g, u: dG = dH u s (1 + g (1 - s)), dU = dH g s,
         // s = sigmoid(g) (core/src/CUDA/kernel/swiglu.cu:34-55 of the reference engine).
         // g and u come in, and dG and dU go out, as 32 x 32 bf16 blocks moved by TMA (64-byte
@@ -500,7 +620,13 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
                            make_uint4(packed_lo[4 * q], packed_lo[4 * q + 1], packed_lo[4 * q + 2],
                                       packed_lo[4 * q + 3]));
                 }
-              if (args.save_g != nullptr) {
+              if constexpr (kSave8) {
+                if (n0 + c0 < args.n_total) {  // F is a multiple of 32
+                  const size_t sc = (size_t)(sg.out_row0 + row_in_seg) * (args.n_total >> 5) + ((n0 + c0) >> 5);
+                  args.scales_g[sc] = (uint8_t)store_block8(g, args.codes_g + out_elem + c0);
+                  args.scales_u[sc] = (uint8_t)store_block8(u, args.codes_u + out_elem + c0);
+                }
+              } else if (args.save_g != nullptr) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                   if (n0 + c0 + q * 8 < args.n_total) {
@@ -520,7 +646,18 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
             }
           } else {
             tmem_ld_wait();
-            if (row_ok) {
+            if (row_ok && args.out_bf16) {
+              __nv_bfloat16* out_row = static_cast<__nv_bfloat16*>(args.out) + out_elem;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (n0 + c0 + q * 8 < args.n_total) {
+                  uint32_t w4[4];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    w4[j] = pack_bf16(__uint_as_float(g[8 * q + 2 * j]), __uint_as_float(g[8 * q + 2 * j + 1]));
+                  __stcs(reinterpret_cast<uint4*>(out_row + c0 + q * 8), make_uint4(w4[0], w4[1], w4[2], w4[3]));
+                }
+            } else if (row_ok) {
               float* out_row = static_cast<float*>(args.out) + out_elem;
 #pragma unroll
               for (int q = 0; q < 8; ++q)
@@ -682,7 +819,7 @@ int launch_expert_ffn_2sm(const AxmMoeDesc* d, const void* x_perm, int32_t a_row
   if ((rc = map2_rows(&a2, h, rows_total, F, h_ld))) return rc;
   a2_lo = a2;
   if (exact && (rc = map2_rows(&a2_lo, static_cast<const __nv_bfloat16*>(h) + F, rows_total, F, h_ld))) return rc;
-  Gemm2Args ga;
+  Gemm2Args ga = {};
   ga.h_ld = (int)h_ld;
   ga.lo_off = exact ? F : 0;
   ga.two_term = 0;
@@ -777,7 +914,7 @@ int launch_bwd_dh_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t n
     if ((rc = encode_tensor_map_sw64(&m_dg, d_g, 2, dims, strides, box))) return rc;
     if ((rc = encode_tensor_map_sw64(&m_du, d_u, 2, dims, strides, box))) return rc;
   }
-  Gemm2Args ga;
+  Gemm2Args ga = {};
   ga.segments = segments;
   ga.num_segments = num_segments;
   ga.routed_experts = E;
@@ -802,7 +939,7 @@ int launch_bwd_dh_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t n
 // Returns AXM_ERR_DEVICE when pairs cannot be scheduled, so that the caller can fall back.
 int launch_bwd_dx_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t num_segments,
                       int32_t rows_total, const void* d_g, const void* d_u, const void* w_gate,
-                      const void* w_up, void* d_xp, int32_t* status, cudaStream_t st) {
+                      const void* w_up, void* d_xp, int32_t* status, cudaStream_t st, bool out_bf16) {
   static SmemLimitCache smem_dx = {};
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(grouped_gemm_2sm_kernel<kModeDX>), kGemm2SmemBytes,
                                    &smem_dx, "grouped_gemm_2sm_kernel<dX>"))
@@ -817,7 +954,7 @@ int launch_bwd_dx_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t n
   if ((rc = map2_rows(&m_du, d_u, (uint64_t)rows_total, F))) return rc;
   if ((rc = map2_weights_kmajor(&m_wg, w_gate, E, D, F))) return rc;
   if ((rc = map2_weights_kmajor(&m_wu, w_up, E, D, F))) return rc;
-  Gemm2Args ga;
+  Gemm2Args ga = {};
   ga.segments = segments;
   ga.num_segments = num_segments;
   ga.routed_experts = E;
@@ -825,6 +962,7 @@ int launch_bwd_dx_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t n
   ga.n_total = D;
   ga.k_total = F;
   ga.out = d_xp;
+  ga.out_bf16 = out_bf16 ? 1 : 0;
   ga.save_g = nullptr;
   ga.save_u = nullptr;
   ga.out1 = nullptr;
@@ -836,6 +974,96 @@ int launch_bwd_dx_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t n
   grouped_gemm_2sm_kernel<kModeDX><<<grid, kGemmThreads, kGemm2SmemBytes, st>>>(m_dg, m_du, m_wg, m_wu, m_wg,
                                                                                 m_wu, m_dg, m_dg, m_dg, m_dg, ga);
   return check_launch("grouped_gemm_2sm_kernel<dX>");
+}
+
+// The training step with g and u kept in 8 bits (host side: mx8_train.cu).  Forward: h (bf16, this
+// call's scratch), o, and the kept codes and scale bytes.
+int launch_train8_forward(const AxmMoeDesc* d, const AxmSegment* segments, int32_t num_segments, int32_t rows_total,
+                          const void* x_perm, const void* w_gate, const void* w_up, const void* w_down,
+                          const AxmMx8Checkpoint* keep, void* h, void* o, bool o_bf16, int32_t* status,
+                          cudaStream_t st) {
+  static SmemLimitCache smem = {};
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(grouped_gemm_2sm_kernel<kModeSwiGLU8>), kGemm2SmemBytes,
+                                   &smem, "grouped_gemm_2sm_kernel<SwiGLU, 8 bits>"))
+    return rc;
+  const int grid = grid_2sm();
+  if (grid < 0) return grid;
+  if (grid < 2) return fail(AXM_ERR_DEVICE, "two-SM clusters cannot be scheduled on this device");
+  const int D = d->d_model, F = d->d_ff, E = d->num_experts;
+  CUtensorMap a1, g, u, a2, dn;
+  int rc;
+  if ((rc = map2_rows(&a1, x_perm, rows_total, D))) return rc;
+  if ((rc = map2_weights(&g, w_gate, E, D, F))) return rc;
+  if ((rc = map2_weights(&u, w_up, E, D, F))) return rc;
+  if ((rc = map2_rows(&a2, h, rows_total, F))) return rc;
+  if ((rc = map2_weights(&dn, w_down, E, F, D))) return rc;
+  Gemm2Args ga = {};
+  ga.segments = segments;
+  ga.num_segments = num_segments;
+  ga.routed_experts = E;
+  ga.status = status;
+  ga.k_splits = 1;
+  ga.n_total = F;
+  ga.k_total = D;
+  ga.out = h;
+  ga.h_ld = F;
+  ga.codes_g = static_cast<uint8_t*>(keep->gate_codes);
+  ga.codes_u = static_cast<uint8_t*>(keep->up_codes);
+  ga.scales_g = static_cast<uint8_t*>(keep->gate_scales);
+  ga.scales_u = static_cast<uint8_t*>(keep->up_scales);
+  grouped_gemm_2sm_kernel<kModeSwiGLU8><<<grid, kGemmThreads, kGemm2SmemBytes, st>>>(a1, a1, g, u, g, u, a1, a1, a1, a1,
+                                                                                     ga);
+  if ((rc = check_launch("grouped_gemm_2sm_kernel<swiglu, 8 bits>"))) return rc;
+  ga.n_total = D;
+  ga.k_total = F;
+  ga.out = o;
+  ga.out_bf16 = o_bf16 ? 1 : 0;
+  grouped_gemm_2sm_kernel<kModeDown><<<grid, kGemmThreads, kGemm2SmemBytes, st>>>(a2, a2, dn, dn, dn, dn, a2, a2, a2, a2,
+                                                                                  ga);
+  return check_launch("grouped_gemm_2sm_kernel<down>");
+}
+
+// Backward of the same: dG, dU and h (bf16, this call's scratch) from the kept codes.
+int launch_train8_dh(const AxmMoeDesc* d, const AxmSegment* segments, int32_t num_segments, int32_t rows_total,
+                     const void* d_o, const void* w_down, const AxmMx8Checkpoint* keep, void* d_g, void* d_u, void* h,
+                     int32_t* status, cudaStream_t st) {
+  static SmemLimitCache smem = {};
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(grouped_gemm_2sm_kernel<kModeDH8>), kGemm2DhSmemBytes,
+                                   &smem, "grouped_gemm_2sm_kernel<dH, 8 bits>"))
+    return rc;
+  const int grid = grid_2sm();
+  if (grid < 0) return grid;
+  if (grid < 2) return fail(AXM_ERR_DEVICE, "two-SM clusters cannot be scheduled on this device");
+  const int D = d->d_model, F = d->d_ff, E = d->num_experts;
+  CUtensorMap m_do, m_wd, m_h, m_dg, m_du;
+  int rc;
+  if ((rc = map2_rows(&m_do, d_o, (uint64_t)rows_total, D))) return rc;
+  if ((rc = map2_weights_kmajor(&m_wd, w_down, E, F, D))) return rc;
+  const uint64_t dims[2] = {(uint64_t)F, (uint64_t)rows_total};
+  const uint64_t strides[1] = {(uint64_t)F * 2};
+  const uint32_t box[2] = {32, 32};
+  if ((rc = encode_tensor_map_sw64(&m_h, h, 2, dims, strides, box))) return rc;
+  if ((rc = encode_tensor_map_sw64(&m_dg, d_g, 2, dims, strides, box))) return rc;
+  if ((rc = encode_tensor_map_sw64(&m_du, d_u, 2, dims, strides, box))) return rc;
+  Gemm2Args ga = {};
+  ga.segments = segments;
+  ga.num_segments = num_segments;
+  ga.routed_experts = E;
+  ga.status = status;
+  ga.k_splits = 1;
+  ga.n_total = F;
+  ga.k_total = D;
+  ga.out = d_g;
+  ga.out1 = d_u;
+  ga.out2 = h;
+  ga.h_ld = F;
+  ga.codes_g = static_cast<uint8_t*>(keep->gate_codes);
+  ga.codes_u = static_cast<uint8_t*>(keep->up_codes);
+  ga.scales_g = static_cast<uint8_t*>(keep->gate_scales);
+  ga.scales_u = static_cast<uint8_t*>(keep->up_scales);
+  grouped_gemm_2sm_kernel<kModeDH8><<<grid, kGemmThreads, kGemm2DhSmemBytes, st>>>(m_do, m_do, m_wd, m_wd, m_wd, m_wd,
+                                                                                   m_h, m_h, m_dg, m_du, ga);
+  return check_launch("grouped_gemm_2sm_kernel<dH, 8 bits>");
 }
 
 }  // namespace axm

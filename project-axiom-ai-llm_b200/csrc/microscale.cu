@@ -403,12 +403,12 @@ extern "C" int axm_mx4_quantize_rows(const void* x, int32_t x_dtype, int64_t ld,
   const char* what = "axm_mx4_quantize_rows";
   if (int rc = check_rows(rows, k, num_segments, what)) return rc;
   if (int rc = check_dtype(x_dtype, what)) return rc;
+  if (rows == 0) return AXM_OK;  // matrices without rows may have no address
   if (!x || !codes || !scales) return fail(AXM_ERR_ARGUMENT, "%s: null pointer", what);
   if (segments != nullptr && num_segments == 0) return fail(AXM_ERR_ARGUMENT, "%s: an empty segment table", what);
   if (row_src != nullptr && row_div <= 0) return fail(AXM_ERR_ARGUMENT, "%s: row_div %d must be positive", what, row_div);
   if (int rc = check_matrix(x, x_dtype, ld, k, what)) return rc;
   if (misaligned(codes, 16) || misaligned(scales, 16)) return fail(AXM_ERR_ARGUMENT, "%s: codes and scales must be 16-byte aligned", what);
-  if (rows == 0) return AXM_OK;
   if (int rc = require_device()) return rc;
   const Mx4Gather from = {row_src, row_div, rows, 1};
   return launch_quantize_rows<4>(x, x_dtype, ld, from, rows, k, segments, num_segments, codes, scales,
@@ -421,11 +421,11 @@ extern "C" int axm_mx4_dequantize_rows(const void* codes, const void* scales, in
   const char* what = "axm_mx4_dequantize_rows";
   if (int rc = check_rows(rows, k, num_segments, what)) return rc;
   if (int rc = check_dtype(out_dtype, what)) return rc;
+  if (rows == 0) return AXM_OK;  // matrices without rows may have no address
   if (!codes || !scales || !out) return fail(AXM_ERR_ARGUMENT, "%s: null pointer", what);
   if (segments != nullptr && num_segments == 0) return fail(AXM_ERR_ARGUMENT, "%s: an empty segment table", what);
   if (int rc = check_matrix(out, out_dtype, ld, k, what)) return rc;
   if (misaligned(codes, 16) || misaligned(scales, 16)) return fail(AXM_ERR_ARGUMENT, "%s: codes and scales must be 16-byte aligned", what);
-  if (rows == 0) return AXM_OK;
   if (int rc = require_device()) return rc;
   return launch_dequantize_rows<4>(codes, scales, rows, k, segments, num_segments, out, out_dtype, ld,
                                    static_cast<cudaStream_t>(stream));
@@ -436,10 +436,10 @@ extern "C" int axm_mx8_quantize_rows(const void* x, int32_t x_dtype, int64_t ld,
   const char* what = "axm_mx8_quantize_rows";
   if (int rc = check_rows(rows, k, 0, what)) return rc;
   if (int rc = check_dtype(x_dtype, what)) return rc;
+  if (rows == 0) return AXM_OK;  // matrices without rows may have no address
   if (!x || !codes || !scales) return fail(AXM_ERR_ARGUMENT, "%s: null pointer", what);
   if (int rc = check_matrix(x, x_dtype, ld, k, what)) return rc;
   if (misaligned(codes, 16)) return fail(AXM_ERR_ARGUMENT, "%s: codes must be 16-byte aligned", what);
-  if (rows == 0) return AXM_OK;
   if (int rc = require_device()) return rc;
   const Mx4Gather from = {nullptr, 1, rows, 1};
   return launch_quantize_rows<8>(x, x_dtype, ld, from, rows, k, nullptr, 0, codes, scales, nullptr,
@@ -451,10 +451,10 @@ extern "C" int axm_mx8_dequantize_rows(const void* codes, const void* scales, in
   const char* what = "axm_mx8_dequantize_rows";
   if (int rc = check_rows(rows, k, 0, what)) return rc;
   if (int rc = check_dtype(out_dtype, what)) return rc;
+  if (rows == 0) return AXM_OK;  // matrices without rows may have no address
   if (!codes || !scales || !out) return fail(AXM_ERR_ARGUMENT, "%s: null pointer", what);
   if (int rc = check_matrix(out, out_dtype, ld, k, what)) return rc;
   if (misaligned(codes, 16)) return fail(AXM_ERR_ARGUMENT, "%s: codes must be 16-byte aligned", what);
-  if (rows == 0) return AXM_OK;
   if (int rc = require_device()) return rc;
   return launch_dequantize_rows<8>(codes, scales, rows, k, nullptr, 0, out, out_dtype, ld,
                                    static_cast<cudaStream_t>(stream));

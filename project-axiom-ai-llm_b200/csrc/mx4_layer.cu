@@ -156,6 +156,7 @@ extern "C" int axm_mx4_linear(const void* x, int32_t x_dtype, int64_t ld, int32_
                               size_t workspace_bytes, void* stream) {
   size_t need = 0;
   if (int rc = axm_mx4_linear_workspace_bytes(tokens, k, n, &need)) return rc;
+  if (tokens == 0) return AXM_OK;  // matrices without rows may have no address
   if (!x || !w_codes || !w_scales || !out) return fail(AXM_ERR_ARGUMENT, "axm_mx4_linear: null pointer");
   if (int rc = check_mx_matrix(x, x_dtype, ld, k, "axm_mx4_linear: x")) return rc;
   if (out_dtype != AXM_DTYPE_BF16 && out_dtype != AXM_DTYPE_FP32)
@@ -163,7 +164,6 @@ extern "C" int axm_mx4_linear(const void* x, int32_t x_dtype, int64_t ld, int32_
   if (off16(w_codes) || off16(w_scales) || off16(out))
     return fail(AXM_ERR_ARGUMENT, "axm_mx4_linear: codes, scales and out must be 16-byte aligned");
   if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
-  if (tokens == 0) return AXM_OK;
   if (int rc = require_device()) return rc;
   const LinearWs w = carve_linear(tokens, k, workspace);
   const Mx4Rows rows = {nullptr, 0, tokens, 1, 0, 0, tokens, w.status};
@@ -191,12 +191,13 @@ extern "C" int axm_mx4_expert_ffn(const AxmMoeDesc* desc, const void* x, int32_t
   const char* what = "axm_mx4_expert_ffn";
   size_t need = 0;
   if (int rc = axm_mx4_expert_ffn_workspace_bytes(desc, rows, num_segments, &need)) return rc;
+  if (rows == 0 || num_segments == 0) return AXM_OK;  // matrices without rows may have no address
   if (!x || !segments || !o) return fail(AXM_ERR_ARGUMENT, "%s: null pointer", what);
   if (int rc = check_experts(experts, what)) return rc;
   if (o_dtype != AXM_DTYPE_BF16 && o_dtype != AXM_DTYPE_FP32) return fail(AXM_ERR_ARGUMENT, "%s: o_dtype %d unknown", what, o_dtype);
   if (off16(x) || off16(o)) return fail(AXM_ERR_ARGUMENT, "%s: x and o must be 16-byte aligned", what);
   if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
-  if (rows == 0 || num_segments == 0 || desc->tokens == 0) return AXM_OK;
+  if (desc->tokens == 0) return AXM_OK;
   if (int rc = require_device()) return rc;
   const int D = desc->d_model, F = desc->d_ff;
   const FfnWs w = carve_expert_ffn(desc, rows, num_segments, workspace);

@@ -7,6 +7,7 @@ checkpoints in 8 bits (formats in include/axm_moe.h).
     Mx4Linear        y = q4(x) . W^T for one weight matrix
     Mx4ExpertFfn     the expert feed-forward over a segment table
     Mx4MoeLayer      the whole layer (MoeLayer's call) with expert weights in 4 bits
+    Mx8TrainFfn      the expert feed-forward's training step, g and u kept in 8 bits between its passes
 
 Like the rest of the package these are thin callers of the C ABI: tensors are device memory,
 work goes to the current stream, nothing synchronises.  The engine keeps its weights in bf16
@@ -282,3 +283,78 @@ class Mx4MoeLayer(_Workspace):
                                                     _pkg.ptr(self.workspace), self.workspace.numel(),
                                                     _pkg.current_stream()))
         return out, self.histogram
+
+
+class Mx8TrainFfn:
+    """Training step of the expert feed-forward: forward(x, segments) -> o keeps the gate's and the up
+    projection's outputs in 8 bits, backward(d_o) gives the gradients from them.
+
+    gate, up [E][D][F] and down [E][F][D] bf16; up to `rows` rows, segments padded to 64 rows with zero
+    rows (the layer's training layout).  dtype: of o and of every gradient.  What is kept is in
+    `checkpoint`; `scratch` (h, dG, dU) holds nothing between calls and may be shared by objects of the
+    same sizes that run one after the other on one stream."""
+
+    def __init__(self, gate, up, down, rows, dtype=torch.bfloat16, scratch=None):
+        self.lib = _pkg.load()
+        e, d, f = gate.shape
+        if up.shape != (e, d, f) or down.shape != (e, f, d):
+            raise ValueError("gate and up are [E][D][F], down is [E][F][D]")
+        for w in (gate, up, down):
+            if w.dtype != torch.bfloat16 or not w.is_contiguous() or not w.is_cuda or w.device != gate.device:
+                raise ValueError("contiguous bf16 CUDA weights on one device are needed")
+        dev = gate.device
+        self.weights, self.rows, self.dtype = (gate, up, down), rows, dtype
+        _dtype(dtype)
+        self.desc = _pkg.make_desc(rows, d, f, e, 1, flags=0)
+        _bytes(self.lib.axm_mx8_checkpoint_bytes, rows, f)  # refuses sizes that cannot be kept
+        self.checkpoint = [torch.empty(rows, n, dtype=torch.uint8, device=dev) for n in (f, f // 32, f, f // 32)]
+        self.keep = _pkg.Mx8Checkpoint(*(t.data_ptr() for t in self.checkpoint))
+        self.scratch = scratch or [torch.empty(rows, f, dtype=torch.bfloat16, device=dev) for _ in range(3)]
+        self.status_word = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.saved = None
+
+    def status(self):
+        """Reads the status word (synchronises); sticky until it is cleared by the caller."""
+        torch.cuda.synchronize(self.status_word.device)
+        return int(self.status_word.item())
+
+    def _check(self, t, what):
+        if t.shape[0] > self.rows or t.shape[1] != self.desc.d_model or t.dtype != torch.bfloat16 or \
+                not t.is_contiguous() or t.device != self.status_word.device:
+            raise ValueError(f"{what}: up to {self.rows} contiguous bf16 rows of {self.desc.d_model} on {self.status_word.device}")
+
+    def forward(self, x, segments, out=None):
+        self._check(x, "x")
+        if segments.dtype != torch.int32 or segments.shape[1:] != (4,) or not segments.is_contiguous() or segments.device != x.device:
+            raise ValueError("segments: a contiguous int32 table n x 4 beside x")
+        if out is None:
+            out = torch.empty(x.shape, dtype=self.dtype, device=x.device)
+        p = _pkg.ptr
+        with _on(x.device):
+            _pkg.check(self.lib.axm_mx8_expert_ffn_train(
+                ctypes.byref(self.desc), p(x), x.shape[0], p(segments), segments.shape[0], *map(p, self.weights),
+                ctypes.byref(self.keep), p(self.scratch[0]), p(out), _dtype(out.dtype), p(self.status_word),
+                _pkg.current_stream()))
+        self.saved = (x, segments)
+        return out
+
+    def backward(self, d_o, weight_grads=True):
+        """{d_x, d_gate, d_up, d_down} (weight_grads False: d_x alone) of the last forward call."""
+        if self.saved is None:
+            raise RuntimeError("backward before forward")
+        x, segments = self.saved
+        self._check(d_o, "d_o")
+        if d_o.shape != x.shape:
+            raise ValueError(f"d_o {tuple(d_o.shape)} is not like x {tuple(x.shape)}")
+        p = _pkg.ptr
+        grads = {"d_x": torch.empty(x.shape, dtype=self.dtype, device=x.device)}
+        if weight_grads:
+            for n, w in zip(("d_gate", "d_up", "d_down"), self.weights):
+                grads[n] = torch.empty(w.shape, dtype=self.dtype, device=x.device)
+        with _on(x.device):
+            _pkg.check(self.lib.axm_mx8_expert_ffn_backward(
+                ctypes.byref(self.desc), p(x), x.shape[0], p(segments), segments.shape[0], ctypes.byref(self.keep), p(d_o),
+                *map(p, self.weights), *map(p, self.scratch), p(grads["d_x"]), p(grads.get("d_gate")),
+                p(grads.get("d_up")), p(grads.get("d_down")), _dtype(self.dtype), p(self.status_word),
+                _pkg.current_stream()))
+        return grads

@@ -90,3 +90,13 @@ def candidates(x, rel, held, emax):
             lo = v if lo is None else torch.minimum(lo, v)
             hi = v if hi is None else torch.maximum(hi, v)
     return lo, hi
+
+
+def ffn_backward(x, g, u, d_o, wg, wu, wd):
+    """One expert's gradients in 64 bits from the gate's and up projection's outputs as kept:
+    (d_x, d_wg, d_wu, d_wd) and the intermediates the error bounds need."""
+    s = torch.sigmoid(g)
+    d_h = d_o @ wd.T
+    slope = s * (1 + g * (1 - s))
+    d_g, d_u, h = d_h * u * slope, d_h * g * s, g * s * u
+    return (d_g @ wg.T + d_u @ wu.T, x.T @ d_g, x.T @ d_u, h.T @ d_o), (d_h, s, d_g, d_u, h)

@@ -175,3 +175,58 @@ def test_python_refuses():
         ms.quantize_weights(torch.zeros(1, 64, 8))
     with pytest.raises(ValueError):
         ms.Mx4Weights.from_checkpoint(torch.zeros(1, 8, 16, dtype=torch.uint8), torch.zeros(1, 8, 1, dtype=torch.uint8))
+
+
+def test_train8_refuses(lib, axm):
+    a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    assert two(lib.axm_mx8_checkpoint_bytes, 128, 96) == (128 * 96, 128 * 3)
+    for args in [(-1, 32), (4, 0), (4, 40)]:
+        assert lib.axm_mx8_checkpoint_bytes(*args, ctypes.byref(a), ctypes.byref(b)) == axm.AXM_ERR_ARGUMENT
+    keep = axm.Mx8Checkpoint(*[FAKE] * 4)
+
+    def forward(d=(64, 64), e=2, x=FAKE, rows=64, seg=FAKE, nseg=2, w=FAKE, k=keep, h=FAKE, o=FAKE, dt=0):
+        desc = axm.make_desc(64, *d, e, 1)
+        return lib.axm_mx8_expert_ffn_train(ctypes.byref(desc), x, rows, seg, nseg, w, FAKE, FAKE,
+                                            None if k is None else ctypes.byref(k), h, o, dt, None, None)
+
+    half, odd = axm.Mx8Checkpoint(*[FAKE] * 4), axm.Mx8Checkpoint(*[FAKE] * 4)
+    half.up_scales, odd.gate_codes = None, ODD
+    common = [dict(d=(60, 64)), dict(d=(64, 40)), dict(e=0), dict(x=None), dict(x=ODD), dict(rows=-1), dict(seg=None),
+              dict(nseg=513), dict(nseg=-1), dict(w=None), dict(k=None), dict(k=half), dict(k=odd), dict(h=None), dict(dt=2)]
+    for kw in common + [dict(o=None), dict(o=ODD)]:
+        assert forward(**kw) == axm.AXM_ERR_ARGUMENT, kw
+    assert forward(rows=0) == axm.AXM_OK and forward(nseg=0) == axm.AXM_OK
+
+    def backward(d=(64, 64), e=2, x=FAKE, rows=64, seg=FAKE, nseg=2, w=FAKE, k=keep, h=FAKE, dt=0, d_o=FAKE, d_x=FAKE,
+                 dw=(FAKE, FAKE, FAKE)):
+        desc = axm.make_desc(64, *d, e, 1)
+        return lib.axm_mx8_expert_ffn_backward(ctypes.byref(desc), x, rows, seg, nseg, None if k is None else ctypes.byref(k),
+                                               d_o, w, FAKE, FAKE, h, FAKE, FAKE, d_x, *dw, dt, None, None)
+
+    for kw in common + [dict(d_o=None), dict(d_x=None), dict(d_x=ODD), dict(dw=(FAKE, None, FAKE)), dict(dw=(FAKE, ODD, FAKE))]:
+        assert backward(**kw) == axm.AXM_ERR_ARGUMENT, kw
+    assert backward(nseg=0) == axm.AXM_OK
+
+
+def test_backward_reference_against_differences():
+    """The reference's gradients are the derivatives of sum(d_o * ((silu(g) u) Wd)) where g and u are
+    held exactly (64-bit central differences: truncation about 1e-4 ** 2, rounding about 1e-16 / 1e-4)."""
+    gen = torch.Generator().manual_seed(5)
+    x, d_o = (torch.randn(6, 8, generator=gen, dtype=torch.float64) for _ in range(2))
+    wg, wu = (torch.randn(8, 4, generator=gen, dtype=torch.float64) for _ in range(2))
+    wd = torch.randn(4, 8, generator=gen, dtype=torch.float64)
+
+    def loss(x, wg, wu, wd):
+        g, u = x @ wg, x @ wu
+        return float((d_o * ((g * torch.sigmoid(g) * u) @ wd)).sum())
+
+    grads, _ = ref.ffn_backward(x, x @ wg, x @ wu, d_o, wg, wu, wd)
+    args = [x, wg, wu, wd]
+    for i, grad in enumerate(grads):
+        for at in range(args[i].numel()):
+            both = []
+            for h in (1e-4, -1e-4):
+                moved = [a.clone() for a in args]
+                moved[i].view(-1)[at] += h
+                both.append(loss(*moved))
+            assert abs((both[0] - both[1]) / 2e-4 - float(grad.reshape(-1)[at])) < 1e-5

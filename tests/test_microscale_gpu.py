@@ -199,6 +199,22 @@ def test_linear_wide_scales(ms, cuda_device, t, k, n):
     assert plan.status() == 0
 
 
+def test_nothing_to_do(ms, cuda_device):
+    """No rows: nothing happens, and nothing fails."""
+    empty = torch.empty(0, 64, dtype=BF16, device=cuda_device)
+    assert ms.dequantize_rows(ms.quantize_rows(empty)).shape == (0, 64)
+    assert ms.dequantize_rows8(*ms.quantize_rows8(empty)).shape == (0, 64)
+    w = ms.quantize_weights(torch.ones(1, 64, 24, device=cuda_device))
+    assert ms.Mx4Linear(w, 4).forward(empty).shape == (0, 24)
+    v = ms.quantize_weights(torch.ones(1, 24 * 4, 64, device=cuda_device))
+    w = ms.quantize_weights(torch.ones(1, 64, 24 * 4, device=cuda_device))
+    segs, _ = table([0], cuda_device)
+    assert ms.Mx4ExpertFfn(w, w, v, rows=4, tokens=4).forward(empty, segs).shape == (0, 64)
+    out = torch.full((3, 64), 2.0, dtype=BF16, device=cuda_device)  # rows, but none in the table
+    ms.Mx4ExpertFfn(w, w, v, rows=4, tokens=4).forward(torch.ones(3, 64, dtype=BF16, device=cuda_device), segs, out=out)
+    assert (out == 2).all()
+
+
 def test_linear_not_finite(ms, cuda_device):
     x = torch.ones(4, 64, device=cuda_device)
     x[1, 3], x[2, 40] = float("nan"), float("inf")
@@ -368,3 +384,135 @@ def test_same_bits_again(ms, cuda_device):
         plan = ms.Mx4Linear(w, t)
         first = plan.forward(x, dtype=FP32).clone()
         assert all(torch.equal(first, plan.forward(x, dtype=FP32)) for _ in range(5))
+
+
+TRAIN = [([1], 8, 32), ([64], 64, 64), ([0, 1, 0, 70], 72, 160), ([3, 0, 2, 0, 0, 11], 256, 512),
+         ([129, 0, 1, 300, 128], 520, 352), ([1] * 30 + [0] * 5 + [65], 136, 96), ([260, 255], 1032, 1408)]
+
+
+def whole_values(g, shape, top, dev, scale):
+    """Whole numbers -top..top times a power of two, in bf16 exactly."""
+    return (torch.randint(-top, top + 1, shape, generator=g, device=dev).double() * scale)
+
+
+@pytest.mark.parametrize("counts,d,f", TRAIN)
+def test_train_step(ms, cuda_device, counts, d, f):
+    """Inputs are small whole numbers times powers of two: g, u and dH are exact in 32 bits, so the
+    kept codes must be the reference's, and every other output is off by its roundings alone."""
+    dev = cuda_device
+    e = len(counts)
+    segs, rows = table(counts, dev, 64)
+    gen = generator(dev, sum(counts) + d)
+    shift = 2.0 ** -((d.bit_length() + 4) // 2)
+    x = whole_values(gen, (rows + 3, d), 4, dev, 0.5)
+    d_o = whole_values(gen, (rows + 3, d), 4, dev, 0.25)
+    for (at, _, n, i), c in zip(segs.tolist(), counts):
+        x[at + c:at + n] = 0
+        d_o[at + c:at + n] = 0
+    gate, up = (whole_values(gen, (e, d, f), 4, dev, shift) for _ in range(2))
+    down = whole_values(gen, (e, f, d), 4, dev, shift)
+    assert d * 16 < 2 ** 24
+    for dt, half in ((FP32, 0.0), (BF16, 2.0 ** -8)):
+        plan = ms.Mx8TrainFfn(gate.to(BF16), up.to(BF16), down.to(BF16), rows=rows + 3, dtype=dt)
+        o = torch.full((rows + 3, d), float("nan"), dtype=dt, device=dev)
+        plan.forward(x.to(BF16), segs, out=o)
+        got = plan.backward(d_o.to(BF16))
+        assert plan.status() == 0
+        gc, gs, uc, us = plan.checkpoint
+        tiny = 2.0 ** -23
+        for _, at, n, i in segs.tolist():
+            r = slice(at, at + n)
+            if n == 0:
+                assert all((got[k][i] == 0).all() for k in ("d_gate", "d_up", "d_down"))
+                continue
+            g, u = x[r] @ gate[i], x[r] @ up[i]
+            for codes, scales, v in ((gc, gs, g), (uc, us, u)):
+                assert torch.equal(scales[r], ref.scale_bytes(v, 8))
+                assert same(ms.dequantize_rows8(codes[r].contiguous(), scales[r].contiguous(), FP32).double(), ref.held8(v))
+
+            def check(name, value, want, slack):
+                err = (value.double() - want).abs()
+                bound = slack + half * (want.abs() + slack) + 1e-30
+                assert (err <= bound).all(), (name, float((err / bound.clamp(min=1e-30)).max()))
+
+            # o: h rounded to bf16 after a sigmoid of a few ulp, then a sum of f products
+            fast = (8 + 1.2 * float(g.abs().max())) * tiny
+            h = g * torch.sigmoid(g) * u
+            check("o", o[r], h @ down[i], (2.0 ** -8 + fast + f * tiny) * 1.01 * (h.abs() @ down[i].abs()))
+            g, u = ref.held8(g), ref.held8(u)
+            (d_x, d_wg, d_wu, d_wd), (d_h, s, d_g, d_u, hh) = ref.ffn_backward(x[r], g, u, d_o[r], gate[i], up[i], down[i])
+            # the slope's two terms may cancel: its error is that of their magnitudes
+            e_g = (d_h * u).abs() * (s + (g * s * (1 - s)).abs()) * fast + 2.0 ** -8 * 1.01 * d_g.abs()
+            e_u = (2.0 ** -8 * 1.01 + fast) * d_u.abs()
+            e_h = (2.0 ** -8 * 1.01 + fast) * hh.abs()
+            a_g, a_u, a_h = d_g.abs() + e_g, d_u.abs() + e_u, hh.abs() + e_h
+            check("d_x", got["d_x"][r], d_x, e_g @ gate[i].abs().T + e_u @ up[i].abs().T +
+                  2 * f * tiny * (a_g @ gate[i].abs().T + a_u @ up[i].abs().T))
+            xa, da = x[r].abs(), d_o[r].abs()
+            check("d_gate", got["d_gate"][i], d_wg, xa.T @ e_g + n * tiny * (xa.T @ a_g))
+            check("d_up", got["d_up"][i], d_wu, xa.T @ e_u + n * tiny * (xa.T @ a_u))
+            check("d_down", got["d_down"][i], d_wd, e_h.T @ da + n * tiny * (a_h.T @ da))
+        assert torch.isnan(o[rows:].float()).all()  # rows behind the last segment are left as they were
+        alone = plan.backward(d_o.to(BF16), weight_grads=False)
+        assert set(alone) == {"d_x"} and torch.equal(alone["d_x"][:rows], got["d_x"][:rows])
+
+
+def test_train_step_again_captured_and_shared_scratch(ms, cuda_device):
+    """The same bits again, from a captured pair of passes and with another object using the same
+    scratch between forward and backward: what is kept is the checkpoint alone."""
+    dev = cuda_device
+    segs, rows = table([70, 0, 64, 9], dev, 64)
+    gen = generator(dev, 1)
+    w = [torch.empty(4, a, b, device=dev).normal_(0, .05, generator=gen).to(BF16) for a, b in ((128, 160), (128, 160), (160, 128))]
+    xs, ds = ([torch.empty(rows, 128, device=dev).normal_(generator=gen).to(BF16) for _ in range(2)] for _ in range(2))
+    a = ms.Mx8TrainFfn(*w, rows=rows)
+    b = ms.Mx8TrainFfn(*w, rows=rows, scratch=a.scratch)
+    want = []
+    for x, d in zip(xs, ds):
+        o = a.forward(x, segs)
+        want.append((o, a.backward(d)))
+    oa, ob = a.forward(xs[0], segs), b.forward(xs[1], segs)
+    gb, ga = b.backward(ds[1]), a.backward(ds[0])
+    for (o, g), (o2, g2) in zip(want, ((oa, ga), (ob, gb))):
+        assert torch.equal(o, o2) and all(torch.equal(g[k], g2[k]) for k in g)
+    x, d = xs[0].clone(), ds[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = a.forward(x, segs)
+        g = a.backward(d)
+    for i in (1, 0, 1):
+        x.copy_(xs[i])
+        d.copy_(ds[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want[i][0]) and all(torch.equal(g[k], want[i][1][k]) for k in g)
+    with pytest.raises(RuntimeError):
+        ms.Mx8TrainFfn(*w, rows=rows).backward(d)
+
+
+def test_train_step_without_rows(ms, cuda_device):
+    w = [torch.ones(2, a, b, dtype=BF16, device=cuda_device) for a, b in ((64, 32), (64, 32), (32, 64))]
+    segs, rows = table([0, 0], cuda_device)
+    plan = ms.Mx8TrainFfn(*w, rows=0)
+    x = torch.empty(0, 64, dtype=BF16, device=cuda_device)
+    plan.forward(x, segs)
+    g = plan.backward(x)
+    assert all((g[k] == 0).all() for k in ("d_gate", "d_up", "d_down"))
+
+
+def test_train_step_not_finite(ms, cuda_device):
+    """A NaN in one row of x: that row's outputs and, as sums over rows, the weights' gradients are NaN;
+    the other rows' outputs are untouched."""
+    dev = cuda_device
+    gen = generator(dev, 2)
+    w = [torch.empty(1, a, b, device=dev).normal_(0, .05, generator=gen).to(BF16) for a, b in ((64, 96), (64, 96), (96, 64))]
+    x, d = (torch.empty(64, 64, device=dev).normal_(generator=gen).to(BF16) for _ in range(2))
+    segs, _ = table([64], dev, 64)
+    plan = ms.Mx8TrainFfn(*w, rows=64)
+    o, g = plan.forward(x, segs), plan.backward(d)
+    y = x.clone()
+    y[5, 3] = float("nan")
+    o2, g2 = plan.forward(y, segs), plan.backward(d)
+    keep = torch.arange(64, device=dev) != 5
+    assert torch.equal(o[keep], o2[keep]) and torch.equal(g["d_x"][keep], g2["d_x"][keep])
+    assert torch.isnan(o2[5]).all() and torch.isnan(g2["d_x"][5]).all() and torch.isnan(g2["d_gate"]).any()
