@@ -204,6 +204,12 @@ def current_stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def raw_stream(device_index):
+    """The current stream of a device as a plain number: current_stream() without the objects, for
+    calls whose own work on the host counts (a fraction of a microsecond instead of two)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def make_desc(tokens, d_model, d_ff, num_experts, top_k, num_shared=0, router_dtype=ROUTER_FP32,
               flags=FLAG_RESIDUAL):
     return MoeDesc(tokens, d_model, d_ff, num_experts, top_k, num_shared, router_dtype, flags)

@@ -9,56 +9,62 @@ namespace axm {
 
 namespace {
 
-// Eight neighbouring values of a row as fp32.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]);
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[2 * j] = bf16_lo(w[j]);
-    v[2 * j + 1] = bf16_hi(w[j]);
+struct Words8 {
+  uint32_t w[8];
+};
+// 32 bytes in one load or store (the address is a multiple of 16 bytes only where kWide is false).
+template <bool kWide>
+__device__ __forceinline__ Words8 load32(const void* p) {
+  Words8 r;
+  if constexpr (kWide) {
+    asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+        : "l"(p));
+  } else {
+    const uint4 a = __ldg(static_cast<const uint4*>(p)), b = __ldg(static_cast<const uint4*>(p) + 1);
+    r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
+    r.w[4] = b.x; r.w[5] = b.y; r.w[6] = b.z; r.w[7] = b.w;
+  }
+  return r;
+}
+template <bool kWide>
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  if constexpr (kWide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    static_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    static_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
 }
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8]);
-template <>
-__device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) =
-      make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-}
-template <>
-__device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
 
-// One warp per 256 neighbouring elements of a row: a lane holds eight of them (a 16-byte load of
-// bf16), four lanes a block.  kBits = 4: scale bytes in tile order, the row's last, partial run
-// padded with zero bytes.  kBits = 8: codes [rows][K], scale bytes [rows][K / 32].
+// Rows are cut into runs of 512 elements, one warp a run: a lane holds sixteen neighbours (32 bytes
+// of bf16), two lanes a block.  A CTA of eight warps gives each row 2^log_wpr of them (as many as
+// the row has runs, up to eight), and a warp has up to kAhead runs' loads in flight.
+// These kernels are bound by their instructions as easily as by memory: a first form with eight
+// elements a lane and fp32 arithmetic throughout issued 160 instructions per 256 elements and read
+// and wrote 3.9 TB/s.
+constexpr int kAhead = 2;
+
+// kBits = 4: scale bytes in tile order, the row's last, partial stage padded with zero bytes.
+// kBits = 8: codes [rows][K], scale bytes [rows][K / 32].
+// kWide: rows start at multiples of 32 bytes.
 // `from` says which source row a row comes from; row_src[r] < 0: zeros.
-template <int kBits, typename T>
+template <int kBits, typename T, bool kWide>
 __global__ void __launch_bounds__(256)
-mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, int rows, int k,
+mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, int rows, int k, int log_wpr,
                         const AxmSegment* __restrict__ segments, int num_segments,
                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int32_t* status) {
   if (status != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
-  const int lane = threadIdx.x & 31;
-  const int runs = (k + 255) / 256;
-  const long long items = (long long)rows * runs;
-  const long long step = (long long)gridDim.x * (blockDim.x >> 5);
-  for (long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); item < items; item += step) {
-    const int row = (int)(item / runs);
-    const int run = (int)(item - (long long)row * runs);
-    const int k0 = run * 256 + lane * 8;
+  constexpr bool kBf16 = sizeof(T) == 2;
+  constexpr int kWords = kBf16 ? 1 : 2;  // 32-byte pieces a lane
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int runs = (k + 511) / 512, wpr = 1 << log_wpr;
+  const int rows_per_cta = 8 >> log_wpr;
+  for (long long row_at = (long long)blockIdx.x * rows_per_cta + (warp >> log_wpr); row_at < rows;
+       row_at += (long long)gridDim.x * rows_per_cta) {
+    const int row = (int)row_at;
     long long src = row;
     if (row >= from.tail_row0) {
       src = (row - from.tail_row0) % from.tail_mod;
@@ -66,87 +72,168 @@ mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, i
       const int s = __ldg(from.row_src + row);
       src = s < 0 ? -1 : s / from.row_div;
     }
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (k0 < k && src >= 0) load8<T>(x + src * ld + k0, v);
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t s = mx_scale_byte<kBits == 4 ? 2 : 8>(top);
-    const float inv = mx_inverse_scale(s);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= inv;
+    const T* in = x + (src < 0 ? 0 : src) * ld;
+    uint8_t* out = codes + (size_t)row * (kBits == 4 ? k >> 1 : k);
+    uint8_t* sc = scales;  // this row's scale bytes; kBits 4: in chunk 0
+    bool placed = true;    // a row behind its segment's end has no place among the tiles
     if constexpr (kBits == 4) {
-      if (k0 < k) *reinterpret_cast<uint32_t*>(codes + (size_t)row * (k >> 1) + (k0 >> 1)) = mx4_pack8(v);
-      int seg = 0, tile_row = row;
+      int seg = 0, first = 0;
       if (segments != nullptr) {
         seg = segment_of_row(segments, num_segments, row);
-        if (seg < 0) continue;  // a row behind its segment's end has no place among the tiles
-        tile_row = row - __ldg(&segments[seg].out_row0);
+        placed = seg >= 0;
+        if (placed) first = __ldg(&segments[seg].out_row0);
       }
-      // the four bytes of a 128-element chunk gathered into one word by the chunk's first lane
-      uint32_t word = s << (8 * ((lane >> 2) & 3));
-      word |= __shfl_xor_sync(0xffffffffu, word, 4);
-      word |= __shfl_xor_sync(0xffffffffu, word, 8);
-      if ((lane & 15) == 0) {
-        const int first = segments != nullptr ? __ldg(&segments[seg].out_row0) : 0;
-        const size_t tile = (size_t)(first / 128 + seg + tile_row / 128);
-        const int r = tile_row & 127;
-        uint8_t* chunk = scales + (tile * mx4_chunks(k) + run * 2 + (lane >> 4)) * 512;
-        *reinterpret_cast<uint32_t*>(chunk + (r & 31) * 16 + (r >> 5) * 4) = word;
-      }
+      const int r = row - first;
+      sc += ((size_t)(first / 128 + (placed ? seg : 0) + r / 128) * mx4_chunks(k)) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4;
     } else {
-      if (k0 < k) {
-        *reinterpret_cast<uint2*>(codes + (size_t)row * k + k0) =
-            make_uint2(mx8_pack4(v[0], v[1], v[2], v[3]), mx8_pack4(v[4], v[5], v[6], v[7]));
-        if ((lane & 3) == 0) scales[(size_t)row * (k >> 5) + (k0 >> 5)] = (uint8_t)s;
+      sc += (size_t)row * (k >> 5);
+    }
+    for (int run0 = warp & (wpr - 1); run0 < runs; run0 += kAhead * wpr) {
+      Words8 v[kAhead][kWords];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int k0 = (run0 + i * wpr) * 512 + lane * 16;  // k is a multiple of 32: all sixteen or none
+        if (k0 < k && src >= 0) {
+#pragma unroll
+          for (int j = 0; j < kWords; ++j) v[i][j] = load32<kWide>(in + k0 + 8 * j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kWords; ++j) v[i][j] = Words8{};
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int run = run0 + i * wpr;
+        if (run >= runs) break;
+        const int k0 = run * 512 + lane * 16;
+        uint32_t top = 0;
+        if constexpr (kBf16) {  // largest magnitude by the bits, two at a time
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = __vmaxu2(top, v[i][0].w[j] & 0x7fff7fffu);
+          top = max(top & 0xffff0000u, top << 16);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) top = max(top, v[i][j >> 3].w[j & 7] & 0x7fffffffu);
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        const uint32_t s = mx_scale_byte<kBits == 4 ? 2 : 8>(top);
+        const float inv = mx_inverse_scale(s);
+        auto value = [&](int j) {  // element j of the lane's sixteen, scaled
+          if constexpr (kBf16) {
+            const uint32_t w = v[i][0].w[j >> 1];
+            return ((j & 1) ? bf16_hi(w) : bf16_lo(w)) * inv;
+          } else {
+            return __uint_as_float(v[i][j >> 3].w[j & 7]) * inv;
+          }
+        };
+        if constexpr (kBits == 4) {
+          uint32_t c[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = value(8 * h + j);
+            c[h] = mx4_pack8(t);
+          }
+          if (k0 < k) *reinterpret_cast<uint2*>(out + (k0 >> 1)) = make_uint2(c[0], c[1]);
+          // the four bytes of a 128-element chunk gathered into one word by the chunk's first lane
+          uint32_t word = s << (8 * ((lane >> 1) & 3));
+          word |= __shfl_xor_sync(0xffffffffu, word, 2);
+          word |= __shfl_xor_sync(0xffffffffu, word, 4);
+          const int chunk = run * 4 + (lane >> 3);
+          if (placed && (lane & 7) == 0 && chunk < mx4_chunks(k)) *reinterpret_cast<uint32_t*>(sc + (size_t)chunk * 512) = word;
+        } else if (k0 < k) {
+          uint32_t c[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) c[h] = mx8_pack4(value(4 * h), value(4 * h + 1), value(4 * h + 2), value(4 * h + 3));
+          *reinterpret_cast<uint4*>(out + k0) = make_uint4(c[0], c[1], c[2], c[3]);
+          if ((lane & 1) == 0) sc[k0 >> 5] = (uint8_t)s;
+        }
       }
     }
   }
 }
 
-template <int kBits, typename T>
+template <int kBits, typename T, bool kWide>
 __global__ void __launch_bounds__(256)
 mx_dequantize_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int k,
-                          const AxmSegment* __restrict__ segments, int num_segments, T* __restrict__ out,
-                          long long ld) {
-  const int lane = threadIdx.x & 31;
-  const int runs = (k + 255) / 256;
-  const long long items = (long long)rows * runs;
-  const long long step = (long long)gridDim.x * (blockDim.x >> 5);
-  for (long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); item < items; item += step) {
-    const int row = (int)(item / runs);
-    const int run = (int)(item - (long long)row * runs);
-    const int k0 = run * 256 + lane * 8;
-    if (k0 >= k) continue;
-    float v[8];
+                          int log_wpr, const AxmSegment* __restrict__ segments, int num_segments,
+                          T* __restrict__ out, long long ld) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int runs = (k + 511) / 512, wpr = 1 << log_wpr;
+  const int rows_per_cta = 8 >> log_wpr;
+  for (long long row_at = (long long)blockIdx.x * rows_per_cta + (warp >> log_wpr); row_at < rows;
+       row_at += (long long)gridDim.x * rows_per_cta) {
+    const int row = (int)row_at;
+    const uint8_t* in = codes + (size_t)row * (kBits == 4 ? k >> 1 : k);
+    const uint8_t* sc = scales;
+    T* to = out + (size_t)row * ld;
     if constexpr (kBits == 4) {
       int seg = 0, first = 0;
       if (segments != nullptr) {
         seg = segment_of_row(segments, num_segments, row);
-        if (seg < 0) continue;
+        if (seg < 0) continue;  // left as it is
         first = __ldg(&segments[seg].out_row0);
       }
       const int r = row - first;
-      const size_t tile = (size_t)(first / 128 + seg + r / 128);
-      const uint8_t* chunk = scales + (tile * mx4_chunks(k) + run * 2 + (lane >> 4)) * 512;
-      const float s = mx_scale_value(__ldg(chunk + (r & 31) * 16 + ((r & 127) >> 5) * 4 + ((lane >> 2) & 3)));
-      const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(codes + (size_t)row * (k >> 1) + (k0 >> 1)));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = mx4_code_value(c >> (4 * j)) * s;
+      sc += ((size_t)(first / 128 + seg + r / 128) * mx4_chunks(k)) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4;
     } else {
-      const float s = mx_scale_value(__ldg(scales + (size_t)row * (k >> 5) + (k0 >> 5)));
-      const uint2 c = __ldg(reinterpret_cast<const uint2*>(codes + (size_t)row * k + k0));
-      const uint32_t w[4] = {c.x & 0xffffu, c.x >> 16, c.y & 0xffffu, c.y >> 16};
+      sc += (size_t)row * (k >> 5);
+    }
+    for (int run0 = warp & (wpr - 1); run0 < runs; run0 += kAhead * wpr) {
+      uint4 c[kAhead];
+      uint32_t s[kAhead];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = mx8_unpack2(w[j]);
-        v[2 * j] = f.x * s;
-        v[2 * j + 1] = f.y * s;
+      for (int i = 0; i < kAhead; ++i) {
+        const int run = run0 + i * wpr, k0 = run * 512 + lane * 16;
+        c[i] = make_uint4(0, 0, 0, 0);
+        s[i] = 0;
+        if (k0 < k) {
+          if constexpr (kBits == 4) {
+            const uint2 t = __ldg(reinterpret_cast<const uint2*>(in + (k0 >> 1)));
+            c[i].x = t.x;
+            c[i].y = t.y;
+            s[i] = __ldg(sc + (size_t)(run * 4 + (lane >> 3)) * 512 + ((lane >> 1) & 3));
+          } else {
+            c[i] = __ldg(reinterpret_cast<const uint4*>(in + k0));
+            s[i] = __ldg(sc + (k0 >> 5));
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int k0 = (run0 + i * wpr) * 512 + lane * 16;
+        if (k0 >= k) break;
+        const uint32_t f = mx_scale_bf16x2(s[i]);
+        uint32_t w[8];
+        if constexpr (kBits == 4) {
+          uint32_t t[4];
+          mx4_decode8(c[i].x, f, t);
+          w[0] = t[0]; w[1] = t[1]; w[2] = t[2]; w[3] = t[3];
+          mx4_decode8(c[i].y, f, t);
+          w[4] = t[0]; w[5] = t[1]; w[6] = t[2]; w[7] = t[3];
+        } else {
+          mx8_decode4(c[i].x, f, w[0], w[1]);
+          mx8_decode4(c[i].y, f, w[2], w[3]);
+          mx8_decode4(c[i].z, f, w[4], w[5]);
+          mx8_decode4(c[i].w, f, w[6], w[7]);
+        }
+        if constexpr (sizeof(T) == 2) {
+          store32<kWide>(to + k0, w);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              v[2 * j] = w[4 * h + j] << 16;
+              v[2 * j + 1] = w[4 * h + j] & 0xffff0000u;
+            }
+            store32<kWide>(to + k0 + 8 * h, v);
+          }
+        }
       }
     }
-    store8<T>(out + (size_t)row * ld + k0, v);
   }
 }
 
@@ -161,10 +248,6 @@ template <>
 __device__ __forceinline__ float2 load2<float>(const float* p) {
   return __ldg(reinterpret_cast<const float2*>(p));
 }
-__device__ __forceinline__ void store2(__nv_bfloat16* p, float a, float b) {
-  *reinterpret_cast<uint32_t*>(p) = pack_bf16(a, b);
-}
-__device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
 
 // Expert weights [E][K][N] (N contiguous, as the engine stores them) to codes [E][N][K / 2]: a
 // block runs down K, so a thread owns two neighbouring columns and walks 32 rows; a warp's loads
@@ -238,41 +321,57 @@ mx4_quantize_weights_kernel(const T* __restrict__ w, int k, int n, uint8_t* __re
   }
 }
 
+// Back to [E][K][N]: a thread owns four neighbouring columns of one block of 32 k, and half a warp
+// writes 64 columns of a row.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 mx4_dequantize_weights_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int k, int n,
                               T* __restrict__ w) {
   __shared__ uint4 tile[kWeightsN * 8];
   const int e = blockIdx.z, n0 = blockIdx.x * kWeightsN, k0 = blockIdx.y * kWeightsK;
-  for (int i = threadIdx.x; i < kWeightsN * 8; i += 256) {
+  // piece p of column c at p ^ (c / 4 % 8): four columns apart is what the lanes read together
+  for (int i = threadIdx.x; i < kWeightsN * 8; i += 128) {
     const int c = i >> 3, piece = i & 7;
     uint4 v = make_uint4(0, 0, 0, 0);
     if (n0 + c < n && k0 + piece * kMxBlock < k)
       v = __ldg(reinterpret_cast<const uint4*>(codes + ((size_t)e * n + n0 + c) * (k >> 1) + (k0 >> 1) + piece * 16));
-    tile[c * 8 + (piece ^ (c & 7))] = v;
+    tile[c * 8 + (piece ^ ((c >> 2) & 7))] = v;
   }
   __syncthreads();
-  const int pair = threadIdx.x & 31, blk = threadIdx.x >> 5;
-  const int col = n0 + 2 * pair, kk = k0 + blk * kMxBlock;
-  if (col >= n || kk >= k) return;
-  float s[2];
-  uint32_t q[2][4];
+  const int quad = threadIdx.x & 15, blk = threadIdx.x >> 4;
+  const int col = n0 + 4 * quad, kk = k0 + blk * kMxBlock;
+  if (col >= n || kk >= k) return;  // n is a multiple of 8: four columns or none
+  uint32_t f[4], q[4][4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int c = 2 * pair + h, cw = col + h;
-    const uint4 v = tile[c * 8 + (blk ^ (c & 7))];
+  for (int h = 0; h < 4; ++h) {
+    const uint4 v = tile[(4 * quad + h) * 8 + (blk ^ (quad & 7))];
     q[h][0] = v.x; q[h][1] = v.y; q[h][2] = v.z; q[h][3] = v.w;
-    const size_t t = (size_t)e * ((n + 127) / 128) + cw / 128;
-    const int r = cw & 127;
-    s[h] = mx_scale_value(__ldg(scales + (t * mx4_chunks(k) + (kk >> 7)) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (blk & 3)));
+  }
+  {  // the four columns' scale bytes are 16 bytes apart
+    const size_t t = (size_t)e * ((n + 127) / 128) + col / 128;
+    const int r = col & 127;
+    const uint8_t* p = scales + (t * mx4_chunks(k) + (kk >> 7)) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (blk & 3);
+#pragma unroll
+    for (int h = 0; h < 4; ++h) f[h] = mx_scale_bf16x2(__ldg(p + 16 * h));
   }
   T* p = w + ((size_t)e * k + kk) * n + col;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 4; ++i) {
+    uint32_t d[4][4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      store2(p + (size_t)(8 * i + j) * n, mx4_code_value(q[0][i] >> (4 * j)) * s[0],
-             mx4_code_value(q[1][i] >> (4 * j)) * s[1]);
+    for (int h = 0; h < 4; ++h) mx4_decode8(q[h][i], f[h], d[h]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t lo, hi;  // columns 0, 1 and 2, 3 of row 8 i + j
+      lo = __byte_perm(d[0][j >> 1], d[1][j >> 1], (j & 1) ? 0x7632 : 0x5410);
+      hi = __byte_perm(d[2][j >> 1], d[3][j >> 1], (j & 1) ? 0x7632 : 0x5410);
+      T* to = p + (size_t)(8 * i + j) * n;
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+      else
+        *reinterpret_cast<float4*>(to) = make_float4(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi));
+    }
+  }
 }
 
 // Scale bytes as checkpoints keep them, [E][N][K / 32], to tile order.
@@ -326,42 +425,60 @@ int check_matrix(const void* p, int32_t dtype, int64_t ld, int32_t k, const char
   return AXM_OK;
 }
 
-unsigned row_grid(int32_t rows, int32_t k) {
-  const long long warps = (long long)rows * ((k + 255) / 256);
-  long long blocks = (warps + 7) / 8;
-  const long long most = 32LL * sm_count();
-  return (unsigned)(blocks < most ? blocks : most);
+// Warps a row (as a power of two) and CTAs of a row kernel.
+struct RowLaunch {
+  int log_wpr;
+  unsigned grid;
+};
+RowLaunch row_launch(int32_t rows, int32_t k) {
+  RowLaunch l = {0, 0};
+  while (l.log_wpr < 3 && (2 << l.log_wpr) <= (k + 511) / 512) ++l.log_wpr;
+  const long long per = 8 >> l.log_wpr;
+  const long long blocks = (rows + per - 1) / per, most = 32LL * sm_count();
+  l.grid = (unsigned)(blocks < most ? blocks : most);
+  return l;
+}
+// Whether every row of a matrix starts at a multiple of 32 bytes.
+bool rows_at_32(const void* p, int64_t ld, int32_t dtype) {
+  return !misaligned(p, 32) && ld * (dtype == AXM_DTYPE_BF16 ? 2 : 4) % 32 == 0;
 }
 
+template <int kBits, typename T>
+int launch_quantize_rows_of(const void* x, bool wide, int64_t ld, const Mx4Gather& from, int32_t rows, int32_t k,
+                            const AxmSegment* segments, int32_t num_segments, void* codes, void* scales,
+                            int32_t* status, cudaStream_t st) {
+  const RowLaunch l = row_launch(rows, k);
+  auto* kernel = wide ? mx_quantize_rows_kernel<kBits, T, true> : mx_quantize_rows_kernel<kBits, T, false>;
+  kernel<<<l.grid, 256, 0, st>>>(static_cast<const T*>(x), ld, from, rows, k, l.log_wpr, segments, num_segments,
+                                 static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), status);
+  return check_launch("mx_quantize_rows_kernel");
+}
 template <int kBits>
 int launch_quantize_rows(const void* x, int32_t dtype, int64_t ld, const Mx4Gather& from, int32_t rows, int32_t k,
                          const AxmSegment* segments, int32_t num_segments, void* codes, void* scales,
                          int32_t* status, cudaStream_t st) {
-  const unsigned grid = row_grid(rows, k);
-  uint8_t* c = static_cast<uint8_t*>(codes);
-  uint8_t* s = static_cast<uint8_t*>(scales);
-  if (dtype == AXM_DTYPE_BF16)
-    mx_quantize_rows_kernel<kBits, __nv_bfloat16><<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(x), ld, from,
-                                                                       rows, k, segments, num_segments, c, s, status);
-  else
-    mx_quantize_rows_kernel<kBits, float><<<grid, 256, 0, st>>>(static_cast<const float*>(x), ld, from, rows, k, segments,
-                                                                num_segments, c, s, status);
-  return check_launch("mx_quantize_rows_kernel");
+  const bool wide = rows_at_32(x, ld, dtype);
+  return dtype == AXM_DTYPE_BF16
+             ? launch_quantize_rows_of<kBits, __nv_bfloat16>(x, wide, ld, from, rows, k, segments, num_segments, codes, scales, status, st)
+             : launch_quantize_rows_of<kBits, float>(x, wide, ld, from, rows, k, segments, num_segments, codes, scales, status, st);
 }
 
+template <int kBits, typename T>
+int launch_dequantize_rows_of(const void* codes, const void* scales, int32_t rows, int32_t k, const AxmSegment* segments,
+                              int32_t num_segments, void* out, bool wide, int64_t ld, cudaStream_t st) {
+  const RowLaunch l = row_launch(rows, k);
+  auto* kernel = wide ? mx_dequantize_rows_kernel<kBits, T, true> : mx_dequantize_rows_kernel<kBits, T, false>;
+  kernel<<<l.grid, 256, 0, st>>>(static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, k,
+                                 l.log_wpr, segments, num_segments, static_cast<T*>(out), ld);
+  return check_launch("mx_dequantize_rows_kernel");
+}
 template <int kBits>
 int launch_dequantize_rows(const void* codes, const void* scales, int32_t rows, int32_t k, const AxmSegment* segments,
                            int32_t num_segments, void* out, int32_t dtype, int64_t ld, cudaStream_t st) {
-  const unsigned grid = row_grid(rows, k);
-  const uint8_t* c = static_cast<const uint8_t*>(codes);
-  const uint8_t* s = static_cast<const uint8_t*>(scales);
-  if (dtype == AXM_DTYPE_BF16)
-    mx_dequantize_rows_kernel<kBits, __nv_bfloat16><<<grid, 256, 0, st>>>(c, s, rows, k, segments, num_segments,
-                                                                         static_cast<__nv_bfloat16*>(out), ld);
-  else
-    mx_dequantize_rows_kernel<kBits, float><<<grid, 256, 0, st>>>(c, s, rows, k, segments, num_segments,
-                                                                  static_cast<float*>(out), ld);
-  return check_launch("mx_dequantize_rows_kernel");
+  const bool wide = rows_at_32(out, ld, dtype);
+  return dtype == AXM_DTYPE_BF16
+             ? launch_dequantize_rows_of<kBits, __nv_bfloat16>(codes, scales, rows, k, segments, num_segments, out, wide, ld, st)
+             : launch_dequantize_rows_of<kBits, float>(codes, scales, rows, k, segments, num_segments, out, wide, ld, st);
 }
 
 }  // namespace
@@ -494,9 +611,9 @@ extern "C" int axm_mx4_dequantize_weights(const void* codes, const void* scales,
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   const uint8_t* s = static_cast<const uint8_t*>(scales);
   if (w_dtype == AXM_DTYPE_BF16)
-    mx4_dequantize_weights_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(c, s, k, n, static_cast<__nv_bfloat16*>(w));
+    mx4_dequantize_weights_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(c, s, k, n, static_cast<__nv_bfloat16*>(w));
   else
-    mx4_dequantize_weights_kernel<float><<<grid, 256, 0, st>>>(c, s, k, n, static_cast<float*>(w));
+    mx4_dequantize_weights_kernel<float><<<grid, 128, 0, st>>>(c, s, k, n, static_cast<float*>(w));
   return check_launch("mx4_dequantize_weights_kernel");
 }
 

@@ -91,12 +91,38 @@ __device__ __forceinline__ uint32_t mx4_pack8(const float (&v)[8]) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
-// The magnitude of an e2m1 code in fp32: 0 0.5 1 1.5 2 3 4 6 (with its sign).
-__device__ __forceinline__ float mx4_code_value(uint32_t code) {
-  const uint32_t m = code & 7u;
-  // exponent field and mantissa bit moved to fp32's places; the one subnormal (0.5) by hand
-  const uint32_t bits = m > 1u ? ((m << 22) + (126u << 23)) : (m ? 0x3f000000u : 0u);
-  return __uint_as_float(bits | ((code & 8u) << 28));
+// Reading back.  What a block holds is exact in bf16 (at most four significant bits, bf16 has the
+// exponents of fp32), so codes are decoded two at a time: their exponent and mantissa bits moved to
+// bf16's places are the value times 2^-126 (e2m1) or 2^-120 (e4m3), subnormal codes included, and
+// two packed multiplications by powers of two put that right.  Half the instructions of decoding
+// one by one in fp32, which is what bounded the kernels that read blocks back.
+__device__ __forceinline__ uint32_t mx_scale_bf16x2(uint32_t s) {  // 2^(s - 127), twice
+  const uint32_t h = s == 255u ? 0x7fc0u : (s == 0u ? 0x0040u : s << 7);
+  return h * 0x10001u;
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Eight e2m1 codes to four bf16 pairs.
+__device__ __forceinline__ void mx4_decode8(uint32_t codes, uint32_t scale2, uint32_t (&out)[4]) {
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const uint32_t c = (codes >> (8 * p)) & 0xffu;
+    const uint32_t x = c | (c << 12);  // the two codes at bits 0 and 16
+    const uint32_t t = ((x << 6) & 0x01c001c0u) | ((x << 12) & 0x80008000u);
+    out[p] = mul_bf16x2(mul_bf16x2(t, 0x7e807e80u), scale2);
+  }
+}
+// Four e4m3 codes to two bf16 pairs.
+__device__ __forceinline__ void mx8_decode4(uint32_t codes, uint32_t scale2, uint32_t& lo, uint32_t& hi) {
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const uint32_t x = __byte_perm(codes, 0, p ? 0x4342 : 0x4140);  // a code in each half
+    const uint32_t t = ((x << 4) & 0x07f007f0u) | ((x << 8) & 0x80008000u);
+    (p ? hi : lo) = mul_bf16x2(mul_bf16x2(t, 0x7b807b80u), scale2);
+  }
 }
 
 // Four values to four e4m3 codes, value 0 in the lowest byte.

@@ -29,15 +29,40 @@ def _dtype(t):
     return _DTYPES[t]
 
 
+class _Here:
+    """The tensors' device is the current one already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
 def _on(device):
     """The library enqueues on the current device: make it the tensors'."""
-    return torch.cuda.device(device)
+    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _rows_of(x):
-    if not x.is_cuda or x.dim() != 2 or x.stride(1) != 1:
+    if not x.is_cuda or x.dim() != 2:
         raise ValueError("a CUDA matrix with contiguous rows is needed")
-    return x.shape[0], x.shape[1], x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
+    rows, k = x.shape
+    ld, one = x.stride()
+    if one != 1 and k > 1:
+        raise ValueError("a CUDA matrix with contiguous rows is needed")
+    return rows, k, ld if rows > 1 else max(ld, k)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _up(n, to):
+    return (n + to - 1) // to * to
 
 
 def _bytes(call, *args):
@@ -47,10 +72,19 @@ def _bytes(call, *args):
 
 
 class Mx4Rows:
-    """Rows in 4 bits: codes [rows][K/2], tile-ordered scales, the segment table they follow."""
+    """Rows in 4 bits: codes [rows][K/2], tile-ordered scales, the segment table they follow.  Both
+    lie in one buffer, the scales from `scales_at` on."""
 
-    def __init__(self, codes, scales, rows, k, segments=None):
-        self.codes, self.scales, self.rows, self.k, self.segments = codes, scales, rows, k, segments
+    def __init__(self, buffer, scales_at, rows, k, segments=None):
+        self.buffer, self.scales_at, self.rows, self.k, self.segments = buffer, scales_at, rows, k, segments
+
+    @property
+    def codes(self):
+        return self.buffer[:self.rows * (self.k // 2)].view(self.rows, self.k // 2)
+
+    @property
+    def scales(self):
+        return self.buffer[self.scales_at:]
 
 
 class Mx4Weights:
@@ -74,7 +108,8 @@ class Mx4Weights:
         _, size = _bytes(lib.axm_mx4_weights_bytes, e, k, n)
         with _on(codes.device):
             packed = torch.empty(size, dtype=torch.uint8, device=codes.device)
-            _pkg.check(lib.axm_mx4_pack_scales(_pkg.ptr(scales), e, k, n, _pkg.ptr(packed), _pkg.current_stream()))
+            _pkg.check(lib.axm_mx4_pack_scales(scales.data_ptr(), e, k, n, packed.data_ptr(),
+                                               _pkg.raw_stream(codes.device.index)))
         return cls(codes, packed, e, k, n)
 
 
@@ -84,27 +119,33 @@ def quantize_rows(x, segments=None, row_src=None, row_div=1):
     src_rows, k, ld = _rows_of(x)
     rows = src_rows if row_src is None else row_src.numel()
     nseg = 0 if segments is None else segments.shape[0]
-    n_codes, n_scales = _bytes(lib.axm_mx4_rows_bytes, rows, nseg, k)
-    with _on(x.device):
-        codes = torch.empty(rows, k // 2, dtype=torch.uint8, device=x.device)
-        scales = torch.empty(n_scales, dtype=torch.uint8, device=x.device)
-        _pkg.check(lib.axm_mx4_quantize_rows(_pkg.ptr(x), _dtype(x.dtype), ld, _pkg.ptr(row_src), row_div, rows, k,
-                                             _pkg.ptr(segments), nseg, _pkg.ptr(codes), _pkg.ptr(scales),
-                                             _pkg.current_stream()))
-    return Mx4Rows(codes, scales, rows, k, segments)
+    # the sizes of axm_mx4_rows_bytes; sizes that it refuses are refused by the call below
+    at = _up(rows * (k // 2), 256)
+    size = at + (rows // 128 + max(nseg, 1)) * (_up(max(k, 0), 256) // 128) * 512
+    device = x.device
+    with _on(device):
+        buffer = torch.empty(size, dtype=torch.uint8, device=device)
+        base = buffer.data_ptr()
+        _pkg.check(lib.axm_mx4_quantize_rows(x.data_ptr(), _dtype(x.dtype), ld, _address(row_src), row_div, rows, k,
+                                             _address(segments), nseg, base, base + at, _pkg.raw_stream(device.index)))
+    return Mx4Rows(buffer, at, rows, k, segments)
 
 
 def dequantize_rows(q, dtype=torch.bfloat16, out=None):
     lib = _pkg.load()
-    with _on(q.codes.device):
+    device, rows, k, ld = q.buffer.device, q.rows, q.k, q.k
+    with _on(device):
         if out is None:
-            out = torch.empty(q.rows, q.k, dtype=dtype, device=q.codes.device)
-        rows, k, ld = _rows_of(out)
-        if (rows, k) != (q.rows, q.k):
-            raise ValueError(f"out is {tuple(out.shape)}, the rows are {(q.rows, q.k)}")
+            out = torch.empty((rows, k), dtype=dtype, device=device)
+        else:
+            got = _rows_of(out)
+            if got[:2] != (rows, k) or out.device != device:
+                raise ValueError(f"out is {tuple(out.shape)} on {out.device}, the rows are {(rows, k)} on {device}")
+            ld = got[2]
         nseg = 0 if q.segments is None else q.segments.shape[0]
-        _pkg.check(lib.axm_mx4_dequantize_rows(_pkg.ptr(q.codes), _pkg.ptr(q.scales), rows, k, _pkg.ptr(q.segments), nseg,
-                                               _pkg.ptr(out), _dtype(out.dtype), ld, _pkg.current_stream()))
+        base = q.buffer.data_ptr()
+        _pkg.check(lib.axm_mx4_dequantize_rows(base, base + q.scales_at, rows, k, _address(q.segments), nseg,
+                                               out.data_ptr(), _dtype(out.dtype), ld, _pkg.raw_stream(device.index)))
     return out
 
 
@@ -112,21 +153,26 @@ def quantize_rows8(x):
     """x [rows][K] to 8 bits: codes [rows][K] (e4m3), scale bytes [rows][K/32]."""
     lib = _pkg.load()
     rows, k, ld = _rows_of(x)
-    with _on(x.device):
-        codes = torch.empty(rows, k, dtype=torch.uint8, device=x.device)
-        scales = torch.empty(rows, k // 32, dtype=torch.uint8, device=x.device)
-        _pkg.check(lib.axm_mx8_quantize_rows(_pkg.ptr(x), _dtype(x.dtype), ld, rows, k, _pkg.ptr(codes), _pkg.ptr(scales),
-                                             _pkg.current_stream()))
+    device = x.device
+    with _on(device):
+        codes = torch.empty((rows, k), dtype=torch.uint8, device=device)
+        scales = torch.empty((rows, k // 32), dtype=torch.uint8, device=device)
+        _pkg.check(lib.axm_mx8_quantize_rows(x.data_ptr(), _dtype(x.dtype), ld, rows, k, codes.data_ptr(),
+                                             scales.data_ptr(), _pkg.raw_stream(device.index)))
     return codes, scales
 
 
 def dequantize_rows8(codes, scales, dtype=torch.bfloat16):
     lib = _pkg.load()
     rows, k = codes.shape
-    with _on(codes.device):
-        out = torch.empty(rows, k, dtype=dtype, device=codes.device)
-        _pkg.check(lib.axm_mx8_dequantize_rows(_pkg.ptr(codes), _pkg.ptr(scales), rows, k, _pkg.ptr(out), _dtype(dtype), k,
-                                               _pkg.current_stream()))
+    device = codes.device
+    if not (codes.is_contiguous() and scales.is_contiguous() and scales.shape == (rows, k // 32) and scales.device == device
+            and codes.dtype == scales.dtype == torch.uint8):
+        raise ValueError("contiguous uint8 codes [rows][K] and scales [rows][K/32] on one device are needed")
+    with _on(device):
+        out = torch.empty((rows, k), dtype=dtype, device=device)
+        _pkg.check(lib.axm_mx8_dequantize_rows(codes.data_ptr(), scales.data_ptr(), rows, k, out.data_ptr(), _dtype(dtype),
+                                               k, _pkg.raw_stream(device.index)))
     return out
 
 
@@ -136,21 +182,23 @@ def quantize_weights(w):
     if not (w.is_cuda and w.dim() == 3 and w.is_contiguous()):
         raise ValueError("a contiguous CUDA tensor [E][K][N] is needed")
     e, k, n = w.shape
-    n_codes, n_scales = _bytes(lib.axm_mx4_weights_bytes, e, k, n)
-    with _on(w.device):
-        codes = torch.empty(e, n, k // 2, dtype=torch.uint8, device=w.device)
-        scales = torch.empty(n_scales, dtype=torch.uint8, device=w.device)
-        _pkg.check(lib.axm_mx4_quantize_weights(_pkg.ptr(w), _dtype(w.dtype), e, k, n, _pkg.ptr(codes), _pkg.ptr(scales),
-                                                _pkg.current_stream()))
+    device = w.device
+    with _on(device):
+        codes = torch.empty((e, n, k // 2), dtype=torch.uint8, device=device)
+        # the size of axm_mx4_weights_bytes; sizes that it refuses are refused by the call below
+        scales = torch.empty(e * (_up(n, 128) // 128) * (_up(k, 256) // 128) * 512, dtype=torch.uint8, device=device)
+        _pkg.check(lib.axm_mx4_quantize_weights(w.data_ptr(), _dtype(w.dtype), e, k, n, codes.data_ptr(), scales.data_ptr(),
+                                                _pkg.raw_stream(device.index)))
     return Mx4Weights(codes, scales, e, k, n)
 
 
 def dequantize_weights(q, dtype=torch.bfloat16):
     lib = _pkg.load()
-    with _on(q.codes.device):
-        w = torch.empty(q.experts, q.k, q.n, dtype=dtype, device=q.codes.device)
-        _pkg.check(lib.axm_mx4_dequantize_weights(_pkg.ptr(q.codes), _pkg.ptr(q.scales), q.experts, q.k, q.n, _pkg.ptr(w),
-                                                  _dtype(dtype), _pkg.current_stream()))
+    device = q.codes.device
+    with _on(device):
+        w = torch.empty((q.experts, q.k, q.n), dtype=dtype, device=device)
+        _pkg.check(lib.axm_mx4_dequantize_weights(q.codes.data_ptr(), q.scales.data_ptr(), q.experts, q.k, q.n, w.data_ptr(),
+                                                  _dtype(dtype), _pkg.raw_stream(device.index)))
     return w
 
 
@@ -187,10 +235,12 @@ class Mx4Linear(_Workspace):
             out = torch.empty(rows, w.n, dtype=dtype, device=x.device)
         elif out.shape != (rows, w.n) or not out.is_contiguous() or out.device != x.device:
             raise ValueError("out must be a contiguous [rows][N] matrix beside x")
-        with _on(x.device):
-            _pkg.check(self.lib.axm_mx4_linear(_pkg.ptr(x), _dtype(x.dtype), ld, rows, k, w.n, _pkg.ptr(w.codes),
-                                               _pkg.ptr(w.scales), _pkg.ptr(out), _dtype(out.dtype),
-                                               _pkg.ptr(self.workspace), self.workspace.numel(), _pkg.current_stream()))
+        device = x.device
+        with _on(device):
+            _pkg.check(self.lib.axm_mx4_linear(x.data_ptr(), _dtype(x.dtype), ld, rows, k, w.n, w.codes.data_ptr(),
+                                               w.scales.data_ptr(), out.data_ptr(), _dtype(out.dtype),
+                                               self.workspace.data_ptr(), self.workspace.numel(),
+                                               _pkg.raw_stream(device.index)))
         return out
 
 
@@ -230,10 +280,10 @@ class Mx4ExpertFfn(_Workspace):
         elif out.shape != x.shape or not out.is_contiguous() or out.device != dev:
             raise ValueError("out must be a contiguous matrix like x")
         with _on(dev):
-            _pkg.check(self.lib.axm_mx4_expert_ffn(ctypes.byref(self.desc), _pkg.ptr(x), rows, _pkg.ptr(segments),
-                                                   segments.shape[0], ctypes.byref(self.table), _pkg.ptr(out),
-                                                   _dtype(out.dtype), _pkg.ptr(self.workspace), self.workspace.numel(),
-                                                   _pkg.current_stream()))
+            _pkg.check(self.lib.axm_mx4_expert_ffn(ctypes.byref(self.desc), x.data_ptr(), rows, segments.data_ptr(),
+                                                   segments.shape[0], ctypes.byref(self.table), out.data_ptr(),
+                                                   _dtype(out.dtype), self.workspace.data_ptr(), self.workspace.numel(),
+                                                   _pkg.raw_stream(dev.index)))
         return out
 
 
@@ -280,8 +330,8 @@ class Mx4MoeLayer(_Workspace):
         with _on(dev):
             _pkg.check(self.lib.axm_moe_forward_mx4(ctypes.byref(self.desc), ctypes.byref(t), ctypes.byref(self.experts),
                                                     None if self.shared is None else ctypes.byref(self.shared),
-                                                    _pkg.ptr(self.workspace), self.workspace.numel(),
-                                                    _pkg.current_stream()))
+                                                    self.workspace.data_ptr(), self.workspace.numel(),
+                                                    _pkg.raw_stream(dev.index)))
         return out, self.histogram
 
 
@@ -329,12 +379,12 @@ class Mx8TrainFfn:
             raise ValueError("segments: a contiguous int32 table n x 4 beside x")
         if out is None:
             out = torch.empty(x.shape, dtype=self.dtype, device=x.device)
-        p = _pkg.ptr
+        p = _address
         with _on(x.device):
             _pkg.check(self.lib.axm_mx8_expert_ffn_train(
                 ctypes.byref(self.desc), p(x), x.shape[0], p(segments), segments.shape[0], *map(p, self.weights),
                 ctypes.byref(self.keep), p(self.scratch[0]), p(out), _dtype(out.dtype), p(self.status_word),
-                _pkg.current_stream()))
+                _pkg.raw_stream(x.device.index)))
         self.saved = (x, segments)
         return out
 
@@ -346,7 +396,7 @@ class Mx8TrainFfn:
         self._check(d_o, "d_o")
         if d_o.shape != x.shape:
             raise ValueError(f"d_o {tuple(d_o.shape)} is not like x {tuple(x.shape)}")
-        p = _pkg.ptr
+        p = _address
         grads = {"d_x": torch.empty(x.shape, dtype=self.dtype, device=x.device)}
         if weight_grads:
             for n, w in zip(("d_gate", "d_up", "d_down"), self.weights):
@@ -356,5 +406,5 @@ class Mx8TrainFfn:
                 ctypes.byref(self.desc), p(x), x.shape[0], p(segments), segments.shape[0], ctypes.byref(self.keep), p(d_o),
                 *map(p, self.weights), *map(p, self.scratch), p(grads["d_x"]), p(grads.get("d_gate")),
                 p(grads.get("d_up")), p(grads.get("d_down")), _dtype(self.dtype), p(self.status_word),
-                _pkg.current_stream()))
+                _pkg.raw_stream(x.device.index)))
         return grads
