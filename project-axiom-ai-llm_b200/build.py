@@ -18,7 +18,7 @@ DROPIN = os.path.join(HERE, "libaxm_moe_dropin.so")
 CORE_SOURCES = ["moe_api.cu", "router.cu", "router_tc.cu", "permute.cu", "grouped_ffn.cu", "noalloc.cu",
                 "ep_exchange.cu", "ep_layer.cu", "ep_train.cu", "grouped_bwd.cu", "backward.cu",
                 "grouped_ffn_2sm.cu", "grouped_bwd_2sm.cu", "checkpoint.cu",
-                "microscale.cu", "mx4_gemm.cu", "mx4_layer.cu", "mx8_train.cu"]
+                "microscale.cu", "mx4_gemm.cu", "mx4_few.cu", "mx4_layer.cu", "mx8_train.cu"]
 DROPIN_SOURCES = ["dropin.cu"]
 
 NVCC_FLAGS = [

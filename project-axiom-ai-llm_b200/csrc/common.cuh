@@ -195,6 +195,21 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
                    smem_u32(bar))
                : "memory");
 }
+// One lane of a converged warp, always the same one.  A loop that feeds the tensor core is run by
+// its whole warp, with only the tcgen05 instructions behind this: descriptors and addresses are then
+// the warp's (uniform registers, which is where those instructions take them from) and not one
+// lane's, which costs a move each.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(yes));
+  return yes != 0;
+}
 // D[tmem] (+)= A[smem] * B[smem], bf16 inputs, fp32 accumulate, one CTA.
 __device__ __forceinline__ void tc_mma_bf16(uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b,
                                             uint32_t idesc, uint32_t accumulate) {

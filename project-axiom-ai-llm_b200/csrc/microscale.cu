@@ -47,6 +47,13 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
 // and wrote 3.9 TB/s.
 constexpr int kAhead = 2;
 
+// What the first kernel of a call clears for the ones behind it.
+struct MxClear {
+  int32_t* status;
+  uint32_t* counters;
+  int num_counters;
+};
+
 // kBits = 4: scale bytes in tile order, the row's last, partial stage padded with zero bytes.
 // kBits = 8: codes [rows][K], scale bytes [rows][K / 32].
 // kWide: rows start at multiples of 32 bytes.
@@ -55,8 +62,13 @@ template <int kBits, typename T, bool kWide>
 __global__ void __launch_bounds__(256)
 mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, int rows, int k, int log_wpr,
                         const AxmSegment* __restrict__ segments, int num_segments,
-                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int32_t* status) {
-  if (status != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
+                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, MxClear clear) {
+  // a product that is launched to start early may prepare itself now; it waits before it reads
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (blockIdx.x == 0) {
+    if (clear.status != nullptr && threadIdx.x == 0) *clear.status = 0;
+    for (int i = threadIdx.x; i < clear.num_counters; i += 256) clear.counters[i] = 0u;
+  }
   constexpr bool kBf16 = sizeof(T) == 2;
   constexpr int kWords = kBf16 ? 1 : 2;  // 32-byte pieces a lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -446,21 +458,21 @@ bool rows_at_32(const void* p, int64_t ld, int32_t dtype) {
 template <int kBits, typename T>
 int launch_quantize_rows_of(const void* x, bool wide, int64_t ld, const Mx4Gather& from, int32_t rows, int32_t k,
                             const AxmSegment* segments, int32_t num_segments, void* codes, void* scales,
-                            int32_t* status, cudaStream_t st) {
+                            const MxClear& clear, cudaStream_t st) {
   const RowLaunch l = row_launch(rows, k);
   auto* kernel = wide ? mx_quantize_rows_kernel<kBits, T, true> : mx_quantize_rows_kernel<kBits, T, false>;
   kernel<<<l.grid, 256, 0, st>>>(static_cast<const T*>(x), ld, from, rows, k, l.log_wpr, segments, num_segments,
-                                 static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), status);
+                                 static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), clear);
   return check_launch("mx_quantize_rows_kernel");
 }
 template <int kBits>
 int launch_quantize_rows(const void* x, int32_t dtype, int64_t ld, const Mx4Gather& from, int32_t rows, int32_t k,
                          const AxmSegment* segments, int32_t num_segments, void* codes, void* scales,
-                         int32_t* status, cudaStream_t st) {
+                         const MxClear& clear, cudaStream_t st) {
   const bool wide = rows_at_32(x, ld, dtype);
   return dtype == AXM_DTYPE_BF16
-             ? launch_quantize_rows_of<kBits, __nv_bfloat16>(x, wide, ld, from, rows, k, segments, num_segments, codes, scales, status, st)
-             : launch_quantize_rows_of<kBits, float>(x, wide, ld, from, rows, k, segments, num_segments, codes, scales, status, st);
+             ? launch_quantize_rows_of<kBits, __nv_bfloat16>(x, wide, ld, from, rows, k, segments, num_segments, codes, scales, clear, st)
+             : launch_quantize_rows_of<kBits, float>(x, wide, ld, from, rows, k, segments, num_segments, codes, scales, clear, st);
 }
 
 template <int kBits, typename T>
@@ -486,7 +498,7 @@ int launch_dequantize_rows(const void* codes, const void* scales, int32_t rows, 
 int launch_mx4_quantize_rows(const void* x, int32_t dtype, int64_t ld, const Mx4Gather& from, const Mx4Rows& rows, int k,
                              void* codes, void* scales, cudaStream_t st) {
   return launch_quantize_rows<4>(x, dtype, ld, from, rows.rows, k, rows.segments, rows.num_segments, codes, scales,
-                                 rows.status, st);
+                                 MxClear{rows.status, rows.few_counters, rows.few_counters ? mx4_few_counters() : 0}, st);
 }
 
 int check_mx_matrix(const void* p, int32_t dtype, int64_t ld, int32_t k, const char* what) {
@@ -529,7 +541,7 @@ extern "C" int axm_mx4_quantize_rows(const void* x, int32_t x_dtype, int64_t ld,
   if (int rc = require_device()) return rc;
   const Mx4Gather from = {row_src, row_div, rows, 1};
   return launch_quantize_rows<4>(x, x_dtype, ld, from, rows, k, segments, num_segments, codes, scales,
-                                 nullptr, static_cast<cudaStream_t>(stream));
+                                 MxClear{}, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int axm_mx4_dequantize_rows(const void* codes, const void* scales, int32_t rows, int32_t k,
@@ -559,7 +571,7 @@ extern "C" int axm_mx8_quantize_rows(const void* x, int32_t x_dtype, int64_t ld,
   if (misaligned(codes, 16)) return fail(AXM_ERR_ARGUMENT, "%s: codes must be 16-byte aligned", what);
   if (int rc = require_device()) return rc;
   const Mx4Gather from = {nullptr, 1, rows, 1};
-  return launch_quantize_rows<8>(x, x_dtype, ld, from, rows, k, nullptr, 0, codes, scales, nullptr,
+  return launch_quantize_rows<8>(x, x_dtype, ld, from, rows, k, nullptr, 0, codes, scales, MxClear{},
                                  static_cast<cudaStream_t>(stream));
 }
 

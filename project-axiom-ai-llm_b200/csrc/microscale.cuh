@@ -39,6 +39,8 @@ struct Mx4Rows {
   int expert_base;     // expert id of the first weight matrix of this launch
   int max_rows;        // most rows any segment can have (the number of tokens)
   int32_t* status;
+  float* few_partial;      // workspace of the few-rows kernels: partial tiles,
+  uint32_t* few_counters;  //   a counter a tile (zero before the first launch of a call)
 };
 
 // q4 of the rows of a bf16 or fp32 matrix (microscale.cu).  Row r < tail_row0 comes from source row
@@ -56,6 +58,15 @@ int launch_mx4_linear(const Mx4Rows& r, const void* a_codes, const void* a_scale
                       const void* w_scales, int experts, int k, int n, void* out, bool out_bf16, cudaStream_t st);
 int launch_mx4_gated(const Mx4Rows& r, const void* a_codes, const void* a_scales, const AxmMx4Experts* w, int experts,
                      int d, int f, void* h_codes, void* h_scales, cudaStream_t st);
+
+// The same for few rows a segment (mx4_few.cu), with its workspace.
+bool mx4_use_few(int max_rows);
+int mx4_few_counters();
+size_t mx4_few_partial_bytes(int max_rows, bool gated);
+int launch_mx4_linear_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, const void* w_codes,
+                          const void* w_scales, int experts, int k, int n, void* out, bool out_bf16, cudaStream_t st);
+int launch_mx4_gated_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, const AxmMx4Experts* w, int experts,
+                         int d, int f, void* h_codes, void* h_scales, cudaStream_t st);
 
 #if defined(__CUDACC__)
 

@@ -1,0 +1,650 @@
+// The 4-bit products of calls with few rows a segment (one token, a short batch, many experts): what
+// counts is how fast the weights stream in, so the roles are turned around.
+//
+// 128 weight rows are the M side of the MMA (cta_group::1), the segment's rows its N side (16, 32, 64 or
+// 128 of them, a template parameter; with 128 a segment may have several such tiles).  A stage is 256
+// reduction elements: 16 KiB of codes and 1 KiB of scale bytes for the weights (twice that for gate
+// and up), 128 bytes of codes a row for the activations.
+//
+// A unit is a weight tile (128 features) with a row tile, dealt out round robin.  An SM can pull
+// more than its share of the memory's bandwidth, so tiles that do not divide evenly among the SMs cost
+// nothing as long as the rest still are many; only where there are few (kEnough) is the reduction of
+// each cut into equal ranges, units of their own.  A cut tile is finished by the unit that arrives last
+// (a counter, nobody waits): all of them leave their partial sums in the workspace, and the last
+// adds them in the order of the reduction, so the result does not depend on who was last.
+// Cutting all work into equal pieces regardless (24 or 25 stages a CTA for a wide layer's 224 gate/up
+// tiles) was built first and lost what it gained to the partial sums: one token's product 4096 -> 14336
+// 17 us, 128 tokens 31 us.
+//
+// The accumulator has a feature a lane and a row a column.  Linear output is stored straight from
+// there (32 neighbouring features of a row).  The gated product's values are turned over through
+// shared memory, sixteen rows at a time, so that a lane holds a row's 32-block and quantises it
+// in registers as the pair kernel does.
+//
+// The weights do not depend on the kernel before: the producer asks for its first stages' weights
+// before it waits for that kernel (programmatic dependent launch), then for the activations.
+#include <cstdlib>
+
+#include "gemm_2sm.cuh"
+#include "microscale.cuh"
+
+namespace axm {
+
+namespace {
+
+constexpr int kThreadsF = 192;
+constexpr int kWCodeBytes = 128 * 128;  // 128 weight rows x 256 elements
+constexpr int kScaleChunk2 = 1024;      // two 512-byte chunks
+
+template <bool kGated, int N>
+struct FewCfg {
+  static constexpr int kWeights = kGated ? 2 : 1;
+  static constexpr int kCodeBytes = kWeights * kWCodeBytes + N * 128;
+  static constexpr int kScaleBytes = (kWeights + 1) * kScaleChunk2;
+  static constexpr int kStageBytes = kCodeBytes + kScaleBytes;
+  static constexpr int kFit = (200 * 1024) / kStageBytes;
+  static constexpr int kStages = kFit < 10 ? kFit : 10;
+  static constexpr int kAccCols = kWeights * N;
+  static constexpr int kAccs = 2 * kAccCols + 48 <= 512 ? 2 : 1;
+  static constexpr int kSf = kAccs * kAccCols;  // first scale column
+  static constexpr int kSfCols = kWeights * 8 + 8;  // weights (8 each), then rows (8)
+  static constexpr int kNeed = kSf + kSfCols;
+  static constexpr int kTmem = kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : kNeed <= 256 ? 256 : 512;
+  static constexpr int kPartial = kWeights * N * 128;  // floats of one partial tile
+};
+
+template <int kStages>
+struct __align__(8) FewShared {
+  uint64_t full[kStages];
+  uint64_t empty[kStages];
+  uint64_t tmem_full[2];
+  uint64_t tmem_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  int is_last;
+  int too_long;
+  int prefix[kMaxSegments + 1];  // row tiles before segment s
+  AxmSegment seg[kMaxSegments];
+  float turn[4][16 * 33];  // per epilogue warp: 16 rows x 32 features
+};
+
+struct FewArgs {
+  const AxmSegment* segments;
+  int num_segments;
+  int rows_total;
+  int seg_base;
+  int expert_base;
+  int n_total;
+  int k_total;
+  int wn_tiles;
+  int out_bf16;
+  void* out;
+  uint8_t* out_scales;
+  float* partial;      // [kUnitsMost] tiles
+  uint32_t* counters;  // [kEnough], zero between launches
+  int* status;
+};
+
+// Block-scaled kind::mxf4 like the pair kernel's, M = 128 of one CTA.
+template <int N>
+constexpr uint32_t few_instr_desc(uint32_t step) {
+  return ((step * 2u) << 4) | (1u << 7) | (1u << 10) | (((uint32_t)N >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24) |
+         ((step * 2u) << 29);
+}
+__device__ __forceinline__ void tc_mma1_mx4(uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                            uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_cp1_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ uint64_t few_scale_desc(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr >> 4) & 0x3fffu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Whether all 128 threads of the epilogue say yes.
+__device__ __forceinline__ bool epilogue_agree(bool yes) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.red.and.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}"
+      : "=r"(r)
+      : "r"((uint32_t)yes)
+      : "memory");
+  return r != 0;
+}
+
+struct FewTile {
+  int seg, f_tile, row_tile;
+};
+
+// One CTA's units, in order.
+struct Units {
+  long long at, end, step;
+  int splits, k_blocks, k_per;
+  __device__ bool next(long long& tile, int& kb0, int& kb1) {
+    if (at >= end) return false;
+    tile = splits == 1 ? at : at / splits;
+    kb0 = (int)(at - tile * splits) * k_per;
+    kb1 = kb0 + k_per < k_blocks ? kb0 + k_per : k_blocks;
+    at += step;
+    return true;
+  }
+};
+// Units below which the reduction is cut, and above which it is not cut further.
+constexpr int kEnough = 96;
+constexpr int kUnitsMost = 256;
+
+template <bool kGated, int N>
+__global__ void __launch_bounds__(kThreadsF, 1)
+mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a_sf,
+               const __grid_constant__ CUtensorMap tm_w0, const __grid_constant__ CUtensorMap tm_w1,
+               const __grid_constant__ CUtensorMap tm_w0_sf, const __grid_constant__ CUtensorMap tm_w1_sf, FewArgs args) {
+  using Cfg = FewCfg<kGated, N>;
+  constexpr int kStages = Cfg::kStages;
+  using Shared = FewShared<kStages>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* tiles = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  unsigned char* scales_s = tiles + (size_t)kStages * Cfg::kCodeBytes;
+  Shared* sh = reinterpret_cast<Shared*>(scales_s + (size_t)kStages * Cfg::kScaleBytes);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int nseg = args.num_segments;
+  const int f_tiles = (args.n_total + 127) / 128;
+  const int k_blocks = (args.k_total + 255) / 256;
+
+  // the next kernel may start its own preparations; it waits for this one before it reads
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  // The segment table is older than the kernel before this one (see the launch), so it may be read
+  // at once.
+  for (int s = threadIdx.x; s < nseg; s += kThreadsF)
+    sh->seg[s] = args.segments != nullptr ? args.segments[s] : AxmSegment{0, 0, args.rows_total, 0};
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sh->full[i], 1);
+      mbar_init(&sh->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh->tmem_full[i], 1);
+      mbar_init(&sh->tmem_empty[i], 4);
+    }
+    sh->abort_flag = 0;
+    sh->too_long = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tma_prefetch_desc(&tm_w0);
+    tma_prefetch_desc(&tm_w0_sf);
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_a_sf);
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc(&sh->tmem_base, Cfg::kTmem);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  if (warp == 0) {  // row tiles before each segment
+    int before = 0;
+    for (int s0 = 0; s0 < nseg; s0 += 32) {
+      const int s = s0 + lane;
+      const int rows = s < nseg ? sh->seg[s].rows : 0;
+      const int mine = rows > 0 ? (rows + N - 1) / N : 0;
+      if (N < 128 && mine > 1) sh->too_long = 1;
+      int sum = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += v;
+      }
+      if (s < nseg) sh->prefix[s] = before + sum - mine;
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) sh->prefix[nseg] = before;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  const uint32_t tmem_base = sh->tmem_base;
+  volatile int* abort_flag = &sh->abort_flag;
+  const long long tiles_n = (long long)sh->prefix[nseg] * f_tiles;
+  int k_per = k_blocks;
+  if (tiles_n > 0 && tiles_n < kEnough) {
+    // the last to arrive reads every range's partial tile: the larger they are, the fewer
+    const int want = min(min((int)(kEnough + tiles_n - 1) / (int)tiles_n, k_blocks), 256 / N);
+    k_per = (k_blocks + want - 1) / want;
+  }
+  const int splits = (k_blocks + k_per - 1) / k_per;  // none of the ranges is empty
+  const Units mine = {(long long)blockIdx.x, tiles_n * splits, (long long)gridDim.x, splits, k_blocks, k_per};
+
+  // tiles: segment by segment, weight tile by weight tile, row tiles innermost
+  auto decode = [&](long long tile) {
+    int lo = 0, hi = nseg - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((long long)sh->prefix[mid] * f_tiles <= tile) lo = mid; else hi = mid - 1;
+    }
+    const int row_tiles = sh->prefix[lo + 1] - sh->prefix[lo];
+    const int local = (int)(tile - (long long)sh->prefix[lo] * f_tiles);
+    FewTile t;
+    t.seg = lo;
+    t.f_tile = local / row_tiles;
+    t.row_tile = local - t.f_tile * row_tiles;
+    return t;
+  };
+
+  if (warp == 0) {
+    // ---- producer --------------------------------------------------------------------------
+    if (lane == 0) {
+      auto weights = [&](int stage, const FewTile& t, int kb) {
+        const int e = (sh->seg[t.seg].expert & 0xffff) - args.expert_base;
+        unsigned char* codes = tiles + (size_t)stage * Cfg::kCodeBytes;
+        unsigned char* sf = scales_s + (size_t)stage * Cfg::kScaleBytes;
+        uint64_t* bar = &sh->full[stage];
+        mbar_expect_tx(bar, Cfg::kStageBytes);
+        tma_load_3d(codes, &tm_w0, bar, kb * 128, t.f_tile * 128, e);
+        tma_load_3d(sf, &tm_w0_sf, bar, 0, kb * 2, e * args.wn_tiles + t.f_tile);
+        if constexpr (kGated) {
+          tma_load_3d(codes + kWCodeBytes, &tm_w1, bar, kb * 128, t.f_tile * 128, e);
+          tma_load_3d(sf + kScaleChunk2, &tm_w1_sf, bar, 0, kb * 2, e * args.wn_tiles + t.f_tile);
+        }
+      };
+      auto rows = [&](int stage, const FewTile& t, int kb) {
+        const AxmSegment sg = sh->seg[t.seg];
+        unsigned char* codes = tiles + (size_t)stage * Cfg::kCodeBytes + Cfg::kWeights * kWCodeBytes;
+        unsigned char* sf = scales_s + (size_t)stage * Cfg::kScaleBytes + Cfg::kWeights * kScaleChunk2;
+        uint64_t* bar = &sh->full[stage];
+        tma_load_3d(codes, &tm_a, bar, kb * 128, sg.out_row0 + t.row_tile * N, 0);
+        tma_load_3d(sf, &tm_a_sf, bar, 0, kb * 2,
+                    sg.out_row0 / 128 + args.seg_base + t.seg + t.row_tile * N / 128);
+      };
+      Units p = mine, q = mine;  // q: the activations of the stages p has asked weights for
+      long long tile;
+      int kb0, kb1;
+      int ahead = 0;
+      // the first ring of weights, before the kernel before this one has finished
+      bool waited = false;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      while (ok && p.next(tile, kb0, kb1)) {
+        const FewTile t = decode(tile);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!waited && ahead == kStages) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            waited = true;
+            int n = 0;
+            long long t2;
+            int b0, b1;
+            while (n < ahead && q.next(t2, b0, b1)) {
+              const FewTile u = decode(t2);
+              for (int b = b0; b < b1 && n < ahead; ++b, ++n) rows(n, u, b);
+            }
+          }
+          if (waited && !mbar_wait(&sh->empty[stage], phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          weights(stage, t, kb);
+          if (waited) rows(stage, t, kb); else ++ahead;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!waited) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        int n = 0;
+        long long t2;
+        int b0, b1;
+        while (n < ahead && q.next(t2, b0, b1)) {
+          const FewTile u = decode(t2);
+          for (int b = b0; b < b1 && n < ahead; ++b, ++n) rows(n, u, b);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer (the whole warp, one elected lane issues) -------------------------------------
+    {
+      const uint64_t codes0 = make_smem_desc(smem_u32(tiles), 16, 1024);
+      const uint64_t scales0 = few_scale_desc(smem_u32(scales_s));
+      const uint32_t sf_w = tmem_base + Cfg::kSf, sf_a = sf_w + Cfg::kWeights * 8;
+      int stage = 0;
+      uint32_t phase = 0;
+      Units p = mine;
+      long long tile;
+      int kb0, kb1;
+      bool ok = true;
+      for (int i = 0; ok && p.next(tile, kb0, kb1); ++i) {
+        const int acc = Cfg::kAccs == 2 ? (i & 1) : 0;
+        const uint32_t turn = Cfg::kAccs == 2 ? (uint32_t)(i >> 1) : (uint32_t)i;
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh->tmem_empty[acc], (turn & 1u) ^ 1u, abort_flag))) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)acc * Cfg::kAccCols;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&sh->full[stage], phase, abort_flag))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          // descriptors count in 16-byte units
+          const uint64_t dw = codes0 + (uint64_t)(stage * (Cfg::kCodeBytes / 16));
+          const uint64_t dr = dw + Cfg::kWeights * kWCodeBytes / 16;
+          const uint64_t sf = scales0 + (uint64_t)(stage * (Cfg::kScaleBytes / 16));
+          if (elect_one()) {
+#pragma unroll
+            for (int w = 0; w < Cfg::kWeights + 1; ++w)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) tc_cp1_scales(sf_w + w * 8 + c * 4, sf + (w * kScaleChunk2 + c * 512) / 16);
+#pragma unroll
+            for (int w = 0; w < Cfg::kWeights; ++w)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                tc_mma1_mx4(d_tmem + w * N, dw + (uint64_t)(w * (kWCodeBytes / 16) + j * 2), dr + (uint64_t)(j * 2),
+                            few_instr_desc<N>(j & 1), sf_w + w * 8 + 4 * (j >> 1), sf_a + 4 * (j >> 1),
+                            (kb > kb0 || j > 0) ? 1u : 0u);
+            tc_commit(&sh->empty[stage]);
+          }
+          __syncwarp();
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) {
+          if (elect_one()) tc_commit(&sh->tmem_full[acc]);
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    // ---- epilogue --------------------------------------------------------------------------------
+    const int quad = warp & 3;
+    float* turn_s = sh->turn[warp - 2];
+    const int feature = quad * 32 + lane;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // outputs and partial sums of earlier launches
+    // a scale tile's rows from the sixteenth (32nd, 64th) on cannot be addressed as a tile of their
+    // own: a table whose segments are longer than the call was told is reported
+    if (sh->too_long && threadIdx.x == 64 && args.status != nullptr) atomicExch(args.status, 15);
+    Units p = mine;
+    long long tile;
+    int kb0, kb1;
+    for (int i = 0; p.next(tile, kb0, kb1); ++i) {
+      const int acc = Cfg::kAccs == 2 ? (i & 1) : 0;
+      const uint32_t turn = Cfg::kAccs == 2 ? (uint32_t)(i >> 1) : (uint32_t)i;
+      const FewTile t = decode(tile);
+      const AxmSegment sg = sh->seg[t.seg];
+      const int rows = min(sg.rows - t.row_tile * N, N);
+      // the four warps go on or give up together: they meet at barriers below
+      if (!epilogue_agree(mbar_wait(&sh->tmem_full[acc], turn & 1u, abort_flag))) break;
+      tc_fence_after();
+      const uint32_t t_addr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)acc * Cfg::kAccCols;
+      const bool whole = splits == 1;
+      bool finish = true;
+      if (!whole) {
+        // at most kUnitsMost units where tiles are cut
+        float* mine_p = args.partial + (size_t)(tile * splits + kb0 / k_per) * Cfg::kPartial;
+#pragma unroll 1
+        for (int n0 = 0; n0 < rows; n0 += 16) {
+#pragma unroll
+          for (int w = 0; w < Cfg::kWeights; ++w) {
+            uint32_t v[16];
+            __syncwarp();
+            tmem_ld16(t_addr + w * N + n0, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (n0 + j < rows) __stcg(mine_p + (size_t)(w * N + n0 + j) * 128 + feature, __uint_as_float(v[j]));
+          }
+        }
+        __threadfence();
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (threadIdx.x == 64) {
+          const uint32_t before = atomicAdd(args.counters + tile, 1u);
+          const bool last = before == (uint32_t)(splits - 1);
+          if (last) args.counters[tile] = 0u;
+          sh->is_last = last ? 1 : 0;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        finish = sh->is_last != 0;
+        if (finish) __threadfence();
+      }
+      if (finish) {
+        // sixteen rows at a time: from tensor memory, or the sum of the pieces' partial tiles
+        auto fetch = [&](int w, int n0, float (&v)[16]) {
+          if (whole) {
+            uint32_t r[16];
+            __syncwarp();
+            tmem_ld16(t_addr + w * N + n0, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+            const float* q = args.partial + (size_t)(tile * splits) * Cfg::kPartial + (size_t)(w * N + n0) * 128 + feature;
+#pragma unroll 2
+            for (int z = 0; z < splits; ++z, q += Cfg::kPartial) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (n0 + j < rows) v[j] += __ldcg(q + j * 128);
+            }
+          }
+        };
+        const int f0 = t.f_tile * 128 + quad * 32;  // this warp's 32 features
+        const size_t row0 = (size_t)sg.out_row0 + t.row_tile * N;
+#pragma unroll 1
+        for (int n0 = 0; n0 < rows; n0 += 16) {
+          if constexpr (kGated) {
+            float g[16], u[16];
+            fetch(0, n0, g);
+            fetch(1, n0, u);
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) turn_s[j * 33 + lane] = __fdividef(g[j], 1.0f + __expf(-g[j])) * u[j];
+            __syncwarp();
+            // lane j: row n0 + j, its 32 features a block (n_total is a multiple of 32)
+            if (lane < 16 && n0 + lane < rows && f0 < args.n_total) {
+              float h[32];
+              uint32_t top = 0;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                h[j] = turn_s[lane * 33 + j];
+                top = max(top, __float_as_uint(h[j]) & 0x7fffffffu);
+              }
+              const uint32_t byte = mx_scale_byte<2>(top);
+              const float inv = mx_inverse_scale(byte);
+              uint32_t q[4];
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = h[8 * b + j] * inv;
+                q[b] = mx4_pack8(x);
+              }
+              const size_t row = row0 + n0 + lane;
+              *reinterpret_cast<uint4*>(static_cast<uint8_t*>(args.out) + row * (size_t)(args.n_total >> 1) + (f0 >> 1)) =
+                  make_uint4(q[0], q[1], q[2], q[3]);
+              const int r = t.row_tile * N + n0 + lane;  // row of the segment
+              const int chunks = mx4_chunks(args.n_total);
+              uint8_t* sf = args.out_scales +
+                            ((size_t)(sg.out_row0 / 128 + args.seg_base + t.seg + r / 128) * chunks + t.f_tile) * 512 +
+                            (r & 31) * 16 + ((r & 127) >> 5) * 4;
+              sf[quad] = (uint8_t)byte;
+            }
+            // scale bytes of blocks behind F: the rest of the last chunk, and the chunk behind an odd number
+            if (lane < 16 && n0 + lane < rows && t.f_tile == f_tiles - 1) {
+              const int r = t.row_tile * N + n0 + lane;
+              const int chunks = mx4_chunks(args.n_total);
+              uint8_t* sf = args.out_scales +
+                            ((size_t)(sg.out_row0 / 128 + args.seg_base + t.seg + r / 128) * chunks + t.f_tile) * 512 +
+                            (r & 31) * 16 + ((r & 127) >> 5) * 4;
+              if (f0 >= args.n_total) sf[quad] = 0;
+              if (quad == 0 && f_tiles < chunks) *reinterpret_cast<uint32_t*>(sf + 512) = 0u;
+            }
+          } else {
+            float v[16];
+            fetch(0, n0, v);
+            if (f0 + lane < args.n_total) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (n0 + j < rows) {
+                  const size_t el = (row0 + n0 + j) * (size_t)args.n_total + f0 + lane;
+                  if (args.out_bf16)
+                    static_cast<__nv_bfloat16*>(args.out)[el] = __float2bfloat16_rn(v[j]);
+                  else
+                    static_cast<float*>(args.out)[el] = v[j];
+                }
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->tmem_empty[acc]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (sh->abort_flag != 0) {
+    long long t0 = clock64();
+    while (clock64() - t0 < 4000000LL) {
+    }
+    if (threadIdx.x == 0 && args.status != nullptr) atomicExch(args.status, kGated ? 13 : 14);
+  }
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::kTmem);
+  }
+}
+
+int map_few(CUtensorMap* m, const void* base, uint64_t experts, uint64_t rows, uint64_t k, uint32_t box_rows) {
+  const uint64_t dims[3] = {k / 2, rows, experts};
+  const uint64_t strides[2] = {k / 2, k / 2 * rows};
+  const uint32_t box[3] = {128, box_rows, 1};
+  return encode_tensor_map_bytes(m, base, 3, dims, strides, box);
+}
+int map_few_scales(CUtensorMap* m, const void* base, uint64_t tiles, int k) {
+  const uint64_t dims[3] = {128, (uint64_t)mx4_chunks(k), tiles};
+  const uint64_t strides[2] = {512, 512ull * mx4_chunks(k)};
+  const uint32_t box[3] = {128, 2, 1};
+  return encode_tensor_map_words(m, base, 3, dims, strides, box);
+}
+
+template <bool kGated, int N>
+int launch_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, const void* const (&w)[4], int experts, int k,
+               int n, FewArgs ga, cudaStream_t st) {
+  using Cfg = FewCfg<kGated, N>;
+  constexpr size_t smem_bytes = 1024 + (size_t)Cfg::kStages * Cfg::kStageBytes + sizeof(FewShared<Cfg::kStages>);
+  static_assert(smem_bytes <= 227u * 1024u, "shared memory of the few-rows kernel");
+  static SmemLimitCache smem = {};
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(mx4_few_kernel<kGated, N>), smem_bytes, &smem, "mx4_few_kernel"))
+    return rc;
+  CUtensorMap a, a_sf, w0, w1, w0_sf, w1_sf;
+  int rc;
+  const int wn = (n + 127) / 128;
+  if ((rc = map_few(&a, a_codes, 1, r.rows, k, N))) return rc;
+  if ((rc = map_few_scales(&a_sf, a_scales, mx4_row_tiles(r.rows, r.table_segments), k))) return rc;
+  if ((rc = map_few(&w0, w[0], experts, n, k, 128))) return rc;
+  if ((rc = map_few_scales(&w0_sf, w[1], (uint64_t)experts * wn, k))) return rc;
+  if constexpr (kGated) {
+    if ((rc = map_few(&w1, w[2], experts, n, k, 128))) return rc;
+    if ((rc = map_few_scales(&w1_sf, w[3], (uint64_t)experts * wn, k))) return rc;
+  } else {
+    w1 = w0;
+    w1_sf = w0_sf;
+  }
+  ga.segments = r.segments;
+  ga.num_segments = r.segments != nullptr ? r.num_segments : 1;
+  ga.rows_total = r.rows;
+  ga.seg_base = r.seg_base;
+  ga.expert_base = r.expert_base;
+  ga.status = r.status;
+  ga.n_total = n;
+  ga.k_total = k;
+  ga.wn_tiles = wn;
+  ga.partial = r.few_partial;
+  ga.counters = r.few_counters;
+  // Starts while the kernel before it drains.  That kernel has waited for everything before itself,
+  // so what is older (weights, segment table) may be read without waiting.
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)sm_count(), 1, 1);
+  cfg.blockDim = dim3(kThreadsF, 1, 1);
+  cfg.dynamicSmemBytes = smem_bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, mx4_few_kernel<kGated, N>, a, a_sf, w0, w1, w0_sf, w1_sf, ga), "mx4_few_kernel");
+}
+
+template <bool kGated>
+int launch_few_n(const Mx4Rows& r, const void* a_codes, const void* a_scales, const void* const (&w)[4], int experts,
+                 int k, int n, const FewArgs& ga, cudaStream_t st) {
+  if (r.max_rows <= 16) return launch_few<kGated, 16>(r, a_codes, a_scales, w, experts, k, n, ga, st);
+  if (r.max_rows <= 32) return launch_few<kGated, 32>(r, a_codes, a_scales, w, experts, k, n, ga, st);
+  if (r.max_rows <= 64) return launch_few<kGated, 64>(r, a_codes, a_scales, w, experts, k, n, ga, st);
+  return launch_few<kGated, 128>(r, a_codes, a_scales, w, experts, k, n, ga, st);
+}
+
+}  // namespace
+
+bool mx4_use_few(int max_rows) {
+  static const int most = getenv("AXM_MX4_FEW") ? atoi(getenv("AXM_MX4_FEW")) : 128;
+  return max_rows <= most;
+}
+
+int mx4_few_counters() { return kEnough; }
+
+size_t mx4_few_partial_bytes(int max_rows, bool gated) {
+  const int n = max_rows <= 16 ? 16 : max_rows <= 32 ? 32 : max_rows <= 64 ? 64 : 128;
+  return (size_t)kUnitsMost * (gated ? 2 : 1) * n * 128 * sizeof(float);
+}
+
+int launch_mx4_linear_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, const void* w_codes,
+                          const void* w_scales, int experts, int k, int n, void* out, bool out_bf16, cudaStream_t st) {
+  FewArgs ga = {};
+  ga.out = out;
+  ga.out_bf16 = out_bf16 ? 1 : 0;
+  const void* const w[4] = {w_codes, w_scales, nullptr, nullptr};
+  return launch_few_n<false>(r, a_codes, a_scales, w, experts, k, n, ga, st);
+}
+
+int launch_mx4_gated_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, const AxmMx4Experts* x, int experts,
+                         int d, int f, void* h_codes, void* h_scales, cudaStream_t st) {
+  FewArgs ga = {};
+  ga.out = h_codes;
+  ga.out_scales = static_cast<uint8_t*>(h_scales);
+  const void* const w[4] = {x->gate_codes, x->gate_scales, x->up_codes, x->up_scales};
+  return launch_few_n<true>(r, a_codes, a_scales, w, experts, d, f, ga, st);
+}
+
+}  // namespace axm

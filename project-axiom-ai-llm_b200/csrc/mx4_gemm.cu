@@ -295,7 +295,13 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     }
   } else if (warp == 1) {
     // ---- MMA issuer: the leader CTA only -----------------------------------------------------
-    if (lane == 0 && rank == 0) {
+    // The whole warp runs the loop, one elected lane issues (see elect_one): with one lane running it,
+    // issuing a stage's ten tcgen05 instructions took about 900 cycles, the MMAs themselves 520.
+    if (rank == 0) {
+      const uint32_t free0 = map_to_cta(smem_u32(&sh->empty[0]), 0), free1 = map_to_cta(smem_u32(&sh->empty[0]), 1);
+      const uint32_t done0 = map_to_cta(smem_u32(&sh->tmem_full[0]), 0), done1 = map_to_cta(smem_u32(&sh->tmem_full[0]), 1);
+      const uint64_t codes0 = make_smem_desc(smem_u32(tiles), 16, 1024);
+      const uint64_t scales0 = scale_desc(smem_u32(scales_s));
       int stage = 0;
       uint32_t phase = 0;
       int tile = 0;
@@ -303,43 +309,49 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
       for (int unit = cluster_id; ok && unit < total_units; unit += num_clusters, ++tile) {
         // the previous tile's epilogue has taken the columns both accumulators share (and, as it
         // works tile by tile, has finished the tile before)
-        if (!mbar_wait(&sh->overlap_free, (uint32_t)(tile & 1) ^ 1u, abort_flag)) {
-          raise_abort();
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh->overlap_free, (uint32_t)(tile & 1) ^ 1u, abort_flag))) {
+          if (lane == 0) raise_abort();
           break;
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + ((tile & 1) ? kAcc1 : 0u);
         for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait(&sh->full[stage], phase, abort_flag)) {
-            raise_abort();
+          if (!__all_sync(0xffffffffu, mbar_wait(&sh->full[stage], phase, abort_flag))) {
+            if (lane == 0) raise_abort();
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(tiles + (size_t)stage * 2 * kCodeBytes);
-          const uint32_t ssf = smem_u32(scales_s + (size_t)stage * (kScaleABytes + kScaleBBytes));
-          const uint64_t da = make_smem_desc(sa, 16, 1024);
-          const uint64_t db = make_smem_desc(sa + kCodeBytes, 16, 1024);
+          // descriptors count in 16-byte units
+          const uint64_t da = codes0 + (uint64_t)(stage * (2 * kCodeBytes / 16));
+          const uint64_t db = da + kCodeBytes / 16;
+          const uint64_t sf = scales0 + (uint64_t)(stage * ((kScaleABytes + kScaleBBytes) / 16));
+          if (elect_one()) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            tc_cp2_scales(tmem_base + kSfA + 4 * c, scale_desc(ssf + 512 * c));
-            tc_cp2_scales(tmem_base + kSfB + 8 * c, scale_desc(ssf + kScaleABytes + 512 * c));
-            tc_cp2_scales(tmem_base + kSfB + 8 * c + 4, scale_desc(ssf + kScaleABytes + 1024 + 512 * c));
+            for (int c = 0; c < 2; ++c) {
+              tc_cp2_scales(tmem_base + kSfA + 4 * c, sf + 32 * c);
+              tc_cp2_scales(tmem_base + kSfB + 8 * c, sf + kScaleABytes / 16 + 32 * c);
+              tc_cp2_scales(tmem_base + kSfB + 8 * c + 4, sf + (kScaleABytes + 1024) / 16 + 32 * c);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)  // 64 elements = 32 bytes a step
+              tc_mma2_mx4(d_tmem, da + (uint64_t)(j * 2), db + (uint64_t)(j * 2), mx4_instr_desc(j & 1),
+                          tmem_base + kSfA + 4 * (j >> 1), tmem_base + kSfB + 8 * (j >> 1), (kb > 0 || j > 0) ? 1u : 0u);
+            tc_commit2(free0 + 8 * stage);
+            tc_commit2(free1 + 8 * stage);
           }
-#pragma unroll
-          for (int j = 0; j < 4; ++j)  // 64 elements = 32 bytes a step
-            tc_mma2_mx4(d_tmem, da + (uint64_t)(j * 2), db + (uint64_t)(j * 2), mx4_instr_desc(j & 1),
-                        tmem_base + kSfA + 4 * (j >> 1), tmem_base + kSfB + 8 * (j >> 1), (kb > 0 || j > 0) ? 1u : 0u);
-          tc_commit2(map_to_cta(smem_u32(&sh->empty[stage]), 0));
-          tc_commit2(map_to_cta(smem_u32(&sh->empty[stage]), 1));
+          __syncwarp();
           if (++stage == kStages4) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (!ok) break;
-        tc_commit2(map_to_cta(smem_u32(&sh->tmem_full[tile & 1]), 0));
-        tc_commit2(map_to_cta(smem_u32(&sh->tmem_full[tile & 1]), 1));
+        if (elect_one()) {
+          tc_commit2(done0 + 8 * (tile & 1));
+          tc_commit2(done1 + 8 * (tile & 1));
+        }
+        __syncwarp();
       }
     }
   } else {

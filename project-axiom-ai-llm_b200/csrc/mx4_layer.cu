@@ -48,9 +48,23 @@ int check_ffn_desc(const AxmMoeDesc* d, const char* what) {
   return AXM_OK;
 }
 
+// Workspace of the few-rows kernels.  Also where the pair kernels run: a workspace made for many
+// rows serves calls with few.
+struct FewWs {
+  uint32_t* counters;
+  float* partial;
+};
+FewWs carve_few(Carver& c, int max_rows, bool gated) {
+  FewWs w;
+  w.counters = static_cast<uint32_t*>(c.take(sizeof(uint32_t) * mx4_few_counters()));
+  w.partial = static_cast<float*>(c.take(mx4_few_partial_bytes(max_rows, gated)));
+  return w;
+}
+
 struct LinearWs {
   int32_t* status;
   void *codes, *scales;
+  FewWs few;
   size_t bytes;
 };
 LinearWs carve_linear(int tokens, int k, void* base) {
@@ -59,6 +73,7 @@ LinearWs carve_linear(int tokens, int k, void* base) {
   w.status = static_cast<int32_t*>(c.take(4));
   w.codes = c.take((size_t)tokens * (k / 2));
   w.scales = c.take((size_t)mx4_row_tiles(tokens, 1) * mx4_chunks(k) * 512);
+  w.few = carve_few(c, tokens, false);
   w.bytes = c.off;
   return w;
 }
@@ -66,9 +81,11 @@ LinearWs carve_linear(int tokens, int k, void* base) {
 struct FfnWs {
   int32_t* status;
   void *x_codes, *x_scales, *h_codes, *h_scales;
+  FewWs few;
   size_t bytes;
 };
-void carve_ffn(Carver& c, int rows, int num_segments, int d, int f, FfnWs* w) {
+void carve_ffn(Carver& c, int rows, int num_segments, int tokens, int d, int f, FfnWs* w) {
+  w->few = carve_few(c, tokens, true);
   w->x_codes = c.take((size_t)rows * (d / 2));
   w->x_scales = c.take((size_t)mx4_row_tiles(rows, num_segments) * mx4_chunks(d) * 512);
   w->h_codes = c.take((size_t)rows * (f / 2));
@@ -78,7 +95,7 @@ FfnWs carve_expert_ffn(const AxmMoeDesc* d, int rows, int num_segments, void* ba
   Carver c{static_cast<char*>(base)};
   FfnWs w;
   w.status = static_cast<int32_t*>(c.take(4));
-  carve_ffn(c, rows, num_segments, d->d_model, d->d_ff, &w);
+  carve_ffn(c, rows, num_segments, d->tokens, d->d_model, d->d_ff, &w);
   w.bytes = c.off;
   return w;
 }
@@ -86,6 +103,11 @@ FfnWs carve_expert_ffn(const AxmMoeDesc* d, int rows, int num_segments, void* ba
 // Both products of the feed-forward over one range of the table.
 int launch_ffn(const Mx4Rows& r, const FfnWs& w, const AxmMx4Experts* experts, int num_experts, int d, int f, void* o,
                bool o_bf16, cudaStream_t st) {
+  if (mx4_use_few(r.max_rows)) {
+    if (int rc = launch_mx4_gated_few(r, w.x_codes, w.x_scales, experts, num_experts, d, f, w.h_codes, w.h_scales, st)) return rc;
+    return launch_mx4_linear_few(r, w.h_codes, w.h_scales, experts->down_codes, experts->down_scales, num_experts, f, d, o,
+                                 o_bf16, st);
+  }
   if (int rc = launch_mx4_gated(r, w.x_codes, w.x_scales, experts, num_experts, d, f, w.h_codes, w.h_scales, st)) return rc;
   return launch_mx4_linear(r, w.h_codes, w.h_scales, experts->down_codes, experts->down_scales, num_experts, f, d, o,
                            o_bf16, st);
@@ -120,7 +142,7 @@ LayerWs carve_layer(const AxmMoeDesc* d, void* base) {
   w.row_src = static_cast<int32_t*>(c.take(4 * T * k));
   w.slot_dst = static_cast<int32_t*>(c.take(4 * T * k));
   w.segments = static_cast<AxmSegment*>(c.take(sizeof(AxmSegment) * (E + S)));
-  carve_ffn(c, (int)rows, (int)(E + S), d->d_model, d->d_ff, &w.ffn);
+  carve_ffn(c, (int)rows, (int)(E + S), d->tokens, d->d_model, d->d_ff, &w.ffn);
   w.o = c.take(4 * rows * d->d_model);
   w.router_scratch_bytes = 0;
   axm_moe_router_scratch_bytes(d, &w.router_scratch_bytes);
@@ -166,11 +188,12 @@ extern "C" int axm_mx4_linear(const void* x, int32_t x_dtype, int64_t ld, int32_
   if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
   if (int rc = require_device()) return rc;
   const LinearWs w = carve_linear(tokens, k, workspace);
-  const Mx4Rows rows = {nullptr, 0, tokens, 1, 0, 0, tokens, w.status};
+  const Mx4Rows rows = {nullptr, 0, tokens, 1, 0, 0, tokens, w.status, w.few.partial, w.few.counters};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Mx4Gather from = {nullptr, 1, tokens, 1};
   if (int rc = launch_mx4_quantize_rows(x, x_dtype, ld, from, rows, k, w.codes, w.scales, st)) return rc;
-  return launch_mx4_linear(rows, w.codes, w.scales, w_codes, w_scales, 1, k, n, out, out_dtype == AXM_DTYPE_BF16, st);
+  return (mx4_use_few(tokens) ? launch_mx4_linear_few : launch_mx4_linear)(rows, w.codes, w.scales, w_codes, w_scales, 1, k,
+                                                                           n, out, out_dtype == AXM_DTYPE_BF16, st);
 }
 
 extern "C" int axm_mx4_expert_ffn_workspace_bytes(const AxmMoeDesc* desc, int32_t rows, int32_t num_segments,
@@ -201,7 +224,7 @@ extern "C" int axm_mx4_expert_ffn(const AxmMoeDesc* desc, const void* x, int32_t
   if (int rc = require_device()) return rc;
   const int D = desc->d_model, F = desc->d_ff;
   const FfnWs w = carve_expert_ffn(desc, rows, num_segments, workspace);
-  const Mx4Rows r = {segments, num_segments, rows, num_segments, 0, 0, desc->tokens, w.status};
+  const Mx4Rows r = {segments, num_segments, rows, num_segments, 0, 0, desc->tokens, w.status, w.few.partial, w.few.counters};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Mx4Gather from = {nullptr, 1, rows, 1};
   if (int rc = launch_mx4_quantize_rows(x, AXM_DTYPE_BF16, D, from, r, D, w.x_codes, w.x_scales, st)) return rc;
@@ -248,7 +271,7 @@ extern "C" int axm_moe_forward_mx4(const AxmMoeDesc* desc, const AxmMoeTensors* 
                            w.segments, cleared ? nullptr : w.ffn.status, st, 1)))
     return rc;
   const int rows = T * (k + S);
-  Mx4Rows r = {w.segments, E + S, rows, E + S, 0, 0, T, nullptr};
+  Mx4Rows r = {w.segments, E + S, rows, E + S, 0, 0, T, nullptr, w.ffn.few.partial, w.ffn.few.counters};
   const Mx4Gather from = {row_src, k, T * k, T};
   if ((rc = launch_mx4_quantize_rows(t->x, AXM_DTYPE_BF16, D, from, r, D, w.ffn.x_codes, w.ffn.x_scales, st))) return rc;
   r.status = w.ffn.status;
