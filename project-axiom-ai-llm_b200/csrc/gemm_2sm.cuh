@@ -86,6 +86,16 @@ __device__ __forceinline__ void tc_commit2(uint32_t bar_cluster_addr) {
                    bar_cluster_addr)
                : "memory");
 }
+// The same for both CTAs of the pair with one instruction: the barrier at this offset in either.
+__device__ __forceinline__ void tc_commit2_both(uint32_t bar_addr) {
+  asm volatile(
+      "{\n\t"
+      ".reg .b16 m;\n\t"
+      "mov.b16 m, 3;\n\t"
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t"
+      "}" ::"r"(bar_addr)
+      : "memory");
+}
 __device__ __forceinline__ void tc_mma2_bf16(uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b,
                                              uint32_t idesc, uint32_t accumulate) {
   asm volatile(

@@ -298,8 +298,6 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     // The whole warp runs the loop, one elected lane issues (see elect_one): with one lane running it,
     // issuing a stage's ten tcgen05 instructions took about 900 cycles, the MMAs themselves 520.
     if (rank == 0) {
-      const uint32_t free0 = map_to_cta(smem_u32(&sh->empty[0]), 0), free1 = map_to_cta(smem_u32(&sh->empty[0]), 1);
-      const uint32_t done0 = map_to_cta(smem_u32(&sh->tmem_full[0]), 0), done1 = map_to_cta(smem_u32(&sh->tmem_full[0]), 1);
       const uint64_t codes0 = make_smem_desc(smem_u32(tiles), 16, 1024);
       const uint64_t scales0 = scale_desc(smem_u32(scales_s));
       int stage = 0;
@@ -337,8 +335,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             for (int j = 0; j < 4; ++j)  // 64 elements = 32 bytes a step
               tc_mma2_mx4(d_tmem, da + (uint64_t)(j * 2), db + (uint64_t)(j * 2), mx4_instr_desc(j & 1),
                           tmem_base + kSfA + 4 * (j >> 1), tmem_base + kSfB + 8 * (j >> 1), (kb > 0 || j > 0) ? 1u : 0u);
-            tc_commit2(free0 + 8 * stage);
-            tc_commit2(free1 + 8 * stage);
+            tc_commit2_both(smem_u32(&sh->empty[stage]));
           }
           __syncwarp();
           if (++stage == kStages4) {
@@ -348,8 +345,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         }
         if (!ok) break;
         if (elect_one()) {
-          tc_commit2(done0 + 8 * (tile & 1));
-          tc_commit2(done1 + 8 * (tile & 1));
+          tc_commit2_both(smem_u32(&sh->tmem_full[tile & 1]));
         }
         __syncwarp();
       }
