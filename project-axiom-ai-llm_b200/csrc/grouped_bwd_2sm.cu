@@ -157,8 +157,9 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
       }
     }
   } else if (warp == 1) {
-    // ---- MMA issuer: the leader CTA only ---------------------------------------------
-    if (lane == 0 && rank == 0) {
+    // ---- MMA issuer: the leader CTA only (the whole warp, one elected lane issues) ------
+    if (rank == 0) {
+      const uint64_t tiles_desc = make_smem_desc(smem_u32(tiles), kBChunkBytes, 1024);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -167,30 +168,31 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
       for (int unit = cluster_id; ok && unit < total_units; unit += num_clusters) {
         const WgradUnit u = decode_wgrad(unit, pairs_w, n_tiles, m_tiles, 0);
         const int k_blocks = (sh->seg[u.seg].rows + BK - 1) / BK;
-        if (!mbar_wait(&sh->tmem_empty[acc], acc_phase ^ 1u, abort_flag)) {
-          raise_abort();
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh->tmem_empty[acc], acc_phase ^ 1u, abort_flag))) {
+          if (lane == 0) raise_abort();
           break;
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)acc * UMMA_N;
         for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait(&sh->full[stage], phase, abort_flag)) {
-            raise_abort();
+          if (!__all_sync(0xffffffffu, mbar_wait(&sh->full[stage], phase, abort_flag))) {
+            if (lane == 0) raise_abort();
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(tiles + (size_t)stage * kStageBytes2);
-          const uint32_t sb = sa + kABytes;
-          // MN-major operands: 64-wide chunks 8192 B apart, 8-k groups 1024 B apart, +2048 B per 16 k
-          const uint64_t da = make_smem_desc(sa, kBChunkBytes, 1024);
-          const uint64_t db = make_smem_desc(sb, kBChunkBytes, 1024);
+          // MN-major operands: 64-wide chunks 8192 B apart, 8-k groups 1024 B apart, +2048 B per 16 k;
+          // descriptors count in 16-byte units
+          const uint64_t da = tiles_desc + (uint64_t)(stage * (kStageBytes2 / 16));
+          const uint64_t db = da + kABytes / 16;
+          if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < BK / UMMA_K; ++j)
-            tc_mma2_bf16(d_tmem, da + (uint64_t)(j * 128), db + (uint64_t)(j * 128), kInstrDescWgrad2,
-                         (kb > 0 || j > 0) ? 1u : 0u);
-          tc_commit2(map_to_cta(smem_u32(&sh->empty[stage]), 0));
-          tc_commit2(map_to_cta(smem_u32(&sh->empty[stage]), 1));
+            for (int j = 0; j < BK / UMMA_K; ++j)
+              tc_mma2_bf16(d_tmem, da + (uint64_t)(j * 128), db + (uint64_t)(j * 128), kInstrDescWgrad2,
+                           (kb > 0 || j > 0) ? 1u : 0u);
+            tc_commit2_both(smem_u32(&sh->empty[stage]));
+          }
+          __syncwarp();
           if (++stage == kStages2) {
             stage = 0;
             phase ^= 1u;
@@ -198,8 +200,8 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
         }
         if (!ok) break;
         // with no rows nothing was issued and the commits arrive at once; the epilogue writes zeros
-        tc_commit2(map_to_cta(smem_u32(&sh->tmem_full[acc]), 0));
-        tc_commit2(map_to_cta(smem_u32(&sh->tmem_full[acc]), 1));
+        if (elect_one()) tc_commit2_both(smem_u32(&sh->tmem_full[acc]));
+        __syncwarp();
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1u;
       }

@@ -311,16 +311,18 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
       }
     }
   } else if (warp == 1) {
-    // ---- MMA issuer: the leader CTA only ---------------------------------------------
-    if (lane == 0 && rank == 0) {
+    // ---- MMA issuer: the leader CTA only (the whole warp, one elected lane issues) ------
+    if (rank == 0) {
+      const uint64_t tiles_desc = make_smem_desc(smem_u32(tiles), 16, 1024);
+      const uint64_t tiles_desc_b = kBKmajor ? tiles_desc : make_smem_desc(smem_u32(tiles), kBChunkBytes, 1024);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
       bool ok = true;
       for (int unit = cluster_id; ok && unit < total_units; unit += num_clusters) {
-        if (!mbar_wait(&sh->tmem_empty[acc], acc_phase ^ 1u, abort_flag)) {
-          raise_abort();
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh->tmem_empty[acc], acc_phase ^ 1u, abort_flag))) {
+          if (lane == 0) raise_abort();
           break;
         }
         tc_fence_after();
@@ -333,32 +335,33 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
           kb1 = kb0 + kb_per < k_blocks ? kb0 + kb_per : k_blocks;
         }
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(&sh->full[stage], phase, abort_flag)) {
-            raise_abort();
+          if (!__all_sync(0xffffffffu, mbar_wait(&sh->full[stage], phase, abort_flag))) {
+            if (lane == 0) raise_abort();
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(tiles + (size_t)stage * kStageBytes2);
-          const uint32_t sb = sa + kABytes;
-          const uint64_t da = make_smem_desc(sa, 16, 1024);
+          // descriptors count in 16-byte units
+          const uint64_t da = tiles_desc + (uint64_t)(stage * (kStageBytes2 / 16));
           // MN-major B: 64-wide chunks 8192 B apart, +2048 B per 16 k; K-major B (kModeDX): like A
-          const uint64_t db = kBKmajor ? make_smem_desc(sb, 16, 1024) : make_smem_desc(sb, kBChunkBytes, 1024);
+          const uint64_t db = tiles_desc_b + (uint64_t)(stage * (kStageBytes2 / 16) + kABytes / 16);
+          if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < BK / UMMA_K; ++j)
-            tc_mma2_bf16(d_tmem, da + (uint64_t)(j * 2), db + (uint64_t)(j * (kBKmajor ? 2 : 128)),
-                         kBKmajor ? kInstrDesc2KB : kInstrDesc2, (kb > kb0 || j > 0) ? 1u : 0u);
-          // free this stage in both CTAs once the MMAs that read it are done
-          tc_commit2(map_to_cta(smem_u32(&sh->empty[stage]), 0));
-          tc_commit2(map_to_cta(smem_u32(&sh->empty[stage]), 1));
+            for (int j = 0; j < BK / UMMA_K; ++j)
+              tc_mma2_bf16(d_tmem, da + (uint64_t)(j * 2), db + (uint64_t)(j * (kBKmajor ? 2 : 128)),
+                           kBKmajor ? kInstrDesc2KB : kInstrDesc2, (kb > kb0 || j > 0) ? 1u : 0u);
+            // free this stage in both CTAs once the MMAs that read it are done
+            tc_commit2_both(smem_u32(&sh->empty[stage]));
+          }
+          __syncwarp();
           if (++stage == kSt) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (!ok) break;
-        tc_commit2(map_to_cta(smem_u32(&sh->tmem_full[acc]), 0));
-        tc_commit2(map_to_cta(smem_u32(&sh->tmem_full[acc]), 1));
+        if (elect_one()) tc_commit2_both(smem_u32(&sh->tmem_full[acc]));
+        __syncwarp();
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1u;
       }
