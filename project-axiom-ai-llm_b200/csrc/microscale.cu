@@ -61,7 +61,7 @@ struct MxClear {
 template <int kBits, typename T, bool kWide>
 __global__ void __launch_bounds__(256)
 mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, int rows, int k, int log_wpr,
-                        const AxmSegment* __restrict__ segments, int num_segments,
+                        const AxmSegment* __restrict__ segments, int num_segments, int tile_rows,
                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, MxClear clear) {
   // a product that is launched to start early may prepare itself now; it waits before it reads
   asm volatile("griddepcontrol.launch_dependents;");
@@ -96,7 +96,9 @@ mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, i
         if (placed) first = __ldg(&segments[seg].out_row0);
       }
       const int r = row - first;
-      sc += ((size_t)(first / 128 + (placed ? seg : 0) + r / 128) * mx4_chunks(k)) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4;
+      const int in_tile = r & (tile_rows - 1);
+      sc += ((size_t)(first / tile_rows + (placed ? seg : 0) + r / tile_rows) * mx4_chunks(k)) * 512 + (in_tile & 31) * 16 +
+            (in_tile >> 5) * 4;
     } else {
       sc += (size_t)row * (k >> 5);
     }
@@ -457,22 +459,22 @@ bool rows_at_32(const void* p, int64_t ld, int32_t dtype) {
 
 template <int kBits, typename T>
 int launch_quantize_rows_of(const void* x, bool wide, int64_t ld, const Mx4Gather& from, int32_t rows, int32_t k,
-                            const AxmSegment* segments, int32_t num_segments, void* codes, void* scales,
+                            const AxmSegment* segments, int32_t num_segments, int tile_rows, void* codes, void* scales,
                             const MxClear& clear, cudaStream_t st) {
   const RowLaunch l = row_launch(rows, k);
   auto* kernel = wide ? mx_quantize_rows_kernel<kBits, T, true> : mx_quantize_rows_kernel<kBits, T, false>;
-  kernel<<<l.grid, 256, 0, st>>>(static_cast<const T*>(x), ld, from, rows, k, l.log_wpr, segments, num_segments,
+  kernel<<<l.grid, 256, 0, st>>>(static_cast<const T*>(x), ld, from, rows, k, l.log_wpr, segments, num_segments, tile_rows,
                                  static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), clear);
   return check_launch("mx_quantize_rows_kernel");
 }
 template <int kBits>
 int launch_quantize_rows(const void* x, int32_t dtype, int64_t ld, const Mx4Gather& from, int32_t rows, int32_t k,
-                         const AxmSegment* segments, int32_t num_segments, void* codes, void* scales,
+                         const AxmSegment* segments, int32_t num_segments, int tile_rows, void* codes, void* scales,
                          const MxClear& clear, cudaStream_t st) {
   const bool wide = rows_at_32(x, ld, dtype);
   return dtype == AXM_DTYPE_BF16
-             ? launch_quantize_rows_of<kBits, __nv_bfloat16>(x, wide, ld, from, rows, k, segments, num_segments, codes, scales, clear, st)
-             : launch_quantize_rows_of<kBits, float>(x, wide, ld, from, rows, k, segments, num_segments, codes, scales, clear, st);
+             ? launch_quantize_rows_of<kBits, __nv_bfloat16>(x, wide, ld, from, rows, k, segments, num_segments, tile_rows, codes, scales, clear, st)
+             : launch_quantize_rows_of<kBits, float>(x, wide, ld, from, rows, k, segments, num_segments, tile_rows, codes, scales, clear, st);
 }
 
 template <int kBits, typename T>
@@ -497,7 +499,7 @@ int launch_dequantize_rows(const void* codes, const void* scales, int32_t rows, 
 
 int launch_mx4_quantize_rows(const void* x, int32_t dtype, int64_t ld, const Mx4Gather& from, const Mx4Rows& rows, int k,
                              void* codes, void* scales, cudaStream_t st) {
-  return launch_quantize_rows<4>(x, dtype, ld, from, rows.rows, k, rows.segments, rows.num_segments, codes, scales,
+  return launch_quantize_rows<4>(x, dtype, ld, from, rows.rows, k, rows.segments, rows.num_segments, rows.tile_rows, codes, scales,
                                  MxClear{rows.status, rows.few_counters, rows.few_counters ? mx4_few_counters() : 0}, st);
 }
 
@@ -540,7 +542,7 @@ extern "C" int axm_mx4_quantize_rows(const void* x, int32_t x_dtype, int64_t ld,
   if (misaligned(codes, 16) || misaligned(scales, 16)) return fail(AXM_ERR_ARGUMENT, "%s: codes and scales must be 16-byte aligned", what);
   if (int rc = require_device()) return rc;
   const Mx4Gather from = {row_src, row_div, rows, 1};
-  return launch_quantize_rows<4>(x, x_dtype, ld, from, rows, k, segments, num_segments, codes, scales,
+  return launch_quantize_rows<4>(x, x_dtype, ld, from, rows, k, segments, num_segments, 128, codes, scales,
                                  MxClear{}, static_cast<cudaStream_t>(stream));
 }
 
@@ -571,7 +573,7 @@ extern "C" int axm_mx8_quantize_rows(const void* x, int32_t x_dtype, int64_t ld,
   if (misaligned(codes, 16)) return fail(AXM_ERR_ARGUMENT, "%s: codes must be 16-byte aligned", what);
   if (int rc = require_device()) return rc;
   const Mx4Gather from = {nullptr, 1, rows, 1};
-  return launch_quantize_rows<8>(x, x_dtype, ld, from, rows, k, nullptr, 0, codes, scales, MxClear{},
+  return launch_quantize_rows<8>(x, x_dtype, ld, from, rows, k, nullptr, 0, 128, codes, scales, MxClear{},
                                  static_cast<cudaStream_t>(stream));
 }
 

@@ -14,7 +14,8 @@
 // chunks follow one another, ceil(K / 256) * 2 of them (a pipeline stage is 256 elements); the
 // bytes of blocks beyond K are 0, those of rows that do not exist are never written.
 // Tiles of activations start at each segment's first row: rows of segment s are in the tiles from
-// out_row0 / 128 + s on (never two segments in one tile, whatever their lengths).
+// out_row0 / 128 + s on (never two segments in one tile, whatever their lengths).  Inside a call that
+// runs on the few-rows kernels they have 16, 32 or 64 rows instead, in the same places of 512 bytes.
 #pragma once
 
 #include "common.cuh"
@@ -24,8 +25,12 @@ namespace axm {
 constexpr int kMxBlock = 32;
 
 __host__ __device__ constexpr int mx4_chunks(int k) { return (k + 255) / 256 * 2; }
-__host__ __device__ constexpr long long mx4_row_tiles(long long rows, int num_segments) {
-  return rows / 128 + num_segments;
+__host__ __device__ constexpr long long mx4_row_tiles(long long rows, int num_segments, int tile_rows = 128) {
+  return rows / tile_rows + num_segments;
+}
+// Room for any tile_rows that mx4_tile_rows chooses, in a workspace made for `rows` or more.
+__host__ __device__ constexpr long long mx4_row_tiles_most(long long rows, int num_segments) {
+  return rows / 128 + 2LL * num_segments;
 }
 
 // The rows of a grouped 4-bit product: a segment table in device memory (its rows are out_row0 ..
@@ -37,7 +42,8 @@ struct Mx4Rows {
   int table_segments;  // segments of the whole table the scale tiles were laid out with
   int seg_base;        // index of segments[0] in that table
   int expert_base;     // expert id of the first weight matrix of this launch
-  int max_rows;        // most rows any segment can have (the number of tokens)
+  int tile_rows;       // rows of a scale tile (and of a row tile of the few-rows kernels: 16, 32, 64, 128)
+  bool few;            // few rows a segment: mx4_few.cu instead of mx4_gemm.cu
   int32_t* status;
   float* few_partial;      // workspace of the few-rows kernels: partial tiles,
   uint32_t* few_counters;  //   a counter a tile (zero before the first launch of a call)
@@ -60,9 +66,9 @@ int launch_mx4_gated(const Mx4Rows& r, const void* a_codes, const void* a_scales
                      int d, int f, void* h_codes, void* h_scales, cudaStream_t st);
 
 // The same for few rows a segment (mx4_few.cu), with its workspace.
-bool mx4_use_few(int max_rows);
+int mx4_tile_rows(int rows, int num_segments, int max_rows);  // of the few-rows kernels; 0: the pair kernels
 int mx4_few_counters();
-size_t mx4_few_partial_bytes(int max_rows, bool gated);
+size_t mx4_few_partial_bytes(bool gated);
 int launch_mx4_linear_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, const void* w_codes,
                           const void* w_scales, int experts, int k, int n, void* out, bool out_bf16, cudaStream_t st);
 int launch_mx4_gated_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, const AxmMx4Experts* w, int experts,

@@ -2,13 +2,14 @@
 // counts is how fast the weights stream in, so the roles are turned around.
 //
 // 128 weight rows are the M side of the MMA (cta_group::1), the segment's rows its N side (16, 32, 64 or
-// 128 of them, a template parameter; with 128 a segment may have several such tiles).  A stage is 256
+// 128 of them, a template parameter; a segment may have several such tiles).  The scale tiles of the
+// activations are laid out with as many rows, so that each tile's bytes begin in the first column.  A stage is 256
 // reduction elements: 16 KiB of codes and 1 KiB of scale bytes for the weights (twice that for gate
 // and up), 128 bytes of codes a row for the activations.
 //
 // A unit is a weight tile (128 features) with a row tile, dealt out round robin.  An SM can pull
 // more than its share of the memory's bandwidth, so tiles that do not divide evenly among the SMs cost
-// nothing as long as the rest still are many; only where there are few (kEnough) is the reduction of
+// nothing as long as the rest still are many; only where there are few (few_enough) is the reduction of
 // each cut into equal ranges, units of their own.  A cut tile is finished by the unit that arrives last
 // (a counter, nobody waits): all of them leave their partial sums in the workspace, and the last
 // adds them in the order of the reduction, so the result does not depend on who was last.
@@ -18,7 +19,7 @@
 //
 // The accumulator has a feature a lane and a row a column.  Linear output is stored straight from
 // there (32 neighbouring features of a row).  The gated product's values are turned over through
-// shared memory, sixteen rows at a time, so that a lane holds a row's 32-block and quantises it
+// shared memory, 32 rows at a time, so that a lane holds a row's 32-block and quantises it
 // in registers as the pair kernel does.
 //
 // The weights do not depend on the kernel before: the producer asks for its first stages' weights
@@ -42,7 +43,7 @@ struct FewCfg {
   static constexpr int kCodeBytes = kWeights * kWCodeBytes + N * 128;
   static constexpr int kScaleBytes = (kWeights + 1) * kScaleChunk2;
   static constexpr int kStageBytes = kCodeBytes + kScaleBytes;
-  static constexpr int kFit = (200 * 1024) / kStageBytes;
+  static constexpr int kFit = (198 * 1024) / kStageBytes;
   static constexpr int kStages = kFit < 10 ? kFit : 10;
   static constexpr int kAccCols = kWeights * N;
   static constexpr int kAccs = 2 * kAccCols + 48 <= 512 ? 2 : 1;
@@ -62,10 +63,9 @@ struct __align__(8) FewShared {
   uint32_t tmem_base;
   int abort_flag;
   int is_last;
-  int too_long;
   int prefix[kMaxSegments + 1];  // row tiles before segment s
   AxmSegment seg[kMaxSegments];
-  float turn[4][16 * 33];  // per epilogue warp: 16 rows x 32 features
+  float turn[4][32 * 33];  // per epilogue warp: 32 rows x 32 features
 };
 
 struct FewArgs {
@@ -80,8 +80,8 @@ struct FewArgs {
   int out_bf16;
   void* out;
   uint8_t* out_scales;
-  float* partial;      // [kUnitsMost] tiles
-  uint32_t* counters;  // [kEnough], zero between launches
+  float* partial;      // a partial tile a unit
+  uint32_t* counters;  // one a tile, zero between launches
   int* status;
 };
 
@@ -151,9 +151,9 @@ struct Units {
     return true;
   }
 };
-// Units below which the reduction is cut, and above which it is not cut further.
-constexpr int kEnough = 96;
-constexpr int kUnitsMost = 256;
+// Units below which the reduction is cut: fewer with wide row tiles, whose partial sums cost more.
+// A cut call has less than twice as many.
+constexpr int few_enough(int n) { return n <= 32 ? 96 : n == 64 ? 64 : 48; }
 
 template <bool kGated, int N>
 __global__ void __launch_bounds__(kThreadsF, 1)
@@ -192,7 +192,6 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       mbar_init(&sh->tmem_empty[i], 4);
     }
     sh->abort_flag = 0;
-    sh->too_long = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tma_prefetch_desc(&tm_w0);
     tma_prefetch_desc(&tm_w0_sf);
@@ -211,7 +210,6 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       const int s = s0 + lane;
       const int rows = s < nseg ? sh->seg[s].rows : 0;
       const int mine = rows > 0 ? (rows + N - 1) / N : 0;
-      if (N < 128 && mine > 1) sh->too_long = 1;
       int sum = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -231,9 +229,9 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
   volatile int* abort_flag = &sh->abort_flag;
   const long long tiles_n = (long long)sh->prefix[nseg] * f_tiles;
   int k_per = k_blocks;
-  if (tiles_n > 0 && tiles_n < kEnough) {
+  if (tiles_n > 0 && tiles_n < few_enough(N)) {
     // the last to arrive reads every range's partial tile: the larger they are, the fewer
-    const int want = min(min((int)(kEnough + tiles_n - 1) / (int)tiles_n, k_blocks), 256 / N);
+    const int want = min(min((int)(few_enough(N) + tiles_n - 1) / (int)tiles_n, k_blocks), 256 / N);
     k_per = (k_blocks + want - 1) / want;
   }
   const int splits = (k_blocks + k_per - 1) / k_per;  // none of the ranges is empty
@@ -278,7 +276,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         uint64_t* bar = &sh->full[stage];
         tma_load_3d(codes, &tm_a, bar, kb * 128, sg.out_row0 + t.row_tile * N, 0);
         tma_load_3d(sf, &tm_a_sf, bar, 0, kb * 2,
-                    sg.out_row0 / 128 + args.seg_base + t.seg + t.row_tile * N / 128);
+                    sg.out_row0 / N + args.seg_base + t.seg + t.row_tile);
       };
       Units p = mine, q = mine;  // q: the activations of the stages p has asked weights for
       long long tile;
@@ -386,9 +384,6 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     float* turn_s = sh->turn[warp - 2];
     const int feature = quad * 32 + lane;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // outputs and partial sums of earlier launches
-    // a scale tile's rows from the sixteenth (32nd, 64th) on cannot be addressed as a tile of their
-    // own: a table whose segments are longer than the call was told is reported
-    if (sh->too_long && threadIdx.x == 64 && args.status != nullptr) atomicExch(args.status, 15);
     Units p = mine;
     long long tile;
     int kb0, kb1;
@@ -405,7 +400,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       const bool whole = splits == 1;
       bool finish = true;
       if (!whole) {
-        // at most kUnitsMost units where tiles are cut
+        // less than 2 few_enough(N) units where tiles are cut
         float* mine_p = args.partial + (size_t)(tile * splits + kb0 / k_per) * Cfg::kPartial;
 #pragma unroll 1
         for (int n0 = 0; n0 < rows; n0 += 16) {
@@ -456,68 +451,75 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         };
         const int f0 = t.f_tile * 128 + quad * 32;  // this warp's 32 features
         const size_t row0 = (size_t)sg.out_row0 + t.row_tile * N;
+        if constexpr (kGated) {
+          const int chunks = mx4_chunks(args.n_total);
+          uint8_t* sf0 = args.out_scales + ((size_t)(sg.out_row0 / N + args.seg_base + t.seg + t.row_tile) * chunks + t.f_tile) * 512;
 #pragma unroll 1
-        for (int n0 = 0; n0 < rows; n0 += 16) {
-          if constexpr (kGated) {
-            float g[16], u[16];
-            fetch(0, n0, g);
-            fetch(1, n0, u);
+          for (int n0 = 0; n0 < rows; n0 += 32) {
+#pragma unroll 1
+            for (int half = 0; half < (N < 32 ? 1 : 2); ++half) {
+              const int m0 = n0 + 16 * half;
+              if (m0 >= rows) break;
+              float g[16], u[16];
+              fetch(0, m0, g);
+              fetch(1, m0, u);
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                turn_s[(16 * half + j) * 33 + lane] = __fdividef(g[j], 1.0f + __expf(-g[j])) * u[j];
+            }
             __syncwarp();
+            // lane j: row n0 + j, its 32 features a block (n_total is a multiple of 32); scale bytes of
+            // blocks behind F are 0, as are those of the chunk behind an odd number of them
+            if (n0 + lane < rows) {
+              const int r = n0 + lane;
+              uint8_t* sf = sf0 + (r & 31) * 16 + (r >> 5) * 4;
+              uint32_t byte = 0;
+              if (f0 < args.n_total) {
+                float h[32];
+                uint32_t top = 0;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) turn_s[j * 33 + lane] = __fdividef(g[j], 1.0f + __expf(-g[j])) * u[j];
-            __syncwarp();
-            // lane j: row n0 + j, its 32 features a block (n_total is a multiple of 32)
-            if (lane < 16 && n0 + lane < rows && f0 < args.n_total) {
-              float h[32];
-              uint32_t top = 0;
+                for (int j = 0; j < 32; ++j) {
+                  h[j] = turn_s[lane * 33 + j];
+                  top = max(top, __float_as_uint(h[j]) & 0x7fffffffu);
+                }
+                byte = mx_scale_byte<2>(top);
+                const float inv = mx_inverse_scale(byte);
+                uint32_t q[4];
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                h[j] = turn_s[lane * 33 + j];
-                top = max(top, __float_as_uint(h[j]) & 0x7fffffffu);
+                for (int b = 0; b < 4; ++b) {
+                  float x[8];
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) x[j] = h[8 * b + j] * inv;
+                  q[b] = mx4_pack8(x);
+                }
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(args.out) +
+                                          (row0 + n0 + lane) * (size_t)(args.n_total >> 1) + (f0 >> 1)) =
+                    make_uint4(q[0], q[1], q[2], q[3]);
               }
-              const uint32_t byte = mx_scale_byte<2>(top);
-              const float inv = mx_inverse_scale(byte);
-              uint32_t q[4];
-#pragma unroll
-              for (int b = 0; b < 4; ++b) {
-                float x[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = h[8 * b + j] * inv;
-                q[b] = mx4_pack8(x);
-              }
-              const size_t row = row0 + n0 + lane;
-              *reinterpret_cast<uint4*>(static_cast<uint8_t*>(args.out) + row * (size_t)(args.n_total >> 1) + (f0 >> 1)) =
-                  make_uint4(q[0], q[1], q[2], q[3]);
-              const int r = t.row_tile * N + n0 + lane;  // row of the segment
-              const int chunks = mx4_chunks(args.n_total);
-              uint8_t* sf = args.out_scales +
-                            ((size_t)(sg.out_row0 / 128 + args.seg_base + t.seg + r / 128) * chunks + t.f_tile) * 512 +
-                            (r & 31) * 16 + ((r & 127) >> 5) * 4;
               sf[quad] = (uint8_t)byte;
+              if (quad == 0 && t.f_tile == f_tiles - 1 && f_tiles < chunks) *reinterpret_cast<uint32_t*>(sf + 512) = 0u;
             }
-            // scale bytes of blocks behind F: the rest of the last chunk, and the chunk behind an odd number
-            if (lane < 16 && n0 + lane < rows && t.f_tile == f_tiles - 1) {
-              const int r = t.row_tile * N + n0 + lane;
-              const int chunks = mx4_chunks(args.n_total);
-              uint8_t* sf = args.out_scales +
-                            ((size_t)(sg.out_row0 / 128 + args.seg_base + t.seg + r / 128) * chunks + t.f_tile) * 512 +
-                            (r & 31) * 16 + ((r & 127) >> 5) * 4;
-              if (f0 >= args.n_total) sf[quad] = 0;
-              if (quad == 0 && f_tiles < chunks) *reinterpret_cast<uint32_t*>(sf + 512) = 0u;
-            }
-          } else {
+            __syncwarp();
+          }
+        } else {
+          const size_t step = args.n_total;
+          size_t el = row0 * step + f0 + lane;
+#pragma unroll 1
+          for (int n0 = 0; n0 < rows; n0 += 16, el += 16 * step) {
             float v[16];
             fetch(0, n0, v);
             if (f0 + lane < args.n_total) {
+              if (args.out_bf16) {
+                __nv_bfloat16* to = static_cast<__nv_bfloat16*>(args.out) + el;
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                if (n0 + j < rows) {
-                  const size_t el = (row0 + n0 + j) * (size_t)args.n_total + f0 + lane;
-                  if (args.out_bf16)
-                    static_cast<__nv_bfloat16*>(args.out)[el] = __float2bfloat16_rn(v[j]);
-                  else
-                    static_cast<float*>(args.out)[el] = v[j];
-                }
+                for (int j = 0; j < 16; ++j, to += step)
+                  if (n0 + j < rows) *to = __float2bfloat16_rn(v[j]);
+              } else {
+                float* to = static_cast<float*>(args.out) + el;
+#pragma unroll
+                for (int j = 0; j < 16; ++j, to += step)
+                  if (n0 + j < rows) *to = v[j];
+              }
             }
           }
         }
@@ -570,7 +572,7 @@ int launch_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, cons
   int rc;
   const int wn = (n + 127) / 128;
   if ((rc = map_few(&a, a_codes, 1, r.rows, k, N))) return rc;
-  if ((rc = map_few_scales(&a_sf, a_scales, mx4_row_tiles(r.rows, r.table_segments), k))) return rc;
+  if ((rc = map_few_scales(&a_sf, a_scales, mx4_row_tiles(r.rows, r.table_segments, N), k))) return rc;
   if ((rc = map_few(&w0, w[0], experts, n, k, 128))) return rc;
   if ((rc = map_few_scales(&w0_sf, w[1], (uint64_t)experts * wn, k))) return rc;
   if constexpr (kGated) {
@@ -609,24 +611,41 @@ int launch_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, cons
 template <bool kGated>
 int launch_few_n(const Mx4Rows& r, const void* a_codes, const void* a_scales, const void* const (&w)[4], int experts,
                  int k, int n, const FewArgs& ga, cudaStream_t st) {
-  if (r.max_rows <= 16) return launch_few<kGated, 16>(r, a_codes, a_scales, w, experts, k, n, ga, st);
-  if (r.max_rows <= 32) return launch_few<kGated, 32>(r, a_codes, a_scales, w, experts, k, n, ga, st);
-  if (r.max_rows <= 64) return launch_few<kGated, 64>(r, a_codes, a_scales, w, experts, k, n, ga, st);
-  return launch_few<kGated, 128>(r, a_codes, a_scales, w, experts, k, n, ga, st);
+  switch (r.tile_rows) {
+    case 16: return launch_few<kGated, 16>(r, a_codes, a_scales, w, experts, k, n, ga, st);
+    case 32: return launch_few<kGated, 32>(r, a_codes, a_scales, w, experts, k, n, ga, st);
+    case 64: return launch_few<kGated, 64>(r, a_codes, a_scales, w, experts, k, n, ga, st);
+    default: return launch_few<kGated, 128>(r, a_codes, a_scales, w, experts, k, n, ga, st);
+  }
 }
 
 }  // namespace
 
-bool mx4_use_few(int max_rows) {
-  static const int most = getenv("AXM_MX4_FEW") ? atoi(getenv("AXM_MX4_FEW")) : 128;
-  return max_rows <= most;
+// Below about 96 rows a segment on average the weights' way in decides, and the few-rows kernels
+// are ahead (64 experts 2048 x 1408, top 6: 515 tokens 85 us against 110, 1030 tokens 109 against 122; 8
+// experts 4096 x 14336, top 2: 256 tokens 163 against 183, 512 tokens 234 against 191).
+// Their row tiles are as wide as a segment has rows at most, or on average with room to spare: a wider
+// tile costs epilogue and tensor time, a narrower one reads the weights again (from L2) for
+// every further tile.
+int mx4_tile_rows(int rows, int num_segments, int max_rows) {
+  static const int most = getenv("AXM_MX4_FEW") ? atoi(getenv("AXM_MX4_FEW")) : 96;
+  if (rows > (long long)most * num_segments) return 0;
+  const int average = (rows + num_segments - 1) / num_segments;
+  for (int n = 16; n <= 64; n *= 2)
+    if ((max_rows <= n || average <= n * 3 / 4) && rows / n + num_segments <= mx4_row_tiles_most(rows, num_segments)) return n;
+  return 128;
 }
 
-int mx4_few_counters() { return kEnough; }
+int mx4_few_counters() { return few_enough(16); }
 
-size_t mx4_few_partial_bytes(int max_rows, bool gated) {
-  const int n = max_rows <= 16 ? 16 : max_rows <= 32 ? 32 : max_rows <= 64 ? 64 : 128;
-  return (size_t)kUnitsMost * (gated ? 2 : 1) * n * 128 * sizeof(float);
+// The same for every width, so that a workspace made for many rows serves few.
+size_t mx4_few_partial_bytes(bool gated) {
+  size_t most = 0;
+  for (int n = 16; n <= 128; n *= 2) {
+    const size_t floats = (size_t)2 * few_enough(n) * (gated ? 2 : 1) * n * 128;
+    most = floats > most ? floats : most;
+  }
+  return most * sizeof(float);
 }
 
 int launch_mx4_linear_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, const void* w_codes,

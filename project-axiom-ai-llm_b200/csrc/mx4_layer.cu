@@ -54,10 +54,10 @@ struct FewWs {
   uint32_t* counters;
   float* partial;
 };
-FewWs carve_few(Carver& c, int max_rows, bool gated) {
+FewWs carve_few(Carver& c, bool gated) {
   FewWs w;
   w.counters = static_cast<uint32_t*>(c.take(sizeof(uint32_t) * mx4_few_counters()));
-  w.partial = static_cast<float*>(c.take(mx4_few_partial_bytes(max_rows, gated)));
+  w.partial = static_cast<float*>(c.take(mx4_few_partial_bytes(gated)));
   return w;
 }
 
@@ -72,8 +72,8 @@ LinearWs carve_linear(int tokens, int k, void* base) {
   LinearWs w;
   w.status = static_cast<int32_t*>(c.take(4));
   w.codes = c.take((size_t)tokens * (k / 2));
-  w.scales = c.take((size_t)mx4_row_tiles(tokens, 1) * mx4_chunks(k) * 512);
-  w.few = carve_few(c, tokens, false);
+  w.scales = c.take((size_t)mx4_row_tiles_most(tokens, 1) * mx4_chunks(k) * 512);
+  w.few = carve_few(c, false);
   w.bytes = c.off;
   return w;
 }
@@ -84,18 +84,18 @@ struct FfnWs {
   FewWs few;
   size_t bytes;
 };
-void carve_ffn(Carver& c, int rows, int num_segments, int tokens, int d, int f, FfnWs* w) {
-  w->few = carve_few(c, tokens, true);
+void carve_ffn(Carver& c, int rows, int num_segments, int d, int f, FfnWs* w) {
+  w->few = carve_few(c, true);
   w->x_codes = c.take((size_t)rows * (d / 2));
-  w->x_scales = c.take((size_t)mx4_row_tiles(rows, num_segments) * mx4_chunks(d) * 512);
+  w->x_scales = c.take((size_t)mx4_row_tiles_most(rows, num_segments) * mx4_chunks(d) * 512);
   w->h_codes = c.take((size_t)rows * (f / 2));
-  w->h_scales = c.take((size_t)mx4_row_tiles(rows, num_segments) * mx4_chunks(f) * 512);
+  w->h_scales = c.take((size_t)mx4_row_tiles_most(rows, num_segments) * mx4_chunks(f) * 512);
 }
 FfnWs carve_expert_ffn(const AxmMoeDesc* d, int rows, int num_segments, void* base) {
   Carver c{static_cast<char*>(base)};
   FfnWs w;
   w.status = static_cast<int32_t*>(c.take(4));
-  carve_ffn(c, rows, num_segments, d->tokens, d->d_model, d->d_ff, &w);
+  carve_ffn(c, rows, num_segments, d->d_model, d->d_ff, &w);
   w.bytes = c.off;
   return w;
 }
@@ -103,7 +103,7 @@ FfnWs carve_expert_ffn(const AxmMoeDesc* d, int rows, int num_segments, void* ba
 // Both products of the feed-forward over one range of the table.
 int launch_ffn(const Mx4Rows& r, const FfnWs& w, const AxmMx4Experts* experts, int num_experts, int d, int f, void* o,
                bool o_bf16, cudaStream_t st) {
-  if (mx4_use_few(r.max_rows)) {
+  if (r.few) {
     if (int rc = launch_mx4_gated_few(r, w.x_codes, w.x_scales, experts, num_experts, d, f, w.h_codes, w.h_scales, st)) return rc;
     return launch_mx4_linear_few(r, w.h_codes, w.h_scales, experts->down_codes, experts->down_scales, num_experts, f, d, o,
                                  o_bf16, st);
@@ -142,7 +142,7 @@ LayerWs carve_layer(const AxmMoeDesc* d, void* base) {
   w.row_src = static_cast<int32_t*>(c.take(4 * T * k));
   w.slot_dst = static_cast<int32_t*>(c.take(4 * T * k));
   w.segments = static_cast<AxmSegment*>(c.take(sizeof(AxmSegment) * (E + S)));
-  carve_ffn(c, (int)rows, (int)(E + S), d->tokens, d->d_model, d->d_ff, &w.ffn);
+  carve_ffn(c, (int)rows, (int)(E + S), d->d_model, d->d_ff, &w.ffn);
   w.o = c.take(4 * rows * d->d_model);
   w.router_scratch_bytes = 0;
   axm_moe_router_scratch_bytes(d, &w.router_scratch_bytes);
@@ -188,11 +188,12 @@ extern "C" int axm_mx4_linear(const void* x, int32_t x_dtype, int64_t ld, int32_
   if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
   if (int rc = require_device()) return rc;
   const LinearWs w = carve_linear(tokens, k, workspace);
-  const Mx4Rows rows = {nullptr, 0, tokens, 1, 0, 0, tokens, w.status, w.few.partial, w.few.counters};
+  const int tile = mx4_tile_rows(tokens, 1, tokens);
+  const Mx4Rows rows = {nullptr, 1, tokens, 1, 0, 0, tile ? tile : 128, tile != 0, w.status, w.few.partial, w.few.counters};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Mx4Gather from = {nullptr, 1, tokens, 1};
   if (int rc = launch_mx4_quantize_rows(x, x_dtype, ld, from, rows, k, w.codes, w.scales, st)) return rc;
-  return (mx4_use_few(tokens) ? launch_mx4_linear_few : launch_mx4_linear)(rows, w.codes, w.scales, w_codes, w_scales, 1, k,
+  return (rows.few ? launch_mx4_linear_few : launch_mx4_linear)(rows, w.codes, w.scales, w_codes, w_scales, 1, k,
                                                                            n, out, out_dtype == AXM_DTYPE_BF16, st);
 }
 
@@ -224,7 +225,8 @@ extern "C" int axm_mx4_expert_ffn(const AxmMoeDesc* desc, const void* x, int32_t
   if (int rc = require_device()) return rc;
   const int D = desc->d_model, F = desc->d_ff;
   const FfnWs w = carve_expert_ffn(desc, rows, num_segments, workspace);
-  const Mx4Rows r = {segments, num_segments, rows, num_segments, 0, 0, desc->tokens, w.status, w.few.partial, w.few.counters};
+  const int tile = mx4_tile_rows(rows, num_segments, desc->tokens);
+  const Mx4Rows r = {segments, num_segments, rows, num_segments, 0, 0, tile ? tile : 128, tile != 0, w.status, w.few.partial, w.few.counters};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Mx4Gather from = {nullptr, 1, rows, 1};
   if (int rc = launch_mx4_quantize_rows(x, AXM_DTYPE_BF16, D, from, r, D, w.x_codes, w.x_scales, st)) return rc;
@@ -271,7 +273,9 @@ extern "C" int axm_moe_forward_mx4(const AxmMoeDesc* desc, const AxmMoeTensors* 
                            w.segments, cleared ? nullptr : w.ffn.status, st, 1)))
     return rc;
   const int rows = T * (k + S);
-  Mx4Rows r = {w.segments, E + S, rows, E + S, 0, 0, T, nullptr, w.ffn.few.partial, w.ffn.few.counters};
+  // one kind of kernel and of scale tile for the whole table: the routed experts'
+  const int tile = mx4_tile_rows(rows, E + S, T);
+  Mx4Rows r = {w.segments, E + S, rows, E + S, 0, 0, tile ? tile : 128, tile != 0, nullptr, w.ffn.few.partial, w.ffn.few.counters};
   const Mx4Gather from = {row_src, k, T * k, T};
   if ((rc = launch_mx4_quantize_rows(t->x, AXM_DTYPE_BF16, D, from, r, D, w.ffn.x_codes, w.ffn.x_scales, st))) return rc;
   r.status = w.ffn.status;

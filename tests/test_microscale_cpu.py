@@ -104,7 +104,7 @@ def test_linear_refuses(lib, axm):
     assert lib.axm_mx4_linear_workspace_bytes(5, 64, 24, ctypes.byref(n)) == 0 and n.value > 0
     assert lib.axm_mx4_linear_workspace_bytes(5, 64, 20, ctypes.byref(n)) == axm.AXM_ERR_ARGUMENT
 
-    def call(x=FAKE, dt=0, ld=64, t=5, k=64, nn=24, wc=FAKE, ws=FAKE, out=FAKE, odt=0, work=FAKE, size=1 << 20):
+    def call(x=FAKE, dt=0, ld=64, t=5, k=64, nn=24, wc=FAKE, ws=FAKE, out=FAKE, odt=0, work=FAKE, size=1 << 26):
         return lib.axm_mx4_linear(x, dt, ld, t, k, nn, wc, ws, out, odt, work, size, None)
 
     for kw in [dict(x=None), dict(wc=None), dict(ws=None), dict(out=None), dict(dt=7), dict(odt=7), dict(ld=62),
@@ -130,7 +130,7 @@ def test_expert_ffn_refuses(lib, axm):
     d = axm.make_desc(4, 64, 64, 2, 1)
     w = experts(axm)
 
-    def call(x=FAKE, rows=4, seg=FAKE, nseg=2, e=w, o=FAKE, dt=0, work=FAKE, size=1 << 20):
+    def call(x=FAKE, rows=4, seg=FAKE, nseg=2, e=w, o=FAKE, dt=0, work=FAKE, size=1 << 26):
         return lib.axm_mx4_expert_ffn(ctypes.byref(d), x, rows, seg, nseg, None if e is None else ctypes.byref(e), o, dt,
                                       work, size, None)
 

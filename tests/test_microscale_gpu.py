@@ -228,7 +228,8 @@ def test_linear_not_finite(ms, cuda_device):
 
 FFN = [([1], 64, 32), ([0, 1, 0, 1], 256, 512), ([3, 0, 2, 0, 0, 11], 96, 160), ([16, 1, 0, 15], 288, 416),
        ([40, 17, 0, 64], 544, 224), ([129, 0, 1, 300, 128], 160, 352), ([1] * 40 + [0] * 24 + [90], 128, 96),
-       ([260, 255], 1024, 1408)]
+       ([260, 255], 1024, 1408), ([0] * 9 + [33, 70], 96, 64), ([50, 3, 45, 64, 65, 0, 40], 160, 288), ([1] * 60 + [200, 130], 64, 96),
+       ([12, 16, 17, 0, 1, 9], 320, 160), ([3] * 512, 64, 64)]
 
 
 def exact_expert_weights(ms, e, k, n, dev, seed, shift):
