@@ -40,12 +40,16 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
 }
 
 // Rows are cut into runs of 512 elements, one warp a run: a lane holds sixteen neighbours (32 bytes
-// of bf16), two lanes a block.  A CTA of eight warps gives each row 2^log_wpr of them (as many as
-// the row has runs, up to eight), and a warp has up to kAhead runs' loads in flight.
+// of bf16), two lanes a block.  Of rows of up to 256 (128) elements a warp takes two (four), 2^log_lanes
+// lanes each.  A CTA of eight warps gives each row 2^log_wpr of them (as many as
+// the row has runs, up to eight; in large calls fewer, so that each has several runs), and a warp
+// has up to kAheadOf<T> runs' loads in flight.
 // These kernels are bound by their instructions as easily as by memory: a first form with eight
 // elements a lane and fp32 arithmetic throughout issued 160 instructions per 256 elements and read
 // and wrote 3.9 TB/s.
-constexpr int kAhead = 2;
+constexpr int kMostAhead = 4;
+template <typename T>
+constexpr int kAheadOf = sizeof(T) == 2 ? kMostAhead : kMostAhead / 2;  // the same registers
 
 // What the first kernel of a call clears for the ones behind it.
 struct MxClear {
@@ -59,9 +63,9 @@ struct MxClear {
 // kWide: rows start at multiples of 32 bytes.
 // `from` says which source row a row comes from; row_src[r] < 0: zeros.
 template <int kBits, typename T, bool kWide>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, int rows, int k, int log_wpr,
-                        const AxmSegment* __restrict__ segments, int num_segments, int tile_rows,
+                        int log_lanes, const AxmSegment* __restrict__ segments, int num_segments, int tile_rows,
                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, MxClear clear) {
   // a product that is launched to start early may prepare itself now; it waits before it reads
   asm volatile("griddepcontrol.launch_dependents;");
@@ -70,43 +74,30 @@ mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, i
     for (int i = threadIdx.x; i < clear.num_counters; i += 256) clear.counters[i] = 0u;
   }
   constexpr bool kBf16 = sizeof(T) == 2;
+  constexpr int kAhead = kAheadOf<T>;
   constexpr int kWords = kBf16 ? 1 : 2;  // 32-byte pieces a lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int runs = (k + 511) / 512, wpr = 1 << log_wpr;
-  const int rows_per_cta = 8 >> log_wpr;
-  for (long long row_at = (long long)blockIdx.x * rows_per_cta + (warp >> log_wpr); row_at < rows;
+  const int log_rpw = 5 - log_lanes;  // rows a warp (more than one only where a row is one run)
+  const int group = lane >> log_lanes, in_row = lane & ((1 << log_lanes) - 1);
+  const int rows_per_cta = (8 >> log_wpr) << log_rpw;
+  for (long long row_at = (long long)blockIdx.x * rows_per_cta + ((warp >> log_wpr) << log_rpw); row_at < rows;
        row_at += (long long)gridDim.x * rows_per_cta) {
-    const int row = (int)row_at;
-    long long src = row;
-    if (row >= from.tail_row0) {
+    const int row = (int)row_at + group;
+    const bool there = row < rows;
+    long long src = there ? row : -1;
+    if (there && row >= from.tail_row0) {
       src = (row - from.tail_row0) % from.tail_mod;
-    } else if (from.row_src != nullptr) {
+    } else if (there && from.row_src != nullptr) {
       const int s = __ldg(from.row_src + row);
       src = s < 0 ? -1 : s / from.row_div;
     }
     const T* in = x + (src < 0 ? 0 : src) * ld;
-    uint8_t* out = codes + (size_t)row * (kBits == 4 ? k >> 1 : k);
-    uint8_t* sc = scales;  // this row's scale bytes; kBits 4: in chunk 0
-    bool placed = true;    // a row behind its segment's end has no place among the tiles
-    if constexpr (kBits == 4) {
-      int seg = 0, first = 0;
-      if (segments != nullptr) {
-        seg = segment_of_row(segments, num_segments, row);
-        placed = seg >= 0;
-        if (placed) first = __ldg(&segments[seg].out_row0);
-      }
-      const int r = row - first;
-      const int in_tile = r & (tile_rows - 1);
-      sc += ((size_t)(first / tile_rows + (placed ? seg : 0) + r / tile_rows) * mx4_chunks(k)) * 512 + (in_tile & 31) * 16 +
-            (in_tile >> 5) * 4;
-    } else {
-      sc += (size_t)row * (k >> 5);
-    }
-    for (int run0 = warp & (wpr - 1); run0 < runs; run0 += kAhead * wpr) {
-      Words8 v[kAhead][kWords];
+    Words8 v[kAhead][kWords];
+    auto fetch = [&](int run0) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int k0 = (run0 + i * wpr) * 512 + lane * 16;  // k is a multiple of 32: all sixteen or none
+        const int k0 = (run0 + i * wpr) * 512 + in_row * 16;  // k is a multiple of 32: all sixteen or none
         if (k0 < k && src >= 0) {
 #pragma unroll
           for (int j = 0; j < kWords; ++j) v[i][j] = load32<kWide>(in + k0 + 8 * j);
@@ -115,11 +106,36 @@ mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, i
           for (int j = 0; j < kWords; ++j) v[i][j] = Words8{};
         }
       }
+    };
+    int run0 = warp & (wpr - 1);
+    fetch(run0);  // on their way while the row's segment is looked up
+    uint8_t* out = codes + (size_t)row * (kBits == 4 ? k >> 1 : k);
+    uint8_t* sc = scales;  // this row's scale bytes; kBits 4: in chunk 0
+    bool placed = there;   // a row behind its segment's end has no place among the tiles
+    if constexpr (kBits == 4) {
+      RowSegment at = {0, 0};
+      if (segments != nullptr) {
+        for (int g = 0; g < (1 << log_rpw); ++g) {
+          const RowSegment found = segment_of_row(segments, num_segments, (int)row_at + g);
+          if (g == group) at = found;
+        }
+        placed = there && at.seg >= 0;
+      }
+      const int r = placed ? row - at.first : 0;
+      const int in_tile = r & (tile_rows - 1);
+      sc += ((size_t)(at.first / tile_rows + (placed ? at.seg : 0) + r / tile_rows) * mx4_chunks(k)) * 512 +
+            (in_tile & 31) * 16 + (in_tile >> 5) * 4;
+    } else {
+      sc += (size_t)row * (k >> 5);
+    }
+    for (; run0 < runs; run0 += kAhead * wpr) {
+      if (run0 >= kAhead * wpr) fetch(run0);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int run = run0 + i * wpr;
         if (run >= runs) break;
-        const int k0 = run * 512 + lane * 16;
+        const int k0 = run * 512 + in_row * 16;
+        const bool write = there && k0 < k;
         uint32_t top = 0;
         if constexpr (kBf16) {  // largest magnitude by the bits, two at a time
 #pragma unroll
@@ -149,14 +165,16 @@ mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, i
             for (int j = 0; j < 8; ++j) t[j] = value(8 * h + j);
             c[h] = mx4_pack8(t);
           }
-          if (k0 < k) *reinterpret_cast<uint2*>(out + (k0 >> 1)) = make_uint2(c[0], c[1]);
+          if (write) *reinterpret_cast<uint2*>(out + (k0 >> 1)) = make_uint2(c[0], c[1]);
           // the four bytes of a 128-element chunk gathered into one word by the chunk's first lane
           uint32_t word = s << (8 * ((lane >> 1) & 3));
           word |= __shfl_xor_sync(0xffffffffu, word, 2);
           word |= __shfl_xor_sync(0xffffffffu, word, 4);
-          const int chunk = run * 4 + (lane >> 3);
+          const int chunk = run * 4 + (in_row >> 3);
           if (placed && (lane & 7) == 0 && chunk < mx4_chunks(k)) *reinterpret_cast<uint32_t*>(sc + (size_t)chunk * 512) = word;
-        } else if (k0 < k) {
+          // eight lanes hold one chunk; a stage has two
+          if (log_lanes == 3 && placed && in_row == 0) *reinterpret_cast<uint32_t*>(sc + 512) = 0u;
+        } else if (write) {
           uint32_t c[4];
 #pragma unroll
           for (int h = 0; h < 4; ++h) c[h] = mx8_pack4(value(4 * h), value(4 * h + 1), value(4 * h + 2), value(4 * h + 3));
@@ -171,26 +189,33 @@ mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, i
 template <int kBits, typename T, bool kWide>
 __global__ void __launch_bounds__(256)
 mx_dequantize_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int k,
-                          int log_wpr, const AxmSegment* __restrict__ segments, int num_segments,
-                          T* __restrict__ out, long long ld) {
+                          int log_wpr, int log_lanes, const AxmSegment* __restrict__ segments,
+                          int num_segments, T* __restrict__ out, long long ld) {
+  constexpr int kAhead = kMostAhead;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int runs = (k + 511) / 512, wpr = 1 << log_wpr;
-  const int rows_per_cta = 8 >> log_wpr;
-  for (long long row_at = (long long)blockIdx.x * rows_per_cta + (warp >> log_wpr); row_at < rows;
+  const int log_rpw = 5 - log_lanes;
+  const int group = lane >> log_lanes, in_row = lane & ((1 << log_lanes) - 1);
+  const int rows_per_cta = (8 >> log_wpr) << log_rpw;
+  for (long long row_at = (long long)blockIdx.x * rows_per_cta + ((warp >> log_wpr) << log_rpw); row_at < rows;
        row_at += (long long)gridDim.x * rows_per_cta) {
-    const int row = (int)row_at;
+    const int row = (int)row_at + group;
+    bool there = row < rows;
     const uint8_t* in = codes + (size_t)row * (kBits == 4 ? k >> 1 : k);
     const uint8_t* sc = scales;
     T* to = out + (size_t)row * ld;
     if constexpr (kBits == 4) {
-      int seg = 0, first = 0;
+      RowSegment at = {0, 0};
       if (segments != nullptr) {
-        seg = segment_of_row(segments, num_segments, row);
-        if (seg < 0) continue;  // left as it is
-        first = __ldg(&segments[seg].out_row0);
+        for (int g = 0; g < (1 << log_rpw); ++g) {
+          const RowSegment found = segment_of_row(segments, num_segments, (int)row_at + g);
+          if (g == group) at = found;
+        }
+        there = there && at.seg >= 0;  // others are left as they are
+        if (at.seg < 0) at = RowSegment{0, row};
       }
-      const int r = row - first;
-      sc += ((size_t)(first / 128 + seg + r / 128) * mx4_chunks(k)) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4;
+      const int r = row - at.first;
+      sc += ((size_t)(at.first / 128 + at.seg + r / 128) * mx4_chunks(k)) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4;
     } else {
       sc += (size_t)row * (k >> 5);
     }
@@ -199,15 +224,15 @@ mx_dequantize_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __re
       uint32_t s[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int run = run0 + i * wpr, k0 = run * 512 + lane * 16;
+        const int run = run0 + i * wpr, k0 = run * 512 + in_row * 16;
         c[i] = make_uint4(0, 0, 0, 0);
         s[i] = 0;
-        if (k0 < k) {
+        if (there && k0 < k) {
           if constexpr (kBits == 4) {
             const uint2 t = __ldg(reinterpret_cast<const uint2*>(in + (k0 >> 1)));
             c[i].x = t.x;
             c[i].y = t.y;
-            s[i] = __ldg(sc + (size_t)(run * 4 + (lane >> 3)) * 512 + ((lane >> 1) & 3));
+            s[i] = __ldg(sc + (size_t)(run * 4 + (in_row >> 3)) * 512 + ((lane >> 1) & 3));
           } else {
             c[i] = __ldg(reinterpret_cast<const uint4*>(in + k0));
             s[i] = __ldg(sc + (k0 >> 5));
@@ -216,8 +241,8 @@ mx_dequantize_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __re
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int k0 = (run0 + i * wpr) * 512 + lane * 16;
-        if (k0 >= k) break;
+        const int k0 = (run0 + i * wpr) * 512 + in_row * 16;
+        if (!there || k0 >= k) break;
         const uint32_t f = mx_scale_bf16x2(s[i]);
         uint32_t w[8];
         if constexpr (kBits == 4) {
@@ -441,13 +466,17 @@ int check_matrix(const void* p, int32_t dtype, int64_t ld, int32_t k, const char
 
 // Warps a row (as a power of two) and CTAs of a row kernel.
 struct RowLaunch {
-  int log_wpr;
+  int log_wpr, log_lanes;
   unsigned grid;
 };
-RowLaunch row_launch(int32_t rows, int32_t k) {
-  RowLaunch l = {0, 0};
-  while (l.log_wpr < 3 && (2 << l.log_wpr) <= (k + 511) / 512) ++l.log_wpr;
-  const long long per = 8 >> l.log_wpr;
+RowLaunch row_launch(int32_t rows, int32_t k, int ahead) {
+  RowLaunch l = {0, k <= 128 ? 3 : k <= 256 ? 4 : 5, 0};
+  const int runs = (k + 511) / 512;
+  while (l.log_wpr < 3 && (2 << l.log_wpr) <= runs) ++l.log_wpr;
+  // enough rows for every SM's warps: several runs a warp rather than several warps a row (not for
+  // fp32 sources, ahead = 1: their runs are twice as long, 8-bit rows 8191 x 5632 58 us against 63)
+  while (l.log_wpr > 0 && (runs >> l.log_wpr) < ahead && ((long long)rows << (l.log_wpr - 1)) >= 128LL * sm_count()) --l.log_wpr;
+  const long long per = (long long)(8 >> l.log_wpr) << (5 - l.log_lanes);
   const long long blocks = (rows + per - 1) / per, most = 32LL * sm_count();
   l.grid = (unsigned)(blocks < most ? blocks : most);
   return l;
@@ -461,9 +490,9 @@ template <int kBits, typename T>
 int launch_quantize_rows_of(const void* x, bool wide, int64_t ld, const Mx4Gather& from, int32_t rows, int32_t k,
                             const AxmSegment* segments, int32_t num_segments, int tile_rows, void* codes, void* scales,
                             const MxClear& clear, cudaStream_t st) {
-  const RowLaunch l = row_launch(rows, k);
+  const RowLaunch l = row_launch(rows, k, sizeof(T) == 2 ? kMostAhead : 1);
   auto* kernel = wide ? mx_quantize_rows_kernel<kBits, T, true> : mx_quantize_rows_kernel<kBits, T, false>;
-  kernel<<<l.grid, 256, 0, st>>>(static_cast<const T*>(x), ld, from, rows, k, l.log_wpr, segments, num_segments, tile_rows,
+  kernel<<<l.grid, 256, 0, st>>>(static_cast<const T*>(x), ld, from, rows, k, l.log_wpr, l.log_lanes, segments, num_segments, tile_rows,
                                  static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), clear);
   return check_launch("mx_quantize_rows_kernel");
 }
@@ -480,10 +509,10 @@ int launch_quantize_rows(const void* x, int32_t dtype, int64_t ld, const Mx4Gath
 template <int kBits, typename T>
 int launch_dequantize_rows_of(const void* codes, const void* scales, int32_t rows, int32_t k, const AxmSegment* segments,
                               int32_t num_segments, void* out, bool wide, int64_t ld, cudaStream_t st) {
-  const RowLaunch l = row_launch(rows, k);
+  const RowLaunch l = row_launch(rows, k, kMostAhead);
   auto* kernel = wide ? mx_dequantize_rows_kernel<kBits, T, true> : mx_dequantize_rows_kernel<kBits, T, false>;
   kernel<<<l.grid, 256, 0, st>>>(static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, k,
-                                 l.log_wpr, segments, num_segments, static_cast<T*>(out), ld);
+                                 l.log_wpr, l.log_lanes, segments, num_segments, static_cast<T*>(out), ld);
   return check_launch("mx_dequantize_rows_kernel");
 }
 template <int kBits>

@@ -178,16 +178,29 @@ __device__ __forceinline__ float2 mx8_unpack2(uint32_t two) {
 }
 
 // The segment that output row `row` belongs to (the last one that starts at or before it and has
-// rows); tables are ordered by out_row0.  -1: the row is behind its segment's end.
-__device__ __forceinline__ int segment_of_row(const AxmSegment* segments, int n, int row) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(&segments[mid].out_row0) <= row) lo = mid; else hi = mid - 1;
+// rows), and its first row; tables are ordered by out_row0.  -1: the row is behind its segment's end.
+// By a whole warp: 32 entries at a time, all loads of a round at once (a binary search is a chain of
+// dependent loads, 3 us for 64 segments, which every row of a small call waited for).
+struct RowSegment {
+  int seg, first;
+};
+__device__ __forceinline__ RowSegment segment_of_row(const AxmSegment* segments, int n, int row) {
+  const int lane = threadIdx.x & 31;
+  RowSegment r = {-1, 0};
+  int rows = 0;
+  for (int s0 = 0; s0 < n; s0 += 32) {
+    const int4 e = s0 + lane < n ? __ldg(reinterpret_cast<const int4*>(segments) + s0 + lane) : make_int4(0, 0x7fffffff, 0, 0);
+    // segments without rows share their start with the next one: the last of them is found
+    const uint32_t here = __ballot_sync(0xffffffffu, e.y <= row);
+    if (here == 0) break;
+    const int at = 31 - __clz(here);
+    r.seg = s0 + at;
+    r.first = __shfl_sync(0xffffffffu, e.y, at);
+    rows = __shfl_sync(0xffffffffu, e.z, at);
+    if (at < 31) break;
   }
-  // segments without rows share their start with the next one: the last of them was found
-  const int first = __ldg(&segments[lo].out_row0);
-  return (row >= first && row - first < __ldg(&segments[lo].rows)) ? lo : -1;
+  if (row - r.first >= rows) r.seg = -1;
+  return r;
 }
 
 #endif

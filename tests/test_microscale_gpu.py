@@ -63,7 +63,7 @@ def held_float(x, bits, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
-@pytest.mark.parametrize("rows,k", [(1, 32), (1, 4096), (7, 96), (129, 288), (300, 544), (1031, 2048)])
+@pytest.mark.parametrize("rows,k", [(1, 32), (1, 4096), (7, 96), (129, 288), (300, 544), (1031, 2048), (77, 128), (1001, 64), (515, 256), (3, 224)])
 def test_rows_4_bits(ms, cuda_device, rows, k, dtype):
     x = awkward(rows, k, dtype, cuda_device, rows + k)
     q = ms.quantize_rows(x)
@@ -84,7 +84,7 @@ def test_rows_4_bits(ms, cuda_device, rows, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
-@pytest.mark.parametrize("rows,k", [(1, 32), (3, 4096), (129, 288), (1031, 416)])
+@pytest.mark.parametrize("rows,k", [(1, 32), (3, 4096), (129, 288), (1031, 416), (77, 128), (1001, 64), (515, 256), (3, 224)])
 def test_rows_8_bits(ms, cuda_device, rows, k, dtype):
     x = awkward(rows, k, dtype, cuda_device, rows * k)
     codes, s = ms.quantize_rows8(x)
@@ -110,14 +110,14 @@ def test_rows_with_strides_and_sources(ms, cuda_device):
         ms.quantize_rows(wide[:, 4:4 + 288])  # not 16-byte aligned
 
 
+@pytest.mark.parametrize("k", [96, 160, 544])
 @pytest.mark.parametrize("counts", [[5], [0, 3, 0, 0, 200, 1, 0], [128, 128, 127, 129, 0], [1] * 70, [300, 0, 0]])
-def test_rows_by_segments(ms, cuda_device, counts):
+def test_rows_by_segments(ms, cuda_device, counts, k):
     segs, rows = table(counts, cuda_device)
-    k = 160
     x = awkward(rows + 9, k, FP32, cuda_device, sum(counts))  # nine rows behind the last segment
     q = ms.quantize_rows(x, segments=segs)
     s = ref.scale_bytes(x, 2)
-    got = q.scales.view(-1, 2, 512)
+    got = q.scales.view(-1, (k + 255) // 256 * 2, 512)
     at = 0
     for e, c in enumerate(counts):
         if c:
