@@ -109,6 +109,29 @@ __device__ __forceinline__ void tc_mma2_bf16(uint32_t d_tmem, uint64_t desc_a, u
 }
 
 
+// Programmatic launches: a kernel that is followed by one launched this way lets it start at once, and
+// one launched this way waits, before it touches global memory, until everything before it is done.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Launches a pair kernel (its clusters of two are compiled in) so that it may start, up to its
+// wait_for_previous(), while the kernel before it drains.
+template <typename Kernel, typename... Args>
+int launch_overlapping(const char* what, Kernel kernel, int grid, int threads, size_t smem, cudaStream_t st,
+                       const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
+
 // Number of CTAs to launch (two per cluster), 0 when pairs cannot be scheduled, or a
 // negative status (defined in grouped_ffn_2sm.cu).
 int grid_2sm();

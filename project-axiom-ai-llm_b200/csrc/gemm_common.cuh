@@ -118,15 +118,24 @@ bool use_2sm_kernels();
 // Input-gradient GEMM of the backward pass on CTA pairs (grouped_ffn_2sm.cu).
 int launch_bwd_dx_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t num_segments,
                       int32_t rows_total, const void* d_g, const void* d_u, const void* w_gate,
-                      const void* w_up, void* d_xp, int32_t* status, cudaStream_t st, bool out_bf16 = false);
+                      const void* w_up, void* d_xp, int32_t* status, cudaStream_t st, bool out_bf16 = false,
+                      bool overlap = false);
 // dH GEMM of the backward pass with the SwiGLU derivative, on CTA pairs (grouped_ffn_2sm.cu).
 int launch_bwd_dh_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t num_segments,
                       int32_t rows_total, const void* d_o, const void* w_down, const void* g, const void* u,
                       void* d_g, void* d_u, int32_t* status, cudaStream_t st);
-// Weight-gradient GEMM of the backward pass on CTA pairs (grouped_bwd_2sm.cu).
+// Weight-gradient GEMMs of the backward pass on CTA pairs (grouped_bwd_2sm.cu): up to three of them in
+// one launch.
+struct WgradProblem {
+  const void* a;  // [rows][m]
+  int32_t m;
+  const void* b;  // [rows][n]
+  int32_t n;
+  void* d_w;      // [experts][m][n]
+};
 int launch_wgrad_2sm(const AxmSegment* segments, int32_t num_segments, int32_t rows_total, int32_t experts,
-                     const void* a, int32_t m_total, const void* b, int32_t n_total, void* d_w,
-                     int32_t* status, cudaStream_t st, bool out_bf16 = false);
+                     const WgradProblem* problems, int32_t num_problems, int32_t* status, cudaStream_t st,
+                     bool out_bf16 = false, bool overlap = false);
 // The training step with g and u kept in 8 bits (grouped_ffn_2sm.cu).
 int launch_train8_forward(const AxmMoeDesc* d, const AxmSegment* segments, int32_t num_segments, int32_t rows_total,
                           const void* x_perm, const void* w_gate, const void* w_up, const void* w_down,

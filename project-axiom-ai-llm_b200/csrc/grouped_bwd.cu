@@ -552,7 +552,10 @@ int launch_expert_ffn_backward(const AxmMoeDesc* desc, const AxmSegment* segment
                        int n_total, void* out, const CUtensorMap& omap, const char* what) -> int {
     int r = AXM_ERR_DEVICE;
     if (use_2sm_kernels())
-      r = launch_wgrad_2sm(segments, num_segments, rows_total, E, am, m_total, bm, n_total, out, status, st);
+      {
+      const WgradProblem one = {am, m_total, bm, n_total, out};
+      r = launch_wgrad_2sm(segments, num_segments, rows_total, E, &one, 1, status, st);
+    }
     if (r != AXM_ERR_DEVICE) return r;
     a.m_total = m_total;
     a.n_total = n_total;

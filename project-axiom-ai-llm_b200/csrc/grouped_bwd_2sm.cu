@@ -35,12 +35,20 @@ constexpr size_t kWgrad2SmemBytes =
     1024 + (size_t)kStages2 * kStageBytes2 + kWgradStagingBytes + sizeof(WgradShared2);
 static_assert(kWgrad2SmemBytes <= 227u * 1024u, "shared memory of the pair weight-gradient kernel");
 
+constexpr int kWgradProblems = 3;
 struct Wgrad2Args {
   const AxmSegment* segments;
   int num_segments;
-  int m_total;  // rows of one expert's gradient
-  int n_total;  // columns
+  int num_problems;
+  int m_total[kWgradProblems];  // rows of one expert's gradient
+  int n_total[kWgradProblems];  // columns
+  int units_before[kWgradProblems + 1];
   int* status;
+  int overlap;  // see launch_overlapping
+};
+// The maps of a launch's problems: A, B and the gradient.
+struct Wgrad2Maps {
+  CUtensorMap a[kWgradProblems], b[kWgradProblems], out[kWgradProblems];
 };
 
 // fp32 accumulate, bf16 A and B both MN-major, N = 256, M = 256 over the pair
@@ -48,13 +56,19 @@ constexpr uint32_t kInstrDescWgrad2 = (1u << 4) | (1u << 7) | (1u << 10) | (1u <
                                       ((uint32_t)(UMMA_N >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
 
 struct WgradUnit {
-  int seg, n_tile, m_tile, a_m_tile;
+  int problem, seg, n_tile, m_tile, a_m_tile;
   bool live;  // false: this half of the pair has no tile (odd number of m-tiles)
 };
 
-__device__ __forceinline__ WgradUnit decode_wgrad(int unit, int pairs_w, int n_tiles, int m_tiles, int rank) {
-  const int per = pairs_w * n_tiles;
+__device__ __forceinline__ WgradUnit decode_wgrad(const Wgrad2Args& args, int unit, int rank) {
   WgradUnit u;
+  u.problem = 0;
+  while (u.problem + 1 < args.num_problems && unit >= args.units_before[u.problem + 1]) ++u.problem;
+  unit -= args.units_before[u.problem];
+  const int n_tiles = (args.n_total[u.problem] + UMMA_N - 1) / UMMA_N;
+  const int m_tiles = (args.m_total[u.problem] + BM - 1) / BM;
+  const int pairs_w = (m_tiles + 1) / 2;
+  const int per = pairs_w * n_tiles;
   u.seg = unit / per;
   const int local = unit - u.seg * per;
   u.n_tile = local / pairs_w;
@@ -69,8 +83,7 @@ __device__ __forceinline__ WgradUnit decode_wgrad(int unit, int pairs_w, int n_t
 // the largest outputs of a training step.
 template <bool kBf16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
-grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                         const __grid_constant__ CUtensorMap tm_out, Wgrad2Args args) {
+grouped_wgrad_2sm_kernel(const __grid_constant__ Wgrad2Maps maps, const __grid_constant__ Wgrad2Args args) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* tiles = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -83,13 +96,10 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
   const uint32_t peer = rank ^ 1u;
   const int cluster_id = blockIdx.x >> 1;
   const int num_clusters = gridDim.x >> 1;
-  const int n_tiles = (args.n_total + UMMA_N - 1) / UMMA_N;
-  const int m_tiles = (args.m_total + BM - 1) / BM;
-  const int pairs_w = (m_tiles + 1) / 2;
   const int nseg = args.num_segments;
-  const int total_units = nseg * pairs_w * n_tiles;
+  const int total_units = args.units_before[args.num_problems];
 
-  for (int s = threadIdx.x; s < nseg; s += kGemmThreads) sh->seg[s] = args.segments[s];
+  if (args.overlap) launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages2; ++i) {
       mbar_init(&sh->full[i], 1);
@@ -101,16 +111,17 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
     }
     sh->abort_flag = 0;
     fence_barrier_init();
-    tma_prefetch_desc(&tm_a);
-    tma_prefetch_desc(&tm_b);
-    tma_prefetch_desc(&tm_out);
+    tma_prefetch_desc(&maps.a[0]);
+    tma_prefetch_desc(&maps.b[0]);
+    tma_prefetch_desc(&maps.out[0]);
   }
-  __syncthreads();
   if (warp == 1) {
     __syncwarp();
     tmem_alloc2(&sh->tmem_base, kTmemCols);
     tmem_relinquish2();
   }
+  if (args.overlap) wait_for_previous();
+  for (int s = threadIdx.x; s < nseg; s += kGemmThreads) sh->seg[s] = args.segments[s];
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // barriers of both CTAs are initialised before anyone signals across
@@ -129,7 +140,7 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
       uint32_t phase = 0;
       bool ok = true;
       for (int unit = cluster_id; ok && unit < total_units; unit += num_clusters) {
-        const WgradUnit u = decode_wgrad(unit, pairs_w, n_tiles, m_tiles, (int)rank);
+        const WgradUnit u = decode_wgrad(args, unit, (int)rank);
         const AxmSegment sg = sh->seg[u.seg];
         const int k_blocks = (sg.rows + BK - 1) / BK;
         const int a_col = u.a_m_tile * BM;
@@ -146,9 +157,9 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
           const uint32_t bar = map_to_cta(smem_u32(&sh->full[stage]), 0);
           const int row = sg.a_row0 + kb * BK;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) tma2_load_2d(sa + c * kBChunkBytes, &tm_a, bar, a_col + c * 64, row);
+          for (int c = 0; c < 2; ++c) tma2_load_2d(sa + c * kBChunkBytes, &maps.a[u.problem], bar, a_col + c * 64, row);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) tma2_load_2d(sb + c * kBChunkBytes, &tm_b, bar, b_col + c * 64, row);
+          for (int c = 0; c < 2; ++c) tma2_load_2d(sb + c * kBChunkBytes, &maps.b[u.problem], bar, b_col + c * 64, row);
           if (++stage == kStages2) {
             stage = 0;
             phase ^= 1u;
@@ -166,7 +177,7 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
       uint32_t acc_phase = 0;
       bool ok = true;
       for (int unit = cluster_id; ok && unit < total_units; unit += num_clusters) {
-        const WgradUnit u = decode_wgrad(unit, pairs_w, n_tiles, m_tiles, 0);
+        const WgradUnit u = decode_wgrad(args, unit, 0);
         const int k_blocks = (sh->seg[u.seg].rows + BK - 1) / BK;
         if (!__all_sync(0xffffffffu, mbar_wait(&sh->tmem_empty[acc], acc_phase ^ 1u, abort_flag))) {
           if (lane == 0) raise_abort();
@@ -215,7 +226,7 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
     const uint32_t leader_tmem_empty0 = map_to_cta(smem_u32(&sh->tmem_empty[0]), 0);
     const uint32_t leader_tmem_empty1 = map_to_cta(smem_u32(&sh->tmem_empty[1]), 0);
     for (int unit = cluster_id; unit < total_units; unit += num_clusters) {
-      const WgradUnit u = decode_wgrad(unit, pairs_w, n_tiles, m_tiles, (int)rank);
+      const WgradUnit u = decode_wgrad(args, unit, (int)rank);
       const AxmSegment sg = sh->seg[u.seg];
       const int k_blocks = (sg.rows + BK - 1) / BK;
       if (!__all_sync(0xffffffffu, mbar_wait(&sh->tmem_full[acc], acc_phase, abort_flag))) break;
@@ -238,7 +249,7 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
           // swizzle of the output map (and free of bank conflicts); one TMA store per block.
           if (lane == 0) bulk_wait_read();  // the previous block's store has read the buffer
           __syncwarp();
-          if (n0 + c0 < args.n_total && block_row0 < args.m_total) {
+          if (n0 + c0 < args.n_total[u.problem] && block_row0 < args.m_total[u.problem]) {
             if constexpr (kBf16) {  // rows of 64 bytes, the 64-byte swizzle of the bf16 output map
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
@@ -258,7 +269,7 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
-              tma_store_3d(&tm_out, stage_w, n0 + c0, block_row0, sg.expert & 0xffff);
+              tma_store_3d(&maps.out[u.problem], stage_w, n0 + c0, block_row0, sg.expert & 0xffff);
               bulk_commit_group();
             }
           }
@@ -302,8 +313,8 @@ int map_kbox(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols) {
 
 template <bool kBf16>
 static int launch_wgrad_as(const AxmSegment* segments, int32_t num_segments, int32_t rows_total, int32_t experts,
-                           const void* a, int32_t m_total, const void* b, int32_t n_total, void* d_w, int32_t* status,
-                           cudaStream_t st) {
+                           const WgradProblem* problems, int32_t num_problems, int32_t* status, cudaStream_t st,
+                           bool overlap) {
   static SmemLimitCache smem = {};
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(grouped_wgrad_2sm_kernel<kBf16>), kWgrad2SmemBytes,
                                    &smem, "grouped_wgrad_2sm_kernel"))
@@ -311,37 +322,54 @@ static int launch_wgrad_as(const AxmSegment* segments, int32_t num_segments, int
   const int grid = grid_2sm();
   if (grid < 0) return grid;
   if (grid < 2) return fail(AXM_ERR_DEVICE, "two-SM clusters cannot be scheduled on this device");
-  CUtensorMap ma, mb, mo;
-  int rc;
-  if ((rc = map_kbox(&ma, a, (uint64_t)rows_total, (uint64_t)m_total))) return rc;
-  if ((rc = map_kbox(&mb, b, (uint64_t)rows_total, (uint64_t)n_total))) return rc;
-  const uint64_t dims[3] = {(uint64_t)n_total, (uint64_t)m_total, (uint64_t)experts};
-  const uint64_t size = kBf16 ? 2 : 4;
-  const uint64_t strides[2] = {(uint64_t)n_total * size, (uint64_t)n_total * (uint64_t)m_total * size};
-  const uint32_t box[3] = {32, 32, 1};
-  if constexpr (kBf16) {
-    if ((rc = encode_tensor_map_sw64(&mo, d_w, 3, dims, strides, box))) return rc;
-  } else {
-    if ((rc = encode_tensor_map_f32(&mo, d_w, 3, dims, strides, box))) return rc;
-  }
-  Wgrad2Args wa;
+  Wgrad2Maps maps;
+  Wgrad2Args wa = {};
   wa.segments = segments;
   wa.num_segments = num_segments;
-  wa.m_total = m_total;
-  wa.n_total = n_total;
+  wa.num_problems = num_problems;
   wa.status = status;
-  grouped_wgrad_2sm_kernel<kBf16><<<grid, kGemmThreads, kWgrad2SmemBytes, st>>>(ma, mb, mo, wa);
+  wa.overlap = overlap ? 1 : 0;
+  for (int p = 0; p < num_problems; ++p) {
+    const WgradProblem& w = problems[p];
+    int rc;
+    if ((rc = map_kbox(&maps.a[p], w.a, (uint64_t)rows_total, (uint64_t)w.m))) return rc;
+    if ((rc = map_kbox(&maps.b[p], w.b, (uint64_t)rows_total, (uint64_t)w.n))) return rc;
+    const uint64_t dims[3] = {(uint64_t)w.n, (uint64_t)w.m, (uint64_t)experts};
+    const uint64_t size = kBf16 ? 2 : 4;
+    const uint64_t strides[2] = {(uint64_t)w.n * size, (uint64_t)w.n * (uint64_t)w.m * size};
+    const uint32_t box[3] = {32, 32, 1};
+    if constexpr (kBf16) {
+      if ((rc = encode_tensor_map_sw64(&maps.out[p], w.d_w, 3, dims, strides, box))) return rc;
+    } else {
+      if ((rc = encode_tensor_map_f32(&maps.out[p], w.d_w, 3, dims, strides, box))) return rc;
+    }
+    wa.m_total[p] = w.m;
+    wa.n_total[p] = w.n;
+    const int pairs_w = ((w.m + BM - 1) / BM + 1) / 2, n_tiles = (w.n + UMMA_N - 1) / UMMA_N;
+    wa.units_before[p + 1] = wa.units_before[p] + num_segments * pairs_w * n_tiles;
+  }
+  for (int p = num_problems; p < kWgradProblems; ++p) {
+    maps.a[p] = maps.a[0];
+    maps.b[p] = maps.b[0];
+    maps.out[p] = maps.out[0];
+  }
+  if (overlap)
+    return launch_overlapping("grouped_wgrad_2sm_kernel", grouped_wgrad_2sm_kernel<kBf16>, grid, kGemmThreads,
+                              kWgrad2SmemBytes, st, maps, wa);
+  grouped_wgrad_2sm_kernel<kBf16><<<grid, kGemmThreads, kWgrad2SmemBytes, st>>>(maps, wa);
   return check_launch("grouped_wgrad_2sm_kernel");
 }
 
-// dW[e] = A^T . B over each segment's rows: A [rows_total][m_total], B [rows_total][n_total]
-// (bf16), dW [experts][m_total][n_total] fp32 or bf16.  AXM_ERR_DEVICE when pairs cannot be
+// dW[e] = A^T . B over each segment's rows: A [rows_total][m], B [rows_total][n] (bf16), dW
+// [experts][m][n] fp32 or bf16, for each of the problems.  AXM_ERR_DEVICE when pairs cannot be
 // scheduled, so that the caller can fall back to the one-SM kernel.
 int launch_wgrad_2sm(const AxmSegment* segments, int32_t num_segments, int32_t rows_total, int32_t experts,
-                     const void* a, int32_t m_total, const void* b, int32_t n_total, void* d_w,
-                     int32_t* status, cudaStream_t st, bool out_bf16) {
-  return out_bf16 ? launch_wgrad_as<true>(segments, num_segments, rows_total, experts, a, m_total, b, n_total, d_w, status, st)
-                  : launch_wgrad_as<false>(segments, num_segments, rows_total, experts, a, m_total, b, n_total, d_w, status, st);
+                     const WgradProblem* problems, int32_t num_problems, int32_t* status, cudaStream_t st, bool out_bf16,
+                     bool overlap) {
+  if (num_problems < 1 || num_problems > kWgradProblems)
+    return fail(AXM_ERR_ARGUMENT, "launch_wgrad_2sm: %d problems", num_problems);
+  return out_bf16 ? launch_wgrad_as<true>(segments, num_segments, rows_total, experts, problems, num_problems, status, st, overlap)
+                  : launch_wgrad_as<false>(segments, num_segments, rows_total, experts, problems, num_problems, status, st, overlap);
 }
 
 }  // namespace axm

@@ -66,6 +66,9 @@ struct Gemm2Args {
   uint8_t* scales_g;
   uint8_t* scales_u;
   void* out2;    // kModeDH8: h
+  // The launch overlaps with the ones before and after it (the training step with 8-bit checkpoints,
+  // whose kernels follow one another): see launch_overlapping.
+  int overlap;
 };
 
 constexpr int kStagesDh = 5;  // operand stages of kModeDH (one stage's room goes to its epilogue blocks)
@@ -190,7 +193,7 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
   const int k_blocks = (kDX || two_term) ? 2 * kb_half : kb_half;
   const int nseg = args.num_segments;
 
-  for (int s = threadIdx.x; s < nseg; s += kGemmThreads) sh->seg[s] = args.segments[s];
+  if (args.overlap) launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSt; ++i) {
       mbar_init(&sh->full[i], 1);
@@ -213,12 +216,14 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
     tma_prefetch_desc(&tm_b0);
     if (kSwiGLU) tma_prefetch_desc(&tm_b1);
   }
-  __syncthreads();
   if (warp == 1) {
     __syncwarp();
     tmem_alloc2(&sh->tmem_base, kTmemCols);
     tmem_relinquish2();
   }
+  if (args.overlap) wait_for_previous();
+  for (int s = threadIdx.x; s < nseg; s += kGemmThreads) sh->seg[s] = args.segments[s];
+  __syncthreads();
   if (threadIdx.x == 0) {
     int acc = 0;
     for (int s = 0; s < nseg; ++s) {
@@ -942,7 +947,7 @@ int launch_bwd_dh_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t n
 // Returns AXM_ERR_DEVICE when pairs cannot be scheduled, so that the caller can fall back.
 int launch_bwd_dx_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t num_segments,
                       int32_t rows_total, const void* d_g, const void* d_u, const void* w_gate,
-                      const void* w_up, void* d_xp, int32_t* status, cudaStream_t st, bool out_bf16) {
+                      const void* w_up, void* d_xp, int32_t* status, cudaStream_t st, bool out_bf16, bool overlap) {
   static SmemLimitCache smem_dx = {};
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(grouped_gemm_2sm_kernel<kModeDX>), kGemm2SmemBytes,
                                    &smem_dx, "grouped_gemm_2sm_kernel<dX>"))
@@ -974,6 +979,11 @@ int launch_bwd_dx_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t n
   ga.two_term = 0;
   ga.k_splits = 1;
   ga.split_stride = 0;
+  if (overlap) {
+    ga.overlap = 1;
+    return launch_overlapping("grouped_gemm_2sm_kernel<dX>", grouped_gemm_2sm_kernel<kModeDX>, grid, kGemmThreads,
+                              kGemm2SmemBytes, st, m_dg, m_du, m_wg, m_wu, m_wg, m_wu, m_dg, m_dg, m_dg, m_dg, ga);
+  }
   grouped_gemm_2sm_kernel<kModeDX><<<grid, kGemmThreads, kGemm2SmemBytes, st>>>(m_dg, m_du, m_wg, m_wu, m_wg,
                                                                                 m_wu, m_dg, m_dg, m_dg, m_dg, ga);
   return check_launch("grouped_gemm_2sm_kernel<dX>");
@@ -1014,16 +1024,16 @@ int launch_train8_forward(const AxmMoeDesc* d, const AxmSegment* segments, int32
   ga.codes_u = static_cast<uint8_t*>(keep->up_codes);
   ga.scales_g = static_cast<uint8_t*>(keep->gate_scales);
   ga.scales_u = static_cast<uint8_t*>(keep->up_scales);
-  grouped_gemm_2sm_kernel<kModeSwiGLU8><<<grid, kGemmThreads, kGemm2SmemBytes, st>>>(a1, a1, g, u, g, u, a1, a1, a1, a1,
-                                                                                     ga);
-  if ((rc = check_launch("grouped_gemm_2sm_kernel<swiglu, 8 bits>"))) return rc;
+  ga.overlap = 1;
+  if ((rc = launch_overlapping("grouped_gemm_2sm_kernel<swiglu, 8 bits>", grouped_gemm_2sm_kernel<kModeSwiGLU8>, grid,
+                               kGemmThreads, kGemm2SmemBytes, st, a1, a1, g, u, g, u, a1, a1, a1, a1, ga)))
+    return rc;
   ga.n_total = D;
   ga.k_total = F;
   ga.out = o;
   ga.out_bf16 = o_bf16 ? 1 : 0;
-  grouped_gemm_2sm_kernel<kModeDown><<<grid, kGemmThreads, kGemm2SmemBytes, st>>>(a2, a2, dn, dn, dn, dn, a2, a2, a2, a2,
-                                                                                  ga);
-  return check_launch("grouped_gemm_2sm_kernel<down>");
+  return launch_overlapping("grouped_gemm_2sm_kernel<down>", grouped_gemm_2sm_kernel<kModeDown>, grid, kGemmThreads,
+                            kGemm2SmemBytes, st, a2, a2, dn, dn, dn, dn, a2, a2, a2, a2, ga);
 }
 
 // Backward of the same: dG, dU and h (bf16, this call's scratch) from the kept codes.
@@ -1064,9 +1074,9 @@ int launch_train8_dh(const AxmMoeDesc* d, const AxmSegment* segments, int32_t nu
   ga.codes_u = static_cast<uint8_t*>(keep->up_codes);
   ga.scales_g = static_cast<uint8_t*>(keep->gate_scales);
   ga.scales_u = static_cast<uint8_t*>(keep->up_scales);
-  grouped_gemm_2sm_kernel<kModeDH8><<<grid, kGemmThreads, kGemm2DhSmemBytes, st>>>(m_do, m_do, m_wd, m_wd, m_wd, m_wd,
-                                                                                   m_h, m_h, m_dg, m_du, ga);
-  return check_launch("grouped_gemm_2sm_kernel<dH, 8 bits>");
+  ga.overlap = 1;
+  return launch_overlapping("grouped_gemm_2sm_kernel<dH, 8 bits>", grouped_gemm_2sm_kernel<kModeDH8>, grid, kGemmThreads,
+                            kGemm2DhSmemBytes, st, m_do, m_do, m_wd, m_wd, m_wd, m_wd, m_h, m_h, m_dg, m_du, ga);
 }
 
 }  // namespace axm

@@ -99,9 +99,8 @@ extern "C" int axm_mx8_expert_ffn_backward(const AxmMoeDesc* desc, const void* x
   }
   int rc;
   if ((rc = launch_train8_dh(desc, segments, num_segments, rows, d_o, w_down, keep, d_g, d_u, h, status, st))) return rc;
-  if ((rc = launch_bwd_dx_2sm(desc, segments, num_segments, rows, d_g, d_u, w_gate, w_up, d_x, status, st, bf16))) return rc;
+  if ((rc = launch_bwd_dx_2sm(desc, segments, num_segments, rows, d_g, d_u, w_gate, w_up, d_x, status, st, bf16, true))) return rc;
   if (!wgrad) return AXM_OK;
-  if ((rc = launch_wgrad_2sm(segments, num_segments, rows, E, h, F, d_o, D, d_w_down, status, st, bf16))) return rc;
-  if ((rc = launch_wgrad_2sm(segments, num_segments, rows, E, x, D, d_g, F, d_w_gate, status, st, bf16))) return rc;
-  return launch_wgrad_2sm(segments, num_segments, rows, E, x, D, d_u, F, d_w_up, status, st, bf16);
+  const WgradProblem all[3] = {{h, F, d_o, D, d_w_down}, {x, D, d_g, F, d_w_gate}, {x, D, d_u, F, d_w_up}};
+  return launch_wgrad_2sm(segments, num_segments, rows, E, all, 3, status, st, bf16, true);
 }
