@@ -73,8 +73,13 @@ struct Gemm2Args {
 
 constexpr int kStagesDh = 5;  // operand stages of kModeDH (one stage's room goes to its epilogue blocks)
 constexpr int kDhSlots = 3;   // 4 KiB slots (g / dG block + u / dU block) per epilogue warp
-constexpr int kDh8Slots = 2;  // kModeDH8: 6 KiB slots (dG, dU and h blocks; nothing comes in through them)
-static_assert(kDh8Slots * 6144 == kDhSlots * 4096, "both forms use the same room");
+// kModeDH8: one 6 KiB slot (dG, dU and h blocks; nothing comes in through it) for each of eight warps
+static_assert(8 * 6144 == 4 * kDhSlots * 4096, "both forms use the same room");
+
+// Epilogue warps of a mode: the 8-bit forms have more to do for a tile than four warps finish under its
+// MMAs, so there two warps share each quarter of the rows, half of the tile's columns each.
+constexpr int epilogue_warps(int mode) { return mode == kModeSwiGLU8 || mode == kModeDH8 ? 8 : 4; }
+constexpr int gemm2_threads(int mode) { return 64 + 32 * epilogue_warps(mode); }
 
 // fp32 accumulate, bf16 A (K-major) and B (MN-major), N = 256, M = 256 over the pair
 constexpr uint32_t kInstrDesc2 = (1u << 4) | (1u << 7) | (1u << 10) | (0u << 15) | (1u << 16) |
@@ -149,7 +154,7 @@ __device__ __forceinline__ uint32_t store_block8(const uint32_t (&v)[32], uint8_
 }
 
 template <int kMode>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm2_threads(kMode), 1)
 grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a_alt,
                         const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1,
                         const __grid_constant__ CUtensorMap tm_b0_sh, const __grid_constant__ CUtensorMap tm_b1_sh,
@@ -208,7 +213,7 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh->tmem_full[i], 1);
-      mbar_init(&sh->tmem_empty[i], 8);
+      mbar_init(&sh->tmem_empty[i], 2 * epilogue_warps(kMode));
     }
     sh->abort_flag = 0;
     fence_barrier_init();
@@ -222,7 +227,7 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
     tmem_relinquish2();
   }
   if (args.overlap) wait_for_previous();
-  for (int s = threadIdx.x; s < nseg; s += kGemmThreads) sh->seg[s] = args.segments[s];
+  for (int s = threadIdx.x; s < nseg; s += gemm2_threads(kMode)) sh->seg[s] = args.segments[s];
   __syncthreads();
   if (threadIdx.x == 0) {
     int acc = 0;
@@ -374,6 +379,10 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
   } else {
     // ---- epilogue: every CTA drains its own 128 accumulator rows -----------------------
     const int quad = warp & 3;
+    // this warp's columns of the tile, in blocks of 32
+    constexpr int kSplit = epilogue_warps(kMode) / 4;
+    const int jb0 = kSplit == 2 ? ((warp - 2) >> 2) * (BN_OUT / 64) : 0;
+    const int jb1 = kSplit == 2 ? jb0 + BN_OUT / 64 : BN_OUT / 32;
     int acc = 0;
     uint32_t acc_phase = 0;
     uint32_t dh_issued = 0, dh_used = 0;  // kModeDH: blocks of g / u requested (lane 0) and consumed
@@ -417,8 +426,8 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
       if constexpr (kRead8) {
         // The same derivative from g and u in 8 bits.  A lane reads its own row: 32 codes of each
         // (two 16-byte pieces, a whole sector) and a scale byte a block, one block ahead of their
-        // use.  dG, dU and h leave as in the bf16 form, through two slots of three blocks.
-        unsigned char* slots = staging + (size_t)((warp - 2) & 3) * kDh8Slots * 6144;
+        // use.  dG, dU and h leave as in the bf16 form, through the warp's slot of three blocks.
+        unsigned char* dg_s = staging + (size_t)(warp - 2) * 6144;
         auto piece_smem = [&](int row, int piece) { return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); };
         const bool mine = lane < dh_rows_left;
         const size_t row_at = (size_t)(dh_row0 + (mine ? lane : 0));
@@ -435,11 +444,10 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
           gs = __ldg(args.scales_g + sc);
           us = __ldg(args.scales_u + sc);
         };
-        fetch(0);
+        fetch(jb0);
 #pragma unroll 1
-        for (int jb = 0; jb < BN_OUT / 32; ++jb) {
+        for (int jb = jb0; jb < jb1; ++jb) {
           if (!dh_valid(jb)) break;
-          unsigned char* dg_s = slots + (size_t)(dh_used % kDh8Slots) * 6144;
           const int c0 = jb * 32;
           uint32_t v[32];
           __syncwarp();
@@ -447,9 +455,9 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
           const uint32_t gw[8] = {gc[0].x, gc[0].y, gc[0].z, gc[0].w, gc[1].x, gc[1].y, gc[1].z, gc[1].w};
           const uint32_t uw[8] = {uc8[0].x, uc8[0].y, uc8[0].z, uc8[0].w, uc8[1].x, uc8[1].y, uc8[1].z, uc8[1].w};
           const float g_scale = mx_scale_value(gs), u_scale = mx_scale_value(us);
-          fetch(jb + 1);
+          if (jb + 1 < jb1) fetch(jb + 1);
           tmem_ld_wait();
-          if (dh_full && lane == 0) bulk_wait_read_but_one();  // this slot's stores, a block before the last ones
+          if (dh_full && lane == 0) bulk_wait_read();  // the last block's stores have read the slot
           __syncwarp();
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
@@ -498,7 +506,6 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
               tma_store_2d(&tm_g, dg_s + 4096, n0 + c0, dh_row0);  // the map of h
               bulk_commit_group();
             }
-            ++dh_used;
           }
         }
       } else if constexpr (kDH) {
@@ -593,7 +600,7 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
         }
       } else if (uc.live) {
 #pragma unroll 1
-        for (int c0 = 0; c0 < BN_OUT; c0 += 32) {
+        for (int c0 = 32 * jb0; c0 < 32 * jb1; c0 += 32) {
           uint32_t g[32];
           __syncwarp();
           tmem_ld32(t_addr + c0, g);
@@ -1026,7 +1033,7 @@ int launch_train8_forward(const AxmMoeDesc* d, const AxmSegment* segments, int32
   ga.scales_u = static_cast<uint8_t*>(keep->up_scales);
   ga.overlap = 1;
   if ((rc = launch_overlapping("grouped_gemm_2sm_kernel<swiglu, 8 bits>", grouped_gemm_2sm_kernel<kModeSwiGLU8>, grid,
-                               kGemmThreads, kGemm2SmemBytes, st, a1, a1, g, u, g, u, a1, a1, a1, a1, ga)))
+                               gemm2_threads(kModeSwiGLU8), kGemm2SmemBytes, st, a1, a1, g, u, g, u, a1, a1, a1, a1, ga)))
     return rc;
   ga.n_total = D;
   ga.k_total = F;
@@ -1075,7 +1082,7 @@ int launch_train8_dh(const AxmMoeDesc* d, const AxmSegment* segments, int32_t nu
   ga.scales_g = static_cast<uint8_t*>(keep->gate_scales);
   ga.scales_u = static_cast<uint8_t*>(keep->up_scales);
   ga.overlap = 1;
-  return launch_overlapping("grouped_gemm_2sm_kernel<dH, 8 bits>", grouped_gemm_2sm_kernel<kModeDH8>, grid, kGemmThreads,
+  return launch_overlapping("grouped_gemm_2sm_kernel<dH, 8 bits>", grouped_gemm_2sm_kernel<kModeDH8>, grid, gemm2_threads(kModeDH8),
                             kGemm2DhSmemBytes, st, m_do, m_do, m_wd, m_wd, m_wd, m_wd, m_h, m_h, m_dg, m_du, ga);
 }
 
