@@ -63,7 +63,12 @@ enum {
    * down projection multiplies both by the same weights, so every output meets that
    * bound; the down projection then does twice the tensor-core work and h takes twice
    * the room (workspace sizes follow the flag).  Inference entry points only. */
-  AXM_FLAG_H_EXACT = 4
+  AXM_FLAG_H_EXACT = 4,
+  /* Training step on one GPU: what the backward pass needs of the forward pass is kept in 8 bits
+   * (the gate's and the up projection's outputs and the expert rows; the format of axm_mx8_*), the
+   * rest is rebuilt: 2 F + D bytes a row and 3 % where the plain form keeps 6 F + 6 D.  Gradients are
+   * those of the kept values.  d_model and d_ff must be multiples of 32. */
+  AXM_FLAG_SAVE_8BIT = 8
 };
 
 /* Problem shape.  D and F must be multiples of 8 (16-byte rows); E <= 256;
@@ -327,6 +332,15 @@ AXM_API int axm_moe_forward_train(const AxmMoeDesc* desc, const AxmMoeTrain* ten
                                   void* workspace, size_t workspace_bytes, void* stream);
 AXM_API int axm_moe_backward(const AxmMoeDesc* desc, const AxmMoeTrain* tensors, void* workspace,
                              size_t workspace_bytes, void* stream);
+
+/* The same two calls with the workspace in two pieces: `kept` holds what the backward pass needs of the
+ * forward pass, `scratch` nothing between calls.  A model of many layers has a `kept` for each and one
+ * `scratch` (of the largest) for all that run one after the other on a stream.  Both 256-byte aligned. */
+AXM_API int axm_moe_train_split_bytes(const AxmMoeDesc* desc, size_t* kept_bytes, size_t* scratch_bytes);
+AXM_API int axm_moe_forward_train_split(const AxmMoeDesc* desc, const AxmMoeTrain* tensors, void* kept,
+                                        size_t kept_bytes, void* scratch, size_t scratch_bytes, void* stream);
+AXM_API int axm_moe_backward_split(const AxmMoeDesc* desc, const AxmMoeTrain* tensors, void* kept,
+                                   size_t kept_bytes, void* scratch, size_t scratch_bytes, void* stream);
 
 /* AdamW step (decoupled weight decay, bias correction with `step` >= 1) over one MoE
  * weight matrix as the engine stores it: fp32 master, two fp32 moments, bf16 working

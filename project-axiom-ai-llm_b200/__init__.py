@@ -28,6 +28,7 @@ ROUTER_FP32 = 1
 FLAG_RESIDUAL = 1
 FLAG_HIST_ACCUMULATE = 2
 FLAG_H_EXACT = 4
+FLAG_SAVE_8BIT = 8
 ROUTE_BLOCKS = 296
 SEG_ALT_A = 1 << 30
 DTYPE_BF16 = 0
@@ -136,6 +137,10 @@ def load():
     lib.axm_moe_train_workspace_bytes.argtypes = [dp, ctypes.POINTER(sz)]
     lib.axm_moe_forward_train.argtypes = [dp, tp, vp, sz, vp]
     lib.axm_moe_backward.argtypes = [dp, tp, vp, sz, vp]
+    szq = ctypes.POINTER(sz)
+    lib.axm_moe_train_split_bytes.argtypes = [dp, szq, szq]
+    lib.axm_moe_forward_train_split.argtypes = [dp, tp, vp, sz, vp, sz, vp]
+    lib.axm_moe_backward_split.argtypes = [dp, tp, vp, sz, vp, sz, vp]
     lib.axm_moe_permute_padded.argtypes = [dp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp]
     lib.axm_moe_adamw_step.argtypes = [vp, vp, vp, vp, vp, ctypes.c_int64] + [ctypes.c_float] * 5 + [i32, vp]
     lib.axm_moe_adamw_step_engine.argtypes = ([vp] * 5 + [ctypes.c_int64, ctypes.c_int64] +
@@ -226,6 +231,13 @@ def workspace_bytes(desc):
     n = ctypes.c_size_t(0)
     check(load().axm_moe_workspace_bytes(ctypes.byref(desc), ctypes.byref(n)))
     return n.value
+
+
+def train_split_bytes(desc):
+    """Bytes of the training step's workspace: (kept from forward to backward, scratch)."""
+    a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    check(load().axm_moe_train_split_bytes(ctypes.byref(desc), ctypes.byref(a), ctypes.byref(b)))
+    return a.value, b.value
 
 
 class MoeLayer:
@@ -345,9 +357,14 @@ class MoeLayer:
 
 class MoeTrainLayer:
     """Forward + backward of one MoE layer (training step).  step(x, d_out) returns
-    (out, aux_loss, grads) with grads = dict(d_x, d_router_w, d_w_gate, d_w_up, d_w_down)."""
+    (out, aux_loss, grads) with grads = dict(d_x, d_router_w, d_w_gate, d_w_up, d_w_down).
 
-    def __init__(self, weights, tokens, top_k, aux_alpha=0.01, device="cuda", weight_grads=True):
+    save_8bit keeps what the backward pass needs in 8 bits (AXM_FLAG_SAVE_8BIT).  With `scratch` (a
+    byte tensor of at least train_split_bytes(desc)[1]) the layer's own workspace holds only what lives
+    from forward to backward; layers that run one after the other on a stream can share one scratch."""
+
+    def __init__(self, weights, tokens, top_k, aux_alpha=0.01, device="cuda", weight_grads=True, save_8bit=False,
+                 scratch=None):
         self.lib = load()
         self.w = weights
         wr = weights["router_w"]
@@ -355,11 +372,13 @@ class MoeTrainLayer:
         F = weights["w_gate"].shape[2]
         rdt = ROUTER_FP32 if wr.dtype == torch.float32 else ROUTER_BF16
         S = self.S = 0 if weights.get("shared_gate") is None else weights["shared_gate"].shape[0]
-        self.desc = make_desc(tokens, D, F, E, top_k, S, rdt, FLAG_RESIDUAL)
+        self.desc = make_desc(tokens, D, F, E, top_k, S, rdt, FLAG_RESIDUAL | (FLAG_SAVE_8BIT if save_8bit else 0))
         dev = torch.device(device)
-        n = ctypes.c_size_t(0)
-        check(self.lib.axm_moe_train_workspace_bytes(ctypes.byref(self.desc), ctypes.byref(n)))
-        self.workspace = torch.empty(n.value, dtype=torch.uint8, device=dev)
+        kept, shared = train_split_bytes(self.desc)
+        if scratch is not None and scratch.numel() < shared:
+            raise ValueError(f"scratch has {scratch.numel()} bytes, {shared} are needed")
+        self.scratch = scratch
+        self.workspace = torch.empty(kept + shared if scratch is None else kept, dtype=torch.uint8, device=dev)
         f32 = torch.float32
         self.out = torch.empty(tokens, D, dtype=torch.bfloat16, device=dev)
         self.aux = torch.zeros(1, dtype=f32, device=dev)
@@ -399,15 +418,25 @@ class MoeTrainLayer:
 
     def forward(self, x):
         t = self.tensors(x, None)
-        check(self.lib.axm_moe_forward_train(ctypes.byref(self.desc), ctypes.byref(t),
-                                             ptr(self.workspace), self.workspace.numel(),
-                                             current_stream()))
+        if self.scratch is None:
+            check(self.lib.axm_moe_forward_train(ctypes.byref(self.desc), ctypes.byref(t),
+                                                 ptr(self.workspace), self.workspace.numel(),
+                                                 current_stream()))
+        else:
+            check(self.lib.axm_moe_forward_train_split(ctypes.byref(self.desc), ctypes.byref(t), ptr(self.workspace),
+                                                       self.workspace.numel(), ptr(self.scratch),
+                                                       self.scratch.numel(), current_stream()))
         return self.out
 
     def backward(self, x, d_out):
         t = self.tensors(x, d_out)
-        check(self.lib.axm_moe_backward(ctypes.byref(self.desc), ctypes.byref(t), ptr(self.workspace),
-                                        self.workspace.numel(), current_stream()))
+        if self.scratch is None:
+            check(self.lib.axm_moe_backward(ctypes.byref(self.desc), ctypes.byref(t), ptr(self.workspace),
+                                            self.workspace.numel(), current_stream()))
+        else:
+            check(self.lib.axm_moe_backward_split(ctypes.byref(self.desc), ctypes.byref(t), ptr(self.workspace),
+                                                  self.workspace.numel(), ptr(self.scratch), self.scratch.numel(),
+                                                  current_stream()))
         return self.d_x
 
     def step(self, x, d_out):

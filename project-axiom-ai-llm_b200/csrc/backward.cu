@@ -13,6 +13,8 @@
 //
 //   L = sum(dOut * out) + aux,  out = x + y,  aux = alpha * E * sum_e f_e * P_e,
 //   f_e = count_e / (T k) (constant), P_e = mean_t p[t, e].
+#include "gemm_common.cuh"
+#include "microscale.cuh"
 #include "router.cuh"
 
 namespace axm {
@@ -555,6 +557,21 @@ int launch_bwd_prepare_shared(const float* d_out, void* d_o, int T, int Tp, int 
   return check_launch("bwd_prepare_shared_kernel");
 }
 
+// The permuted activations again, from what the forward pass left of the permutation: row r of x_perm is
+// x[row_src[r] / k], rows that pad an expert to the alignment (row_src -1) are zero.
+__global__ void __launch_bounds__(256)
+train_gather_rows_kernel(const __nv_bfloat16* __restrict__ x, const int32_t* __restrict__ row_src,
+                         const int32_t* __restrict__ offsets, int E, int k, int D, __nv_bfloat16* __restrict__ x_perm) {
+  const int rows = offsets[E], chunks = D / 8;
+  const int warps = gridDim.x * (blockDim.x >> 5), lane = threadIdx.x & 31;
+  for (int r = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); r < rows; r += warps) {
+    const int s = __ldg(row_src + r);
+    const uint4* from = reinterpret_cast<const uint4*>(x + (size_t)(s < 0 ? 0 : s / k) * D);
+    uint4* to = reinterpret_cast<uint4*>(x_perm + (size_t)r * D);
+    for (int c = lane; c < chunks; c += 32) to[c] = s < 0 ? make_uint4(0u, 0u, 0u, 0u) : __ldg(from + c);
+  }
+}
+
 struct TrainWs {
   int32_t* status;
   float* logits;
@@ -572,22 +589,29 @@ struct TrainWs {
   float* dz;
   float* dwr_partial;
   void *x_perm, *g, *u, *h, *o, *d_o, *d_g, *d_u, *d_xp;
+  AxmMx8Checkpoint keep;         // AXM_FLAG_SAVE_8BIT: g and u,
+  void *o_codes, *o_scales;      //   and the routed experts' rows
   void* router_scratch;
   size_t router_scratch_bytes;
   int rows_max;     // rows of every row buffer: routed rows (padded) + shared experts' rows
   int shared_row0;  // first row of shared expert 0 (a fixed place behind the routed rows)
   int shared_rows;  // rows per shared expert: the tokens padded to a multiple of 64
-  size_t bytes;
+  size_t kept_bytes, scratch_bytes;
 };
 
-static TrainWs carve_train(const AxmMoeDesc* d, void* base) {
-  TrainWs w;
-  size_t off = 0;
-  auto take = [&](size_t n) {
+// `kept` and `scratch`: the two pieces of the workspace (null: only measures).  `save` takes from the
+// first what the backward pass needs of the forward pass, `take` from the second.
+static TrainWs carve_train(const AxmMoeDesc* d, void* kept, void* scratch) {
+  TrainWs w = {};
+  size_t kept_off = 0, scratch_off = 0;
+  auto from = [](void* base, size_t& off, size_t n) {
     void* p = base ? static_cast<char*>(base) + off : nullptr;
     off += (n + 255) & ~static_cast<size_t>(255);
     return p;
   };
+  auto save = [&](size_t n) { return from(kept, kept_off, n); };
+  auto take = [&](size_t n) { return from(scratch, scratch_off, n); };
+  const bool in8 = (d->flags & AXM_FLAG_SAVE_8BIT) != 0;
   const size_t T = d->tokens, D = d->d_model, F = d->d_ff, E = d->num_experts, k = d->top_k, S = d->num_shared;
   const size_t R0 = (T * k + (kTrainAlign - 1) * E + kTrainAlign - 1) / kTrainAlign * kTrainAlign;
   const size_t Tp = (T + kTrainAlign - 1) / kTrainAlign * kTrainAlign;
@@ -595,26 +619,38 @@ static TrainWs carve_train(const AxmMoeDesc* d, void* base) {
   w.rows_max = (int)R;
   w.shared_row0 = (int)R0;
   w.shared_rows = (int)Tp;
-  w.status = static_cast<int32_t*>(take(4));
-  w.logits = static_cast<float*>(take(4 * T * E));
-  w.topk_idx = static_cast<int32_t*>(take(4 * T * k));
-  w.topk_gate = static_cast<float*>(take(4 * T * k));
+  w.status = static_cast<int32_t*>(save(4));
+  w.logits = static_cast<float*>(save(4 * T * E));
+  w.topk_idx = static_cast<int32_t*>(save(4 * T * k));
+  w.topk_gate = static_cast<float*>(save(4 * T * k));
   w.block_counts = static_cast<int32_t*>(take(4 * AXM_ROUTE_BLOCKS * E));
-  w.counts = static_cast<int32_t*>(take(4 * E));
-  w.offsets = static_cast<int32_t*>(take(4 * (E + 1)));
-  w.row_src = static_cast<int32_t*>(take(4 * R0));
-  w.slot_dst = static_cast<int32_t*>(take(4 * T * k));
-  w.segments = static_cast<AxmSegment*>(take(sizeof(AxmSegment) * (E + S)));
+  w.counts = static_cast<int32_t*>(save(4 * E));
+  w.offsets = static_cast<int32_t*>(save(4 * (E + 1)));
+  w.row_src = static_cast<int32_t*>(save(4 * R0));
+  w.slot_dst = static_cast<int32_t*>(save(4 * T * k));
+  w.segments = static_cast<AxmSegment*>(save(sizeof(AxmSegment) * (E + S)));
   w.aux_partial = static_cast<float*>(take(4 * AXM_ROUTE_BLOCKS * E));
-  w.aux_coef = static_cast<float*>(take(4 * E));
+  w.aux_coef = static_cast<float*>(save(4 * E));
   w.d_gate = static_cast<float*>(take(4 * T * k));
   w.dz = static_cast<float*>(take(4 * T * E));
   w.dwr_partial = static_cast<float*>(take(4 * (size_t)kDwrChunks * D * E));
-  w.x_perm = take(2 * R * D);
-  w.g = take(2 * R * F);
-  w.u = take(2 * R * F);
-  w.h = take(2 * R * F);
-  w.o = take(4 * R * D);
+  if (in8) {
+    w.keep.gate_codes = save(R * F);
+    w.keep.up_codes = save(R * F);
+    w.keep.gate_scales = save(R * (F / kMxBlock));
+    w.keep.up_scales = save(R * (F / kMxBlock));
+    w.o_codes = save(R0 * D);
+    w.o_scales = save(R0 * (D / kMxBlock));
+    w.x_perm = take(2 * R * D);
+    w.h = take(2 * R * F);
+    w.o = take(4 * R * D);
+  } else {
+    w.x_perm = save(2 * R * D);
+    w.g = save(2 * R * F);
+    w.u = save(2 * R * F);
+    w.h = save(2 * R * F);
+    w.o = save(4 * R * D);
+  }
   w.d_o = take(2 * R * D);
   w.d_g = take(2 * R * F);
   w.d_u = take(2 * R * F);
@@ -622,7 +658,8 @@ static TrainWs carve_train(const AxmMoeDesc* d, void* base) {
   w.router_scratch_bytes = 0;
   axm_moe_router_scratch_bytes(d, &w.router_scratch_bytes);
   w.router_scratch = take(w.router_scratch_bytes);
-  w.bytes = off;
+  w.kept_bytes = kept_off;
+  w.scratch_bytes = scratch_off;
   return w;
 }
 
@@ -636,6 +673,8 @@ static int validate_train(const AxmMoeDesc* d) {
   if (d->top_k <= 0 || d->top_k > 8 || d->top_k > d->num_experts)
     return fail(AXM_ERR_ARGUMENT, "top_k %d not in 1..min(num_experts, 8)", d->top_k);
   if (d->num_shared < 0 || d->num_shared > 8) return fail(AXM_ERR_ARGUMENT, "num_shared %d not in 0..8", d->num_shared);
+  if ((d->flags & AXM_FLAG_SAVE_8BIT) && (d->d_model % kMxBlock || d->d_ff % kMxBlock))
+    return fail(AXM_ERR_ARGUMENT, "AXM_FLAG_SAVE_8BIT: d_model %d and d_ff %d must be multiples of 32", d->d_model, d->d_ff);
   if (d->router_dtype != AXM_ROUTER_BF16 && d->router_dtype != AXM_ROUTER_FP32)
     return fail(AXM_ERR_ARGUMENT, "router_dtype %d unknown", d->router_dtype);
   if ((long long)d->tokens * d->top_k + 64LL * d->num_experts + ((long long)d->tokens + 64) * d->num_shared > 0x7fffffffLL)
@@ -643,13 +682,33 @@ static int validate_train(const AxmMoeDesc* d) {
   return AXM_OK;
 }
 
+static int check_pieces(const AxmMoeDesc* d, void* kept, size_t kept_bytes, void* scratch, size_t scratch_bytes,
+                        TrainWs* out) {
+  if (kept == nullptr || scratch == nullptr ||
+      ((reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(scratch)) & 255) != 0)
+    return fail(AXM_ERR_WORKSPACE, "workspace is null or not 256-byte aligned");
+  *out = carve_train(d, kept, scratch);
+  if (kept_bytes < out->kept_bytes || scratch_bytes < out->scratch_bytes)
+    return fail(AXM_ERR_WORKSPACE, "workspace has %zu + %zu bytes, %zu + %zu needed", kept_bytes, scratch_bytes,
+                out->kept_bytes, out->scratch_bytes);
+  return AXM_OK;
+}
+
+// One workspace: what is kept first, the scratch behind it.
 static int check_ws(const AxmMoeDesc* d, void* ws, size_t bytes, TrainWs* out) {
   if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) != 0)
     return fail(AXM_ERR_WORKSPACE, "workspace is null or not 256-byte aligned");
-  *out = carve_train(d, ws);
-  if (bytes < out->bytes) return fail(AXM_ERR_WORKSPACE, "workspace has %zu bytes, %zu needed", bytes, out->bytes);
+  const TrainWs size = carve_train(d, nullptr, nullptr);
+  const size_t need = size.kept_bytes + size.scratch_bytes;
+  if (bytes < need) return fail(AXM_ERR_WORKSPACE, "workspace has %zu bytes, %zu needed", bytes, need);
+  *out = carve_train(d, ws, static_cast<char*>(ws) + size.kept_bytes);
   return AXM_OK;
 }
+
+static int forward_train(const AxmMoeDesc* desc, const AxmMoeTrain* t, const TrainWs& w, void* stream);
+static int backward(const AxmMoeDesc* desc, const AxmMoeTrain* t, const TrainWs& w, void* stream);
+static int check_forward_train(const AxmMoeDesc* desc, const AxmMoeTrain* t);
+static int check_backward(const AxmMoeDesc* desc, const AxmMoeTrain* t);
 
 }  // namespace axm
 
@@ -658,19 +717,61 @@ using namespace axm;
 extern "C" int axm_moe_train_workspace_bytes(const AxmMoeDesc* desc, size_t* bytes) {
   if (int rc = validate_train(desc)) return rc;
   if (bytes == nullptr) return fail(AXM_ERR_ARGUMENT, "bytes is null");
-  *bytes = carve_train(desc, nullptr).bytes;
+  const TrainWs w = carve_train(desc, nullptr, nullptr);
+  *bytes = w.kept_bytes + w.scratch_bytes;
+  return AXM_OK;
+}
+
+extern "C" int axm_moe_train_split_bytes(const AxmMoeDesc* desc, size_t* kept_bytes, size_t* scratch_bytes) {
+  if (int rc = validate_train(desc)) return rc;
+  if (kept_bytes == nullptr || scratch_bytes == nullptr) return fail(AXM_ERR_ARGUMENT, "bytes is null");
+  const TrainWs w = carve_train(desc, nullptr, nullptr);
+  *kept_bytes = w.kept_bytes;
+  *scratch_bytes = w.scratch_bytes;
   return AXM_OK;
 }
 
 extern "C" int axm_moe_forward_train(const AxmMoeDesc* desc, const AxmMoeTrain* t, void* workspace,
                                      size_t workspace_bytes, void* stream) {
+  if (int rc = check_forward_train(desc, t)) return rc;
+  TrainWs w;
+  if (int rc = check_ws(desc, workspace, workspace_bytes, &w)) return rc;
+  return forward_train(desc, t, w, stream);
+}
+extern "C" int axm_moe_forward_train_split(const AxmMoeDesc* desc, const AxmMoeTrain* t, void* kept, size_t kept_bytes,
+                                           void* scratch, size_t scratch_bytes, void* stream) {
+  if (int rc = check_forward_train(desc, t)) return rc;
+  TrainWs w;
+  if (int rc = check_pieces(desc, kept, kept_bytes, scratch, scratch_bytes, &w)) return rc;
+  return forward_train(desc, t, w, stream);
+}
+extern "C" int axm_moe_backward(const AxmMoeDesc* desc, const AxmMoeTrain* t, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  if (int rc = check_backward(desc, t)) return rc;
+  TrainWs w;
+  if (int rc = check_ws(desc, workspace, workspace_bytes, &w)) return rc;
+  return backward(desc, t, w, stream);
+}
+extern "C" int axm_moe_backward_split(const AxmMoeDesc* desc, const AxmMoeTrain* t, void* kept, size_t kept_bytes,
+                                      void* scratch, size_t scratch_bytes, void* stream) {
+  if (int rc = check_backward(desc, t)) return rc;
+  TrainWs w;
+  if (int rc = check_pieces(desc, kept, kept_bytes, scratch, scratch_bytes, &w)) return rc;
+  return backward(desc, t, w, stream);
+}
+
+namespace axm {
+
+static int check_forward_train(const AxmMoeDesc* desc, const AxmMoeTrain* t) {
   if (int rc = validate_train(desc)) return rc;
   if (!t || !t->x || !t->router_w || !t->w_gate || !t->w_up || !t->w_down || !t->out)
     return fail(AXM_ERR_ARGUMENT, "axm_moe_forward_train: x, router_w, w_gate, w_up, w_down, out are required");
   if (desc->num_shared > 0 && (!t->shared_gate || !t->shared_up || !t->shared_down))
     return fail(AXM_ERR_ARGUMENT, "num_shared > 0 needs shared_gate, shared_up and shared_down");
-  TrainWs w;
-  if (int rc = check_ws(desc, workspace, workspace_bytes, &w)) return rc;
+  return AXM_OK;
+}
+
+static int forward_train(const AxmMoeDesc* desc, const AxmMoeTrain* t, const TrainWs& w, void* stream) {
   if (int rc = require_device()) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int T = desc->tokens, E = desc->num_experts, k = desc->top_k, S = desc->num_shared;
@@ -687,10 +788,13 @@ extern "C" int axm_moe_forward_train(const AxmMoeDesc* desc, const AxmMoeTrain* 
                            w.slot_dst, w.x_perm, w.segments, router_cleared_status ? nullptr : w.status, st,
                            kTrainAlign)))
     return rc;
-  if ((rc = launch_expert_ffn(&d, w.x_perm, w.rows_max, nullptr, 0, w.segments, E, t->w_gate, t->w_up,
-                              t->w_down, nullptr, nullptr, nullptr, w.h, w.o, w.rows_max, w.status, st,
-                              nullptr, nullptr, w.g, w.u)))
-    return rc;
+  const bool in8 = (desc->flags & AXM_FLAG_SAVE_8BIT) != 0;
+  rc = in8 ? launch_train8_forward(&d, w.segments, E, w.rows_max, w.x_perm, t->w_gate, t->w_up, t->w_down, &w.keep, w.h,
+                                   w.o, false, w.status, st)
+           : launch_expert_ffn(&d, w.x_perm, w.rows_max, nullptr, 0, w.segments, E, t->w_gate, t->w_up,
+                               t->w_down, nullptr, nullptr, nullptr, w.h, w.o, w.rows_max, w.status, st,
+                               nullptr, nullptr, w.g, w.u);
+  if (rc) return rc;
   if (S > 0) {
     train_shared_rows_kernel<<<2 * sm_count(), 256, 0, st>>>(static_cast<const __nv_bfloat16*>(t->x),
                                                              static_cast<__nv_bfloat16*>(w.x_perm), w.segments, T,
@@ -698,11 +802,17 @@ extern "C" int axm_moe_forward_train(const AxmMoeDesc* desc, const AxmMoeTrain* 
     AxmMoeDesc ds = d;
     ds.num_experts = S;
     ds.top_k = 1;
-    if ((rc = launch_expert_ffn(&ds, w.x_perm, w.rows_max, nullptr, 0, w.segments + E, S, t->shared_gate,
-                                t->shared_up, t->shared_down, nullptr, nullptr, nullptr, w.h, w.o, w.rows_max,
-                                w.status, st, nullptr, nullptr, w.g, w.u)))
-      return rc;
+    rc = in8 ? launch_train8_forward(&ds, w.segments + E, S, w.rows_max, w.x_perm, t->shared_gate, t->shared_up,
+                                     t->shared_down, &w.keep, w.h, w.o, false, w.status, st)
+             : launch_expert_ffn(&ds, w.x_perm, w.rows_max, nullptr, 0, w.segments + E, S, t->shared_gate,
+                                 t->shared_up, t->shared_down, nullptr, nullptr, nullptr, w.h, w.o, w.rows_max,
+                                 w.status, st, nullptr, nullptr, w.g, w.u);
+    if (rc) return rc;
   }
+  // the routed experts' rows: the gates' gradients multiply them
+  if (in8 && (rc = axm_mx8_quantize_rows(w.o, AXM_DTYPE_FP32, desc->d_model, w.shared_row0, desc->d_model, w.o_codes,
+                                         w.o_scales, stream)))
+    return rc;
   AxmMoeDesc dc = *desc;
   dc.flags &= ~(AXM_FLAG_HIST_ACCUMULATE | AXM_FLAG_H_EXACT);
   const float* o_shared = S > 0 ? static_cast<const float*>(w.o) + (size_t)w.shared_row0 * desc->d_model : nullptr;
@@ -718,8 +828,7 @@ extern "C" int axm_moe_forward_train(const AxmMoeDesc* desc, const AxmMoeTrain* 
   return check_launch("forward_train");
 }
 
-extern "C" int axm_moe_backward(const AxmMoeDesc* desc, const AxmMoeTrain* t, void* workspace,
-                                size_t workspace_bytes, void* stream) {
+static int check_backward(const AxmMoeDesc* desc, const AxmMoeTrain* t) {
   if (int rc = validate_train(desc)) return rc;
   if (!t || !t->x || !t->router_w || !t->w_gate || !t->w_up || !t->w_down || !t->d_out || !t->d_x)
     return fail(AXM_ERR_ARGUMENT, "axm_moe_backward: x, weights, d_out and d_x are required");
@@ -733,25 +842,40 @@ extern "C" int axm_moe_backward(const AxmMoeDesc* desc, const AxmMoeTrain* t, vo
     if (routed != shared_any || shared_any != shared_all)
       return fail(AXM_ERR_ARGUMENT, "shared experts' weight gradients: all three exactly when the routed experts' are given");
   }
-  TrainWs w;
-  if (int rc = check_ws(desc, workspace, workspace_bytes, &w)) return rc;
+  return AXM_OK;
+}
+
+static int backward(const AxmMoeDesc* desc, const AxmMoeTrain* t, const TrainWs& w, void* stream) {
   if (int rc = require_device()) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int D = desc->d_model, E = desc->num_experts, k = desc->top_k;
+  const int D = desc->d_model, E = desc->num_experts, k = desc->top_k, S = desc->num_shared;
+  const bool in8 = (desc->flags & AXM_FLAG_SAVE_8BIT) != 0;
 
   // Shared-memory limits of the two router-gradient kernels are settled before anything is
   // launched, so that a refusal leaves no half-finished backward pass behind.
   int rc;
   if ((rc = bwd_source_limits(E, desc->router_dtype))) return rc;
+  if (in8) {  // what was not kept: the permuted activations, and the experts' rows in fp32
+    train_gather_rows_kernel<<<4 * sm_count(), 256, 0, st>>>(static_cast<const __nv_bfloat16*>(t->x), w.row_src, w.offsets,
+                                                             E, k, D, static_cast<__nv_bfloat16*>(w.x_perm));
+    if ((rc = check_launch("train_gather_rows_kernel"))) return rc;
+    if (S > 0 && (rc = launch_train_shared_rows(t->x, w.x_perm, w.segments, desc->tokens, w.shared_rows, D, E, S,
+                                                w.shared_row0, st)))
+      return rc;
+    if ((rc = axm_mx8_dequantize_rows(w.o_codes, w.o_scales, w.shared_row0, D, w.o, AXM_DTYPE_FP32, D, stream))) return rc;
+  }
   if ((rc = launch_bwd_prepare(t->d_out, static_cast<const float*>(w.o), w.row_src, w.topk_gate, w.offsets, w.d_o,
                                w.d_gate, D, E, k, st)))
     return rc;
   AxmMoeDesc dr = *desc;
   dr.num_shared = 0;  // the routed experts; the shared ones follow as experts of their own
-  if ((rc = axm_moe_expert_ffn_backward(&dr, w.segments, E, w.rows_max, w.x_perm, w.h, w.g, w.u, w.d_o,
-                                        t->w_gate, t->w_up, t->w_down, w.d_g, w.d_u, w.d_xp,
-                                        t->d_w_gate, t->d_w_up, t->d_w_down, w.status, stream)))
-    return rc;
+  rc = in8 ? axm_mx8_expert_ffn_backward(&dr, w.x_perm, w.rows_max, w.segments, E, &w.keep, w.d_o, t->w_gate, t->w_up,
+                                         t->w_down, w.h, w.d_g, w.d_u, w.d_xp, t->d_w_gate, t->d_w_up, t->d_w_down,
+                                         AXM_DTYPE_FP32, w.status, stream)
+           : axm_moe_expert_ffn_backward(&dr, w.segments, E, w.rows_max, w.x_perm, w.h, w.g, w.u, w.d_o,
+                                         t->w_gate, t->w_up, t->w_down, w.d_g, w.d_u, w.d_xp,
+                                         t->d_w_gate, t->d_w_up, t->d_w_down, w.status, stream);
+  if (rc) return rc;
   if (S > 0) {
     bwd_prepare_shared_kernel<<<2 * sm_count(), 256, 0, st>>>(t->d_out, static_cast<__nv_bfloat16*>(w.d_o),
                                                               desc->tokens, w.shared_rows, D, S, w.shared_row0);
@@ -759,15 +883,20 @@ extern "C" int axm_moe_backward(const AxmMoeDesc* desc, const AxmMoeTrain* t, vo
     ds.num_experts = S;
     ds.num_shared = 0;
     ds.top_k = 1;
-    if ((rc = axm_moe_expert_ffn_backward(&ds, w.segments + E, S, w.rows_max, w.x_perm, w.h, w.g, w.u, w.d_o,
-                                          t->shared_gate, t->shared_up, t->shared_down, w.d_g, w.d_u, w.d_xp,
-                                          t->d_shared_gate, t->d_shared_up, t->d_shared_down, w.status, stream)))
-      return rc;
+    rc = in8 ? axm_mx8_expert_ffn_backward(&ds, w.x_perm, w.rows_max, w.segments + E, S, &w.keep, w.d_o, t->shared_gate,
+                                           t->shared_up, t->shared_down, w.h, w.d_g, w.d_u, w.d_xp, t->d_shared_gate,
+                                           t->d_shared_up, t->d_shared_down, AXM_DTYPE_FP32, w.status, stream)
+             : axm_moe_expert_ffn_backward(&ds, w.segments + E, S, w.rows_max, w.x_perm, w.h, w.g, w.u, w.d_o,
+                                           t->shared_gate, t->shared_up, t->shared_down, w.d_g, w.d_u, w.d_xp,
+                                           t->d_shared_gate, t->d_shared_up, t->d_shared_down, w.status, stream);
+    if (rc) return rc;
   }
   return launch_bwd_source_tail(desc, t, w.logits, w.topk_idx, w.d_gate, w.aux_coef, w.dz, w.aux_partial,
                                 w.dwr_partial, static_cast<const float*>(w.d_xp), w.slot_dst, st, S,
                                 static_cast<const float*>(w.d_xp) + (size_t)w.shared_row0 * D, w.shared_rows);
 }
+
+}  // namespace axm
 
 // ---- optimizer step for the MoE weights ---------------------------------------------
 // AdamW with decoupled weight decay over an fp32 master copy, two fp32 moments and the

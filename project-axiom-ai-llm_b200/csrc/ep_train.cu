@@ -171,6 +171,8 @@ EpTrainWs carve(const AxmEpLayout* l, const AxmMoeDesc* d, void* base) {
 
 int validate_ep_train(const AxmEpLayout* l, const AxmMoeDesc* d, int32_t tokens_global) {
   if (int rc = validate_ep_layer(l, d)) return rc;
+  if (d->flags & AXM_FLAG_SAVE_8BIT)
+    return fail(AXM_ERR_ARGUMENT, "AXM_FLAG_SAVE_8BIT: the sharded training step keeps bf16 activations");
   if (d->tokens <= 0) return fail(AXM_ERR_ARGUMENT, "tokens %d must be positive", d->tokens);
   if (tokens_global < d->tokens)
     return fail(AXM_ERR_ARGUMENT, "tokens_global %d is smaller than this rank's %d tokens", tokens_global, d->tokens);

@@ -230,3 +230,33 @@ def test_backward_reference_against_differences():
                 moved[i].view(-1)[at] += h
                 both.append(loss(*moved))
             assert abs((both[0] - both[1]) / 2e-4 - float(grad.reshape(-1)[at])) < 1e-5
+
+
+def test_training_step_workspaces(lib, axm):
+    """The two pieces add up to the one workspace; 8 bits keep less than a third of what bf16 keeps of a
+    large layer; sizes and flags that do not fit are refused."""
+    for flags in (0, axm.FLAG_SAVE_8BIT):
+        for shared in (0, 2):
+            d = axm.make_desc(300, 256, 512, 8, 2, shared, flags=axm.FLAG_RESIDUAL | flags)
+            n = ctypes.c_size_t(0)
+            assert lib.axm_moe_train_workspace_bytes(ctypes.byref(d), ctypes.byref(n)) == 0
+            assert sum(axm.train_split_bytes(d)) == n.value
+    plain = axm.train_split_bytes(axm.make_desc(8192, 2048, 4096, 16, 2))
+    in8 = axm.train_split_bytes(axm.make_desc(8192, 2048, 4096, 16, 2, flags=axm.FLAG_RESIDUAL | axm.FLAG_SAVE_8BIT))
+    assert 3 * in8[0] < plain[0]
+    t = axm.MoeTrain()
+    for f in ("x", "router_w", "w_gate", "w_up", "w_down", "out", "d_out", "d_x"):
+        setattr(t, f, FAKE.value)
+    for d in (axm.make_desc(4, 40, 64, 4, 2, flags=axm.FLAG_SAVE_8BIT), axm.make_desc(4, 64, 40, 4, 2, flags=axm.FLAG_SAVE_8BIT)):
+        a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        assert lib.axm_moe_train_split_bytes(ctypes.byref(d), ctypes.byref(a), ctypes.byref(b)) == axm.AXM_ERR_ARGUMENT
+        assert lib.axm_moe_forward_train(ctypes.byref(d), ctypes.byref(t), FAKE, 1 << 30, None) == axm.AXM_ERR_ARGUMENT
+        assert lib.axm_moe_backward(ctypes.byref(d), ctypes.byref(t), FAKE, 1 << 30, None) == axm.AXM_ERR_ARGUMENT
+    d = axm.make_desc(4, 64, 64, 4, 2, flags=axm.FLAG_SAVE_8BIT)
+    kept, scratch = axm.train_split_bytes(d)
+    for call in (lib.axm_moe_forward_train_split, lib.axm_moe_backward_split):
+        for k, kb, sc, sb in ((FAKE, kept - 1, FAKE, scratch), (FAKE, kept, FAKE, scratch - 1), (None, kept, FAKE, scratch),
+                              (FAKE, kept, None, scratch), (ODD, kept, FAKE, scratch), (FAKE, kept, ODD, scratch)):
+            assert call(ctypes.byref(d), ctypes.byref(t), k, kb, sc, sb, None) == axm.AXM_ERR_WORKSPACE
+        if not torch.cuda.is_available():
+            assert call(ctypes.byref(d), ctypes.byref(t), FAKE, kept, FAKE, scratch, None) == axm.AXM_ERR_DEVICE

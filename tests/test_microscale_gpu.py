@@ -517,3 +517,111 @@ def test_train_step_not_finite(ms, cuda_device):
     keep = torch.arange(64, device=dev) != 5
     assert torch.equal(o[keep], o2[keep]) and torch.equal(g["d_x"][keep], g2["d_x"][keep])
     assert torch.isnan(o2[5]).all() and torch.isnan(g2["d_x"][5]).all() and torch.isnan(g2["d_gate"]).any()
+
+
+def train_weights(gen, dev, d, f, e, shared, shift):
+    w = {"router_w": torch.empty(d, e, device=dev).normal_(0, 0.1, generator=gen)}
+    for n, k, shape in (("w_gate", e, (d, f)), ("w_up", e, (d, f)), ("w_down", e, (f, d)), ("shared_gate", shared, (d, f)),
+                        ("shared_up", shared, (d, f)), ("shared_down", shared, (f, d))):
+        if k:
+            w[n] = whole_values(gen, (k, *shape), 4, dev, shift).to(BF16)
+    return w
+
+
+@pytest.mark.parametrize("t,d,f,e,k,shared", [(1, 32, 64, 2, 1, 0), (70, 96, 160, 5, 2, 0), (130, 256, 512, 8, 2, 2),
+                                              (515, 160, 96, 16, 4, 1), (1000, 512, 704, 8, 2, 0)])
+def test_training_step_of_the_layer(ms, axm, cuda_device, t, d, f, e, k, shared):
+    """AXM_FLAG_SAVE_8BIT against the same step without it.  The forward pass is the same bit for bit.
+    Of the backward pass the weights' gradients are compared with the formula at the kept values
+    (whole numbers, so that g, u and dH are exact); the router's gradient with what the error of the
+    kept expert rows, half a step of e4m3, can make of it."""
+    dev = cuda_device
+    gen = generator(dev, t + d)
+    w = train_weights(gen, dev, d, f, e, shared, 2.0 ** -((d.bit_length() + 4) // 2))
+    x = whole_values(gen, (t, d), 4, dev, 0.5).to(BF16)
+    d_out = whole_values(gen, (t, d), 4, dev, 0.25).float()
+    plain = axm.MoeTrainLayer(w, t, k)
+    in8 = axm.MoeTrainLayer(w, t, k, save_8bit=True)
+    out, aux, want = plain.step(x, d_out)
+    out8, aux8, got = in8.step(x, d_out)
+    torch.cuda.synchronize()
+    for layer in (plain, in8):
+        assert int(layer.workspace[:4].view(torch.int32).item()) == 0
+    assert torch.equal(out, out8) and torch.equal(aux, aux8) and torch.equal(plain.histogram, in8.histogram)
+
+    # routing and gates as the layer's router gives them
+    lib = axm.load()
+    import helpers
+    desc = axm.make_desc(t, d, f, e, k, 0, axm.ROUTER_FP32, axm.FLAG_RESIDUAL)
+    logits, idx, gate, _ = helpers.run_router(axm, desc, x, w["router_w"])
+    X, dO = x.double(), d_out.double()
+    tiny = 2.0 ** -23
+    slack_o = torch.zeros(t, k, dtype=torch.float64, device=dev)  # on the gates' gradients
+
+    def compare(name, value, ref_value, slack):
+        err = (value.double() - ref_value).abs()
+        assert (err <= slack + 1e-30).all(), (name, float((err / (slack + 1e-30)).max()))
+
+    def expert(rows, d_o, wg, wu, wd, names, i):
+        if rows.numel() == 0:
+            assert all((got[n][i] == 0).all() for n in names)
+            return None
+        g, u = X[rows] @ wg, X[rows] @ wu
+        o = (g * torch.sigmoid(g) * u) @ wd
+        fast = (8 + 1.2 * float(g.abs().max())) * tiny
+        g, u = ref.held8(g), ref.held8(u)
+        (_, d_wg, d_wu, d_wd), (d_h, s, d_g, d_u, h) = ref.ffn_backward(X[rows], g, u, d_o, wg, wu, wd)
+        # d_o = bf16(gate dOut) is not a whole number: dH is a sum in 32 bits
+        e_dh = d * tiny * (d_o.abs() @ wd.abs().T)
+        slope = s + (g * s * (1 - s)).abs()
+        e_g = (d_h * u).abs() * slope * fast + e_dh * u.abs() * slope + 2.0 ** -8 * 1.01 * d_g.abs()
+        e_u = (2.0 ** -8 * 1.01 + fast) * d_u.abs() + e_dh * (g * s).abs()
+        e_h = (2.0 ** -8 * 1.01 + fast) * h.abs()
+        n, xa, da = int(rows.numel()), X[rows].abs(), d_o.abs()
+        for nm, v, e1, mag in ((names[0], d_wg, e_g, d_g), (names[1], d_wu, e_u, d_u)):
+            compare(nm, got[nm][i], v, xa.T @ e1 + n * tiny * (xa.T @ (mag.abs() + e1)))
+        compare(names[2], got[names[2]][i], d_wd, e_h.T @ da + n * tiny * ((h.abs() + e_h).T @ da))
+        return o
+
+    for i in range(e):
+        tok, slot = (idx == i).nonzero(as_tuple=True)
+        d_o = (gate[tok, slot].unsqueeze(1) * d_out[tok]).to(BF16).double()
+        o = expert(tok, d_o, *(w[n][i].double() for n in ("w_gate", "w_up", "w_down")), ("d_w_gate", "d_w_up", "d_w_down"), i)
+        if tok.numel():
+            b = o.unflatten(1, (-1, 32)).abs()
+            step = torch.maximum(2.0 ** -4 * b, 2.0 ** -4 * 2.0 ** -6 * b.amax(-1, keepdim=True))  # half a step; subnormals
+            step = torch.maximum(step, torch.where(b > 448 / 512 * b.amax(-1, keepdim=True), b / 8, step))  # 448 .. 512 saturate
+            slack_o[tok, slot] = (dO[tok].abs() * (1.02 * step.flatten(1) + 2.0 ** -7 * b.flatten(1))).sum(1)
+    for i in range(shared):
+        expert(torch.arange(t, device=dev), d_out.to(BF16).double(),
+               *(w[n][i].double() for n in ("shared_gate", "shared_up", "shared_down")),
+               ("d_shared_gate", "d_shared_up", "d_shared_down"), i)
+
+    # d gate / d logits, slot by slot, magnitudes
+    z = logits.double().requires_grad_(True)
+    p = torch.softmax(z, 1).gather(1, idx.long())
+    gates = p / p.sum(1, keepdim=True)
+    reach = torch.zeros(t, e, dtype=torch.float64, device=dev)
+    for j in range(k):
+        grad, = torch.autograd.grad(gates[:, j].sum(), z, retain_graph=True)
+        reach += grad.abs() * slack_o[:, j:j + 1]
+    slack = X.abs().T @ reach
+    compare("d_router_w", got["d_router_w"], want["d_router_w"].double(), slack + 1e-4 * want["d_router_w"].abs().max().double())
+
+    # d_x: the router's share, and 8 bits against 16 in the experts' (held8 is off by 2^-4 of a value
+    # at most, its slope included: see the bound on the weights' gradients above for the exact part)
+    far = (got["d_x"] - want["d_x"]).double()
+    through = (want["d_x"].double() - dO)
+    assert float(far.norm()) <= 0.08 * float(through.norm()) + float((reach @ w["router_w"].double().abs().T).norm())
+
+    # one scratch for two layers, the second running between the first one's passes
+    size = axm.train_split_bytes(in8.desc)[1]
+    scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+    a, b = (axm.MoeTrainLayer(w, t, k, save_8bit=True, scratch=scratch) for _ in range(2))
+    assert a.workspace.numel() + size == in8.workspace.numel()
+    y = torch.flip(x, (0,)).contiguous()
+    a.forward(x)
+    b.forward(y)
+    b.backward(y, d_out)
+    a.backward(x, d_out)
+    assert torch.equal(a.out, out8) and torch.equal(a.d_x, got["d_x"]) and torch.equal(a.d_w_down, got["d_w_down"])
