@@ -14,6 +14,7 @@ work goes to the current stream, nothing synchronises.  The engine keeps its wei
 with fp32 masters (core/src/CUDA/util/gpu_types.cuh:148-168); either is a source here.
 """
 import ctypes
+import functools
 import importlib
 
 import torch
@@ -29,22 +30,17 @@ def _dtype(t):
     return _DTYPES[t]
 
 
-class _Here:
-    """The tensors' device is the current one already."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_here = _Here()
-
-
-def _on(device):
-    """The library enqueues on the current device: make it the tensors'."""
-    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _on_its_device(call):
+    """The library enqueues on the current device: makes that the device of the call's first tensor (or of
+    the object's)."""
+    @functools.wraps(call)
+    def wrapped(first, *args, **kw):
+        device = first.device
+        if device.index is None or device.index == torch.cuda.current_device():  # host tensors are refused inside
+            return call(first, *args, **kw)
+        with torch.cuda.device(device):
+            return call(first, *args, **kw)
+    return wrapped
 
 
 def _rows_of(x):
@@ -59,10 +55,6 @@ def _rows_of(x):
 
 def _address(t):
     return None if t is None else t.data_ptr()
-
-
-def _up(n, to):
-    return (n + to - 1) // to * to
 
 
 def _bytes(call, *args):
@@ -86,12 +78,17 @@ class Mx4Rows:
     def scales(self):
         return self.buffer[self.scales_at:]
 
+    @property
+    def device(self):
+        return self.buffer.device
+
 
 class Mx4Weights:
     """Weights in 4 bits: codes [E][N][K/2], tile-ordered scales."""
 
     def __init__(self, codes, scales, experts, k, n):
         self.codes, self.scales, self.experts, self.k, self.n = codes, scales, experts, k, n
+        self.device = codes.device
 
     @classmethod
     def from_checkpoint(cls, codes, scales):
@@ -106,99 +103,102 @@ class Mx4Weights:
         if scales.shape != (e, n, k // 32):
             raise ValueError(f"scales {tuple(scales.shape)} do not belong to codes {tuple(codes.shape)}")
         _, size = _bytes(lib.axm_mx4_weights_bytes, e, k, n)
-        with _on(codes.device):
+        with torch.cuda.device(codes.device):
             packed = torch.empty(size, dtype=torch.uint8, device=codes.device)
             _pkg.check(lib.axm_mx4_pack_scales(scales.data_ptr(), e, k, n, packed.data_ptr(),
                                                _pkg.raw_stream(codes.device.index)))
         return cls(codes, packed, e, k, n)
 
 
+@_on_its_device
 def quantize_rows(x, segments=None, row_src=None, row_div=1):
     """x [rows][K] bf16 or fp32 to 4 bits; row_src: row r is read from x[row_src[r] // row_div]."""
-    lib = _pkg.load()
-    src_rows, k, ld = _rows_of(x)
-    rows = src_rows if row_src is None else row_src.numel()
-    nseg = 0 if segments is None else segments.shape[0]
+    rows, k, ld = _rows_of(x)
+    nseg = 0
+    if row_src is not None:
+        rows = row_src.numel()
+    if segments is not None:
+        nseg = segments.shape[0]
     # the sizes of axm_mx4_rows_bytes; sizes that it refuses are refused by the call below
-    at = _up(rows * (k // 2), 256)
-    size = at + (rows // 128 + max(nseg, 1)) * (_up(max(k, 0), 256) // 128) * 512
+    at = (rows * (k // 2) + 255) & -256
+    size = at + (rows // 128 + (nseg or 1)) * ((k + 255) >> 8) * 1024
     device = x.device
-    with _on(device):
-        buffer = torch.empty(size, dtype=torch.uint8, device=device)
-        base = buffer.data_ptr()
-        _pkg.check(lib.axm_mx4_quantize_rows(x.data_ptr(), _dtype(x.dtype), ld, _address(row_src), row_div, rows, k,
-                                             _address(segments), nseg, base, base + at, _pkg.raw_stream(device.index)))
+    buffer = torch.empty(size, dtype=torch.uint8, device=device)
+    base = buffer.data_ptr()
+    status = _pkg.load().axm_mx4_quantize_rows(x.data_ptr(), _dtype(x.dtype), ld, _address(row_src), row_div, rows, k,
+                                               _address(segments), nseg, base, base + at, _pkg.raw_stream(device.index))
+    if status:
+        _pkg.check(status)
     return Mx4Rows(buffer, at, rows, k, segments)
 
 
+@_on_its_device
 def dequantize_rows(q, dtype=torch.bfloat16, out=None):
-    lib = _pkg.load()
-    device, rows, k, ld = q.buffer.device, q.rows, q.k, q.k
-    with _on(device):
-        if out is None:
-            out = torch.empty((rows, k), dtype=dtype, device=device)
-        else:
-            got = _rows_of(out)
-            if got[:2] != (rows, k) or out.device != device:
-                raise ValueError(f"out is {tuple(out.shape)} on {out.device}, the rows are {(rows, k)} on {device}")
-            ld = got[2]
-        nseg = 0 if q.segments is None else q.segments.shape[0]
-        base = q.buffer.data_ptr()
-        _pkg.check(lib.axm_mx4_dequantize_rows(base, base + q.scales_at, rows, k, _address(q.segments), nseg,
-                                               out.data_ptr(), _dtype(out.dtype), ld, _pkg.raw_stream(device.index)))
+    buffer, rows, k, ld = q.buffer, q.rows, q.k, q.k
+    device = buffer.device
+    if out is None:
+        out = torch.empty((rows, k), dtype=dtype, device=device)
+    else:
+        got = _rows_of(out)
+        if got[:2] != (rows, k) or out.device != device:
+            raise ValueError(f"out is {tuple(out.shape)} on {out.device}, the rows are {(rows, k)} on {device}")
+        dtype, ld = out.dtype, got[2]
+    segments = q.segments
+    base = buffer.data_ptr()
+    status = _pkg.load().axm_mx4_dequantize_rows(base, base + q.scales_at, rows, k, _address(segments),
+                                                 0 if segments is None else segments.shape[0], out.data_ptr(),
+                                                 _dtype(dtype), ld, _pkg.raw_stream(device.index))
+    if status:
+        _pkg.check(status)
     return out
 
 
+@_on_its_device
 def quantize_rows8(x):
     """x [rows][K] to 8 bits: codes [rows][K] (e4m3), scale bytes [rows][K/32]."""
-    lib = _pkg.load()
     rows, k, ld = _rows_of(x)
     device = x.device
-    with _on(device):
-        codes = torch.empty((rows, k), dtype=torch.uint8, device=device)
-        scales = torch.empty((rows, k // 32), dtype=torch.uint8, device=device)
-        _pkg.check(lib.axm_mx8_quantize_rows(x.data_ptr(), _dtype(x.dtype), ld, rows, k, codes.data_ptr(),
-                                             scales.data_ptr(), _pkg.raw_stream(device.index)))
+    codes = torch.empty((rows, k), dtype=torch.uint8, device=device)
+    scales = torch.empty((rows, k // 32), dtype=torch.uint8, device=device)
+    _pkg.check(_pkg.load().axm_mx8_quantize_rows(x.data_ptr(), _dtype(x.dtype), ld, rows, k, codes.data_ptr(),
+                                                 scales.data_ptr(), _pkg.raw_stream(device.index)))
     return codes, scales
 
 
+@_on_its_device
 def dequantize_rows8(codes, scales, dtype=torch.bfloat16):
-    lib = _pkg.load()
     rows, k = codes.shape
     device = codes.device
-    if not (codes.is_contiguous() and scales.is_contiguous() and scales.shape == (rows, k // 32) and scales.device == device
-            and codes.dtype == scales.dtype == torch.uint8):
-        raise ValueError("contiguous uint8 codes [rows][K] and scales [rows][K/32] on one device are needed")
-    with _on(device):
-        out = torch.empty((rows, k), dtype=dtype, device=device)
-        _pkg.check(lib.axm_mx8_dequantize_rows(codes.data_ptr(), scales.data_ptr(), rows, k, out.data_ptr(), _dtype(dtype),
-                                               k, _pkg.raw_stream(device.index)))
+    if not (codes.is_cuda and codes.is_contiguous() and scales.is_contiguous() and scales.shape == (rows, k // 32) and
+            scales.device == device and codes.dtype == scales.dtype == torch.uint8):
+        raise ValueError("contiguous uint8 codes [rows][K] and scales [rows][K/32] on one CUDA device are needed")
+    out = torch.empty((rows, k), dtype=dtype, device=device)
+    _pkg.check(_pkg.load().axm_mx8_dequantize_rows(codes.data_ptr(), scales.data_ptr(), rows, k, out.data_ptr(),
+                                                   _dtype(dtype), k, _pkg.raw_stream(device.index)))
     return out
 
 
+@_on_its_device
 def quantize_weights(w):
     """w [E][K][N] bf16 or fp32 (the engine's layout, K is summed over) to 4 bits."""
-    lib = _pkg.load()
     if not (w.is_cuda and w.dim() == 3 and w.is_contiguous()):
         raise ValueError("a contiguous CUDA tensor [E][K][N] is needed")
     e, k, n = w.shape
     device = w.device
-    with _on(device):
-        codes = torch.empty((e, n, k // 2), dtype=torch.uint8, device=device)
-        # the size of axm_mx4_weights_bytes; sizes that it refuses are refused by the call below
-        scales = torch.empty(e * (_up(n, 128) // 128) * (_up(k, 256) // 128) * 512, dtype=torch.uint8, device=device)
-        _pkg.check(lib.axm_mx4_quantize_weights(w.data_ptr(), _dtype(w.dtype), e, k, n, codes.data_ptr(), scales.data_ptr(),
-                                                _pkg.raw_stream(device.index)))
+    codes = torch.empty((e, n, k // 2), dtype=torch.uint8, device=device)
+    # the size of axm_mx4_weights_bytes; sizes that it refuses are refused by the call below
+    scales = torch.empty(e * ((n + 127) >> 7) * ((k + 255) >> 8) * 1024, dtype=torch.uint8, device=device)
+    _pkg.check(_pkg.load().axm_mx4_quantize_weights(w.data_ptr(), _dtype(w.dtype), e, k, n, codes.data_ptr(),
+                                                    scales.data_ptr(), _pkg.raw_stream(device.index)))
     return Mx4Weights(codes, scales, e, k, n)
 
 
+@_on_its_device
 def dequantize_weights(q, dtype=torch.bfloat16):
-    lib = _pkg.load()
-    device = q.codes.device
-    with _on(device):
-        w = torch.empty((q.experts, q.k, q.n), dtype=dtype, device=device)
-        _pkg.check(lib.axm_mx4_dequantize_weights(q.codes.data_ptr(), q.scales.data_ptr(), q.experts, q.k, q.n, w.data_ptr(),
-                                                  _dtype(dtype), _pkg.raw_stream(device.index)))
+    device = q.device
+    w = torch.empty((q.experts, q.k, q.n), dtype=dtype, device=device)
+    _pkg.check(_pkg.load().axm_mx4_dequantize_weights(q.codes.data_ptr(), q.scales.data_ptr(), q.experts, q.k, q.n,
+                                                      w.data_ptr(), _dtype(dtype), _pkg.raw_stream(device.index)))
     return w
 
 
@@ -206,6 +206,7 @@ class _Workspace:
     """Scratch of one object; its first word is the status word."""
 
     def _scratch(self, size, device):
+        self.device = device
         self.workspace = torch.empty(max(size, 256), dtype=torch.uint8, device=device)
 
     def status(self):
@@ -226,21 +227,22 @@ class Mx4Linear(_Workspace):
         _pkg.check(self.lib.axm_mx4_linear_workspace_bytes(tokens, weights.k, weights.n, ctypes.byref(n)))
         self._scratch(n.value, weights.codes.device)
 
+    @_on_its_device
     def forward(self, x, out=None, dtype=torch.bfloat16):
-        w = self.w
+        w, device = self.w, self.device
         rows, k, ld = _rows_of(x)
-        if rows > self.tokens or k != w.k or x.device != w.codes.device:
-            raise ValueError(f"x {tuple(x.shape)} on {x.device}: up to {self.tokens} rows of {w.k} on {w.codes.device}")
+        if rows > self.tokens or k != w.k or x.device != device:
+            raise ValueError(f"x {tuple(x.shape)} on {x.device}: up to {self.tokens} rows of {w.k} on {device}")
         if out is None:
-            out = torch.empty(rows, w.n, dtype=dtype, device=x.device)
-        elif out.shape != (rows, w.n) or not out.is_contiguous() or out.device != x.device:
+            out = torch.empty((rows, w.n), dtype=dtype, device=device)
+        elif out.shape != (rows, w.n) or not out.is_contiguous() or out.device != device:
             raise ValueError("out must be a contiguous [rows][N] matrix beside x")
-        device = x.device
-        with _on(device):
-            _pkg.check(self.lib.axm_mx4_linear(x.data_ptr(), _dtype(x.dtype), ld, rows, k, w.n, w.codes.data_ptr(),
-                                               w.scales.data_ptr(), out.data_ptr(), _dtype(out.dtype),
-                                               self.workspace.data_ptr(), self.workspace.numel(),
-                                               _pkg.raw_stream(device.index)))
+        status = self.lib.axm_mx4_linear(x.data_ptr(), _dtype(x.dtype), ld, rows, k, w.n, w.codes.data_ptr(),
+                                         w.scales.data_ptr(), out.data_ptr(), _dtype(out.dtype),
+                                         self.workspace.data_ptr(), self.workspace.numel(),
+                                         _pkg.raw_stream(device.index))
+        if status:
+            _pkg.check(status)
         return out
 
 
@@ -266,10 +268,11 @@ class Mx4ExpertFfn(_Workspace):
                                                                ctypes.byref(n)))
         self._scratch(n.value, gate.codes.device)
 
+    @_on_its_device
     def forward(self, x, segments, out=None, dtype=torch.bfloat16):
         """x [rows][D] bf16, segments int32 [n][4] {a_row0, out_row0, rows, expert} (device)."""
         rows, d, _ = _rows_of(x)
-        dev = self.workspace.device
+        dev = self.device
         if rows > self.rows or d != self.desc.d_model or not x.is_contiguous() or x.dtype != torch.bfloat16 or x.device != dev:
             raise ValueError(f"x: up to {self.rows} contiguous bf16 rows of {self.desc.d_model} on {dev}")
         if segments.dtype != torch.int32 or segments.shape[1:] != (4,) or not segments.is_contiguous() or \
@@ -279,11 +282,10 @@ class Mx4ExpertFfn(_Workspace):
             out = torch.empty(rows, d, dtype=dtype, device=dev)
         elif out.shape != x.shape or not out.is_contiguous() or out.device != dev:
             raise ValueError("out must be a contiguous matrix like x")
-        with _on(dev):
-            _pkg.check(self.lib.axm_mx4_expert_ffn(ctypes.byref(self.desc), x.data_ptr(), rows, segments.data_ptr(),
-                                                   segments.shape[0], ctypes.byref(self.table), out.data_ptr(),
-                                                   _dtype(out.dtype), self.workspace.data_ptr(), self.workspace.numel(),
-                                                   _pkg.raw_stream(dev.index)))
+        _pkg.check(self.lib.axm_mx4_expert_ffn(ctypes.byref(self.desc), x.data_ptr(), rows, segments.data_ptr(),
+                                               segments.shape[0], ctypes.byref(self.table), out.data_ptr(),
+                                               _dtype(out.dtype), self.workspace.data_ptr(), self.workspace.numel(),
+                                               _pkg.raw_stream(dev.index)))
         return out
 
 
@@ -314,9 +316,10 @@ class Mx4MoeLayer(_Workspace):
         self.topk_gate = torch.empty(tokens, top_k, dtype=torch.float32, device=dev)
         self.histogram = torch.zeros(gate.experts, dtype=torch.int32, device=dev)
 
+    @_on_its_device
     def forward(self, x, out=None):
         """out = x + sum of the chosen experts' outputs (without residual: the sum), histogram."""
-        dev = self.workspace.device
+        dev = self.device
         if x.shape != (self.T, self.D) or x.dtype != torch.bfloat16 or not x.is_contiguous() or x.device != dev:
             raise ValueError(f"x: contiguous bf16 {(self.T, self.D)} on {dev}")
         if out is None:
@@ -327,11 +330,10 @@ class Mx4MoeLayer(_Workspace):
             t.router_bias = self.w["router_bias"].data_ptr()
         t.topk_idx, t.topk_gate = self.topk_idx.data_ptr(), self.topk_gate.data_ptr()
         t.histogram = self.histogram.data_ptr()
-        with _on(dev):
-            _pkg.check(self.lib.axm_moe_forward_mx4(ctypes.byref(self.desc), ctypes.byref(t), ctypes.byref(self.experts),
-                                                    None if self.shared is None else ctypes.byref(self.shared),
-                                                    self.workspace.data_ptr(), self.workspace.numel(),
-                                                    _pkg.raw_stream(dev.index)))
+        _pkg.check(self.lib.axm_moe_forward_mx4(ctypes.byref(self.desc), ctypes.byref(t), ctypes.byref(self.experts),
+                                                None if self.shared is None else ctypes.byref(self.shared),
+                                                self.workspace.data_ptr(), self.workspace.numel(),
+                                                _pkg.raw_stream(dev.index)))
         return out, self.histogram
 
 
@@ -352,7 +354,7 @@ class Mx8TrainFfn:
         for w in (gate, up, down):
             if w.dtype != torch.bfloat16 or not w.is_contiguous() or not w.is_cuda or w.device != gate.device:
                 raise ValueError("contiguous bf16 CUDA weights on one device are needed")
-        dev = gate.device
+        dev = self.device = gate.device
         self.weights, self.rows, self.dtype = (gate, up, down), rows, dtype
         _dtype(dtype)
         self.desc = _pkg.make_desc(rows, d, f, e, 1, flags=0)
@@ -373,6 +375,7 @@ class Mx8TrainFfn:
                 not t.is_contiguous() or t.device != self.status_word.device:
             raise ValueError(f"{what}: up to {self.rows} contiguous bf16 rows of {self.desc.d_model} on {self.status_word.device}")
 
+    @_on_its_device
     def forward(self, x, segments, out=None):
         self._check(x, "x")
         if segments.dtype != torch.int32 or segments.shape[1:] != (4,) or not segments.is_contiguous() or segments.device != x.device:
@@ -380,14 +383,14 @@ class Mx8TrainFfn:
         if out is None:
             out = torch.empty(x.shape, dtype=self.dtype, device=x.device)
         p = _address
-        with _on(x.device):
-            _pkg.check(self.lib.axm_mx8_expert_ffn_train(
-                ctypes.byref(self.desc), p(x), x.shape[0], p(segments), segments.shape[0], *map(p, self.weights),
-                ctypes.byref(self.keep), p(self.scratch[0]), p(out), _dtype(out.dtype), p(self.status_word),
-                _pkg.raw_stream(x.device.index)))
+        _pkg.check(self.lib.axm_mx8_expert_ffn_train(
+            ctypes.byref(self.desc), p(x), x.shape[0], p(segments), segments.shape[0], *map(p, self.weights),
+            ctypes.byref(self.keep), p(self.scratch[0]), p(out), _dtype(out.dtype), p(self.status_word),
+            _pkg.raw_stream(self.device.index)))
         self.saved = (x, segments)
         return out
 
+    @_on_its_device
     def backward(self, d_o, weight_grads=True):
         """{d_x, d_gate, d_up, d_down} (weight_grads False: d_x alone) of the last forward call."""
         if self.saved is None:
@@ -401,10 +404,9 @@ class Mx8TrainFfn:
         if weight_grads:
             for n, w in zip(("d_gate", "d_up", "d_down"), self.weights):
                 grads[n] = torch.empty(w.shape, dtype=self.dtype, device=x.device)
-        with _on(x.device):
-            _pkg.check(self.lib.axm_mx8_expert_ffn_backward(
-                ctypes.byref(self.desc), p(x), x.shape[0], p(segments), segments.shape[0], ctypes.byref(self.keep), p(d_o),
-                *map(p, self.weights), *map(p, self.scratch), p(grads["d_x"]), p(grads.get("d_gate")),
-                p(grads.get("d_up")), p(grads.get("d_down")), _dtype(self.dtype), p(self.status_word),
-                _pkg.raw_stream(x.device.index)))
+        _pkg.check(self.lib.axm_mx8_expert_ffn_backward(
+            ctypes.byref(self.desc), p(x), x.shape[0], p(segments), segments.shape[0], ctypes.byref(self.keep), p(d_o),
+            *map(p, self.weights), *map(p, self.scratch), p(grads["d_x"]), p(grads.get("d_gate")),
+            p(grads.get("d_up")), p(grads.get("d_down")), _dtype(self.dtype), p(self.status_word),
+            _pkg.raw_stream(self.device.index)))
         return grads
