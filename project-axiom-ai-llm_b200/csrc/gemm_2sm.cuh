@@ -109,6 +109,52 @@ __device__ __forceinline__ void tc_mma2_bf16(uint32_t d_tmem, uint64_t desc_a, u
 }
 
 
+// Fills the tables that a pair kernel's units are decoded from, out of sh->seg, by one warp: row tiles
+// before each segment, groups of neighbouring segments with one expert, pairs of row tiles before
+// each group.  (By one thread it took 5 us for 64 segments, at the start of every launch.)
+template <typename Shared>
+__device__ __forceinline__ void count_tiles(Shared* sh, int nseg, int n_tiles) {
+  const int lane = threadIdx.x & 31;
+  auto scan = [&](int v) {  // inclusive sum over the lanes
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += t;
+    }
+    return v;
+  };
+  int tiles = 0, groups = 0;
+  for (int s0 = 0; s0 < nseg; s0 += 32) {
+    const int s = s0 + lane;
+    const int rows = s < nseg ? sh->seg[s].rows : 0;
+    const int mine = rows > 0 ? (rows + BM - 1) / BM : 0;
+    const int first = s < nseg && (s == 0 || sh->seg[s].expert != sh->seg[s - 1].expert) ? 1 : 0;
+    const int t = scan(mine), g = scan(first);
+    if (s < nseg) sh->tile_prefix[s] = tiles + t - mine;
+    if (first) sh->group_first[groups + g - 1] = s;
+    tiles += __shfl_sync(0xffffffffu, t, 31);
+    groups += __shfl_sync(0xffffffffu, g, 31);
+  }
+  if (lane == 0) {
+    sh->tile_prefix[nseg] = tiles;
+    sh->group_first[groups] = nseg;
+    sh->num_groups = groups;
+  }
+  __syncwarp();
+  int pairs = 0;
+  for (int g0 = 0; g0 < groups; g0 += 32) {
+    const int g = g0 + lane;
+    const int mine = g < groups ? (sh->tile_prefix[sh->group_first[g + 1]] - sh->tile_prefix[sh->group_first[g]] + 1) / 2 : 0;
+    const int p = scan(mine);
+    if (g < groups) sh->pair_prefix[g] = pairs + p - mine;
+    pairs += __shfl_sync(0xffffffffu, p, 31);
+  }
+  if (lane == 0) {
+    sh->pair_prefix[groups] = pairs;
+    sh->total_units = pairs * n_tiles;
+  }
+}
+
 // Programmatic launches: a kernel that is followed by one launched this way lets it start at once, and
 // one launched this way waits, before it touches global memory, until everything before it is done.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }

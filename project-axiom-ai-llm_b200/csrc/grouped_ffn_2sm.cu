@@ -229,28 +229,7 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
   if (args.overlap) wait_for_previous();
   for (int s = threadIdx.x; s < nseg; s += gemm2_threads(kMode)) sh->seg[s] = args.segments[s];
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int acc = 0;
-    for (int s = 0; s < nseg; ++s) {
-      sh->tile_prefix[s] = acc;
-      int rows = sh->seg[s].rows;
-      acc += rows > 0 ? (rows + BM - 1) / BM : 0;
-    }
-    sh->tile_prefix[nseg] = acc;
-    int ng = 0;
-    for (int s = 0; s < nseg; ++s)
-      if (s == 0 || sh->seg[s].expert != sh->seg[s - 1].expert) sh->group_first[ng++] = s;
-    sh->group_first[ng] = nseg;
-    sh->num_groups = ng;
-    int pairs = 0;
-    for (int g = 0; g < ng; ++g) {
-      sh->pair_prefix[g] = pairs;
-      int mt = sh->tile_prefix[sh->group_first[g + 1]] - sh->tile_prefix[sh->group_first[g]];
-      pairs += (mt + 1) / 2;
-    }
-    sh->pair_prefix[ng] = pairs;
-    sh->total_units = pairs * n_tiles;
-  }
+  if (warp == 0) count_tiles(sh, nseg, n_tiles);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // barriers of both CTAs are initialised before anyone signals across

@@ -475,7 +475,7 @@ RowLaunch row_launch(int32_t rows, int32_t k, int ahead) {
   while (l.log_wpr < 3 && (2 << l.log_wpr) <= runs) ++l.log_wpr;
   // enough rows for every SM's warps: several runs a warp rather than several warps a row (not for
   // fp32 sources, ahead = 1: their runs are twice as long, 8-bit rows 8191 x 5632 58 us against 63)
-  while (l.log_wpr > 0 && (runs >> l.log_wpr) < ahead && ((long long)rows << (l.log_wpr - 1)) >= 128LL * sm_count()) --l.log_wpr;
+  while (l.log_wpr > 0 && (runs >> l.log_wpr) < ahead && ((long long)rows << (l.log_wpr - 1)) >= 16LL * sm_count()) --l.log_wpr;
   const long long per = (long long)(8 >> l.log_wpr) << (5 - l.log_lanes);
   const long long blocks = (rows + per - 1) / per, most = 32LL * sm_count();
   l.grid = (unsigned)(blocks < most ? blocks : most);

@@ -167,6 +167,89 @@ __device__ __forceinline__ uint4 gate_block(const uint32_t (&g)[32], const uint3
   return make_uint4(q[0], q[1], q[2], q[3]);
 }
 
+// The epilogue of one tile by one of four warps: 128 accumulator rows from `acc` on, a row a thread.
+// free_shared() (one lane) is called once the columns that both accumulators use have been read.
+template <int kMode, typename Free>
+__device__ __forceinline__ void drain_tile(const Mx4Args& args, const Unit4& u, const AxmSegment& sg, uint32_t tmem_base,
+                                           int acc, int n_tiles, Free free_shared) {
+  constexpr bool kGated = kMode == kModeGated;
+  constexpr int kCols = kGated ? 128 : 256;
+  const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3;
+  const int row_in_seg = u.m_tile * 128 + quad * 32 + lane;
+  const bool row_ok = u.live && row_in_seg < sg.rows;
+  const size_t row = (size_t)sg.out_row0 + (row_ok ? row_in_seg : 0);
+  const uint32_t t_addr = tmem_base + ((uint32_t)(quad * 32) << 16) + (acc ? kAcc1 : 0u);
+  const int n0 = u.n_tile * kCols;
+  // blocks of 32 columns; the shared columns are the last 24 of accumulator 0 and the first
+  // 24 of accumulator 1
+  constexpr int kBlocks = kCols / 32;
+  uint32_t sf_word = 0;
+#pragma unroll 1
+  for (int i = 0; i < kBlocks; ++i) {
+    const int jb = acc ? i : kBlocks - 1 - i;
+    const int c0 = jb * 32;
+    uint32_t v[32];
+    __syncwarp();
+    tmem_ld32(t_addr + c0, v);
+    if constexpr (kGated) {
+      uint32_t up[32];
+      tmem_ld32(t_addr + 128 + c0, up);
+      tmem_ld_wait();
+      if (i == 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) free_shared();
+      }
+      if (u.live && n0 + c0 < args.n_total) {  // n_total is a multiple of 32
+        uint32_t byte;
+        const uint4 q = gate_block(v, up, byte);
+        sf_word |= byte << (8 * jb);
+        if (row_ok)
+          __stcs(reinterpret_cast<uint4*>(static_cast<uint8_t*>(args.out) + row * (size_t)(args.n_total >> 1) +
+                                          ((n0 + c0) >> 1)), q);
+      }
+    } else {
+      tmem_ld_wait();
+      if (i == 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) free_shared();
+      }
+      if (row_ok) {
+        if (args.out_bf16) {
+          __nv_bfloat16* p = static_cast<__nv_bfloat16*>(args.out) + row * args.n_total + n0 + c0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (n0 + c0 + q * 8 < args.n_total) {
+              uint32_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                w[j] = pack_bf16(__uint_as_float(v[8 * q + 2 * j]), __uint_as_float(v[8 * q + 2 * j + 1]));
+              __stcs(reinterpret_cast<uint4*>(p + q * 8), make_uint4(w[0], w[1], w[2], w[3]));
+            }
+        } else {
+          float* p = static_cast<float*>(args.out) + row * args.n_total + n0 + c0;
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (n0 + c0 + q * 4 < args.n_total)
+              __stcs(reinterpret_cast<uint4*>(p + q * 4), make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+        }
+      }
+    }
+  }
+  if constexpr (kGated) {
+    // one chunk of scale bytes a tile (128 columns); behind the last one of an odd number, zeros
+    if (row_ok) {
+      const int r = row_in_seg & 127;
+      const size_t t = (size_t)(sg.out_row0 / 128 + args.seg_base + u.seg + u.m_tile);
+      const int chunks = mx4_chunks(args.n_total);
+      uint8_t* p = args.out_scales + (t * chunks + u.n_tile) * 512 + (r & 31) * 16 + (r >> 5) * 4;
+      *reinterpret_cast<uint32_t*>(p) = sf_word;
+      if (u.n_tile == n_tiles - 1 && n_tiles < chunks) *reinterpret_cast<uint32_t*>(p + 512) = 0u;
+    }
+  }
+}
+
 template <int kMode>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads4, 1)
 mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a_sf,
@@ -218,27 +301,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     tmem_alloc2(&sh->tmem_base, kTmemCols);
     tmem_relinquish2();
   }
-  if (threadIdx.x == 0) {
-    int acc = 0;
-    for (int s = 0; s < nseg; ++s) {
-      sh->tile_prefix[s] = acc;
-      const int rows = sh->seg[s].rows;
-      acc += rows > 0 ? (rows + 127) / 128 : 0;
-    }
-    sh->tile_prefix[nseg] = acc;
-    int ng = 0;
-    for (int s = 0; s < nseg; ++s)
-      if (s == 0 || sh->seg[s].expert != sh->seg[s - 1].expert) sh->group_first[ng++] = s;
-    sh->group_first[ng] = nseg;
-    sh->num_groups = ng;
-    int pairs = 0;
-    for (int g = 0; g < ng; ++g) {
-      sh->pair_prefix[g] = pairs;
-      pairs += (sh->tile_prefix[sh->group_first[g + 1]] - sh->tile_prefix[sh->group_first[g]] + 1) / 2;
-    }
-    sh->pair_prefix[ng] = pairs;
-    sh->total_units = pairs * n_tiles;
-  }
+  if (warp == 0) count_tiles(sh, nseg, n_tiles);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
@@ -352,88 +415,13 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     }
   } else {
     // ---- epilogue: every CTA drains its own 128 accumulator rows --------------------------------
-    const int quad = warp & 3;
     const uint32_t leader_free = map_to_cta(smem_u32(&sh->overlap_free), 0);
     int tile = 0;
     for (int unit = cluster_id; unit < total_units; unit += num_clusters, ++tile) {
       const Unit4 uc = decode4(sh, n_tiles, unit, (int)rank);
-      const AxmSegment sg = sh->seg[uc.seg];
-      const int acc = tile & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(&sh->tmem_full[acc], (uint32_t)((tile >> 1) & 1), abort_flag))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&sh->tmem_full[tile & 1], (uint32_t)((tile >> 1) & 1), abort_flag))) break;
       tc_fence_after();
-      const int row_in_seg = uc.m_tile * 128 + quad * 32 + lane;
-      const bool row_ok = uc.live && row_in_seg < sg.rows;
-      const size_t row = (size_t)sg.out_row0 + (row_ok ? row_in_seg : 0);
-      const uint32_t t_addr = tmem_base + ((uint32_t)(quad * 32) << 16) + (acc ? kAcc1 : 0u);
-      const int n0 = uc.n_tile * kCols;
-      // blocks of 32 columns; the shared columns are the last 24 of accumulator 0 and the first
-      // 24 of accumulator 1
-      constexpr int kBlocks = kCols / 32;
-      uint32_t sf_word = 0;
-#pragma unroll 1
-      for (int i = 0; i < kBlocks; ++i) {
-        const int jb = acc ? i : kBlocks - 1 - i;
-        const int c0 = jb * 32;
-        uint32_t v[32];
-        __syncwarp();
-        tmem_ld32(t_addr + c0, v);
-        if constexpr (kGated) {
-          uint32_t u[32];
-          tmem_ld32(t_addr + 128 + c0, u);
-          tmem_ld_wait();
-          if (i == 0) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(leader_free);
-          }
-          if (uc.live && n0 + c0 < args.n_total) {  // n_total is a multiple of 32
-            uint32_t byte;
-            const uint4 q = gate_block(v, u, byte);
-            sf_word |= byte << (8 * jb);
-            if (row_ok)
-              __stcs(reinterpret_cast<uint4*>(static_cast<uint8_t*>(args.out) + row * (size_t)(args.n_total >> 1) +
-                                              ((n0 + c0) >> 1)), q);
-          }
-        } else {
-          tmem_ld_wait();
-          if (i == 0) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(leader_free);
-          }
-          if (row_ok) {
-            if (args.out_bf16) {
-              __nv_bfloat16* p = static_cast<__nv_bfloat16*>(args.out) + row * args.n_total + n0 + c0;
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                if (n0 + c0 + q * 8 < args.n_total) {
-                  uint32_t w[4];
-#pragma unroll
-                  for (int j = 0; j < 4; ++j)
-                    w[j] = pack_bf16(__uint_as_float(v[8 * q + 2 * j]), __uint_as_float(v[8 * q + 2 * j + 1]));
-                  __stcs(reinterpret_cast<uint4*>(p + q * 8), make_uint4(w[0], w[1], w[2], w[3]));
-                }
-            } else {
-              float* p = static_cast<float*>(args.out) + row * args.n_total + n0 + c0;
-#pragma unroll
-              for (int q = 0; q < 8; ++q)
-                if (n0 + c0 + q * 4 < args.n_total)
-                  __stcs(reinterpret_cast<uint4*>(p + q * 4), make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
-            }
-          }
-        }
-      }
-      if constexpr (kGated) {
-        // one chunk of scale bytes a tile (128 columns); behind the last one of an odd number, zeros
-        if (row_ok) {
-          const int r = row_in_seg & 127;
-          const size_t t = (size_t)(sg.out_row0 / 128 + args.seg_base + uc.seg + uc.m_tile);
-          const int chunks = mx4_chunks(args.n_total);
-          uint8_t* p = args.out_scales + (t * chunks + uc.n_tile) * 512 + (r & 31) * 16 + (r >> 5) * 4;
-          *reinterpret_cast<uint32_t*>(p) = sf_word;
-          if (uc.n_tile == n_tiles - 1 && n_tiles < chunks) *reinterpret_cast<uint32_t*>(p + 512) = 0u;
-        }
-      }
+      drain_tile<kMode>(args, uc, sh->seg[uc.seg], tmem_base, tile & 1, n_tiles, [&] { mbar_arrive_cluster(leader_free); });
     }
   }
 
