@@ -35,6 +35,7 @@ __host__ __device__ constexpr long long mx4_row_tiles_most(long long rows, int n
 
 // The rows of a grouped 4-bit product: a segment table in device memory (its rows are out_row0 ..
 // of the operand and of the output; a_row0 is not looked at), or none: one segment of all rows.
+enum { kMx4Few = 0, kMx4Single = 1, kMx4Pair = 2 };  // mx4_few.cu; the two of mx4_gemm.cu
 struct Mx4Rows {
   const AxmSegment* segments;
   int num_segments;
@@ -43,7 +44,7 @@ struct Mx4Rows {
   int seg_base;        // index of segments[0] in that table
   int expert_base;     // expert id of the first weight matrix of this launch
   int tile_rows;       // rows of a scale tile (and of a row tile of the few-rows kernels: 16, 32, 64, 128)
-  bool few;            // few rows a segment: mx4_few.cu instead of mx4_gemm.cu
+  int kernel;          // kMx4Few, kMx4Single or kMx4Pair
   int32_t* status;
   float* few_partial;      // workspace of the few-rows kernels: partial tiles,
   uint32_t* few_counters;  //   a counter a tile (zero before the first launch of a call)
@@ -66,7 +67,8 @@ int launch_mx4_gated(const Mx4Rows& r, const void* a_codes, const void* a_scales
                      int d, int f, void* h_codes, void* h_scales, cudaStream_t st);
 
 // The same for few rows a segment (mx4_few.cu), with its workspace.
-int mx4_tile_rows(int rows, int num_segments, int max_rows);  // of the few-rows kernels; 0: the pair kernels
+// The kernel for rows in segments of at most max_rows, and the height of its scale tiles.
+int mx4_choose(int rows, int num_segments, int max_rows, int* tile_rows);
 int mx4_few_counters();
 size_t mx4_few_partial_bytes(bool gated);
 int launch_mx4_linear_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, const void* w_codes,

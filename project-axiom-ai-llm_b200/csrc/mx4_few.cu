@@ -24,8 +24,6 @@
 //
 // The weights do not depend on the kernel before: the producer asks for its first stages' weights
 // before it waits for that kernel (programmatic dependent launch), then for the activations.
-#include <cstdlib>
-
 #include "gemm_2sm.cuh"
 #include "microscale.cuh"
 
@@ -621,19 +619,27 @@ int launch_few_n(const Mx4Rows& r, const void* a_codes, const void* a_scales, co
 
 }  // namespace
 
-// Below about 96 rows a segment on average the weights' way in decides, and the few-rows kernels
-// are ahead (64 experts 2048 x 1408, top 6: 515 tokens 85 us against 110, 1030 tokens 109 against 122; 8
-// experts 4096 x 14336, top 2: 256 tokens 163 against 183, 512 tokens 234 against 191).
-// Their row tiles are as wide as a segment has rows at most, or on average with room to spare: a wider
-// tile costs epilogue and tensor time, a narrower one reads the weights again (from L2) for
-// every further tile.
-int mx4_tile_rows(int rows, int num_segments, int max_rows) {
-  static const int most = getenv("AXM_MX4_FEW") ? atoi(getenv("AXM_MX4_FEW")) : 96;
-  if (rows > (long long)most * num_segments) return 0;
+// What decides is the rows a segment has on average.  Few-rows kernels, one CTA a tile, pairs, in us
+// (experts of a top-k layer; one matrix):
+//   64 experts 2048 x 1408, top 6   64 tokens (6 rows)   60   65   97      256 (24)   66   68  100
+//                                  515 (48)              82   73  105     1030 (97)   87   82  110   2060 (193)  148  133  122
+//   8 experts 4096 x 14336, top 2  128 (32)             133  140  180      256 (64)  164  145  195    512 (128)  234  202  199
+//   one matrix 4096 -> 14336        64                   12   14   15      128        14   16   17    256         20   17   18
+//              14336 -> 4096        64                   20   29   28 (few column tiles: the few-rows kernels cut the reduction)
+// The few-rows kernels' row tiles are as wide as a segment has rows at most, or on average with room to
+// spare: a wider tile costs epilogue and tensor time, a narrower one reads the weights again (from
+// L2) for every further tile.
+int mx4_choose(int rows, int num_segments, int max_rows, int* tile_rows) {
   const int average = (rows + num_segments - 1) / num_segments;
+  *tile_rows = 128;
+  if (average > 128) return kMx4Pair;
+  if (num_segments > 1 && average > 40) return kMx4Single;
   for (int n = 16; n <= 64; n *= 2)
-    if ((max_rows <= n || average <= n * 3 / 4) && rows / n + num_segments <= mx4_row_tiles_most(rows, num_segments)) return n;
-  return 128;
+    if ((max_rows <= n || average <= n * 3 / 4) && rows / n + num_segments <= mx4_row_tiles_most(rows, num_segments)) {
+      *tile_rows = n;
+      break;
+    }
+  return kMx4Few;
 }
 
 int mx4_few_counters() { return few_enough(16); }

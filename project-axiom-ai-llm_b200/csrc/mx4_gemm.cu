@@ -442,6 +442,244 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
   }
 }
 
+// ---- the same tile on one CTA -----------------------------------------------------------------
+// For segments of up to about a hundred rows, whose time is the weights' way in: a pair's second CTA would
+// have no rows of its own there.  M = 128 rows, N = 256 weight rows, all of them staged by the CTA
+// itself: 51 KB a stage, four stages.  The first ring of weights is asked for before the kernel
+// before this one has finished (the weights do not depend on it).
+constexpr int kStages1 = 4;
+constexpr int kStageCodes1 = 3 * kCodeBytes;
+constexpr int kStageScales1 = kScaleABytes + kScaleBBytes;
+constexpr int kStageBytes1 = kStageCodes1 + kStageScales1;
+static_assert(kStages1 <= kStages4, "the control block is the pair kernel's");
+constexpr size_t kMx4SmemBytes1 = 1024 + (size_t)kStages1 * kStageBytes1 + sizeof(Mx4Shared);
+static_assert(kMx4SmemBytes1 <= 227u * 1024u, "shared memory of the 4-bit one-CTA kernel");
+
+constexpr uint32_t mx4_instr_desc1(uint32_t step) {  // M = 128 of one CTA
+  return (mx4_instr_desc(step) & ~(0x1fu << 24)) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma1_mx4(uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                            uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_cp1_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Units: expert group by expert group, column tile by column tile, row tiles innermost.
+__device__ __forceinline__ Unit4 decode1(const Mx4Shared* sh, int n_tiles, int unit) {
+  int lo = 0, hi = sh->num_groups - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (sh->tile_prefix[sh->group_first[mid]] * n_tiles <= unit) lo = mid; else hi = mid - 1;
+  }
+  const int s0 = sh->group_first[lo], s1 = sh->group_first[lo + 1];
+  const int base = sh->tile_prefix[s0];
+  const int mt = sh->tile_prefix[s1] - base;
+  const int local = unit - base * n_tiles;
+  Unit4 u;
+  u.seg0 = s0;
+  u.live = true;
+  u.n_tile = local / mt;
+  const int idx = base + local - u.n_tile * mt;
+  int a = s0, b = s1 - 1;
+  while (a < b) {
+    const int mid = (a + b + 1) >> 1;
+    if (sh->tile_prefix[mid] <= idx) a = mid; else b = mid - 1;
+  }
+  u.seg = a;
+  u.m_tile = idx - sh->tile_prefix[a];
+  return u;
+}
+
+template <int kMode>
+__global__ void __launch_bounds__(kThreads4, 1)
+mx4_gemm_single_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a_sf,
+                       const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1,
+                       const __grid_constant__ CUtensorMap tm_b0_sf, const __grid_constant__ CUtensorMap tm_b1_sf,
+                       Mx4Args args) {
+  constexpr bool kGated = kMode == kModeGated;
+  constexpr int kCols = kGated ? 128 : 256;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* tiles = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  unsigned char* scales_s = tiles + (size_t)kStages1 * kStageCodes1;
+  Mx4Shared* sh = reinterpret_cast<Mx4Shared*>(scales_s + (size_t)kStages1 * kStageScales1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int n_tiles = (args.n_total + kCols - 1) / kCols;
+  const int k_blocks = (args.k_total + kKStage - 1) / kKStage;
+  const int nseg = args.num_segments;
+
+  launch_dependents();
+  // the segment table is older than the kernel before this one, which has waited for everything before
+  // itself
+  for (int s = threadIdx.x; s < nseg; s += kThreads4)
+    sh->seg[s] = args.segments != nullptr ? args.segments[s] : AxmSegment{0, 0, args.rows_total, 0};
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < kStages1; ++i) {
+      mbar_init(&sh->full[i], 1);
+      mbar_init(&sh->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&sh->tmem_full[i], 1);
+    mbar_init(&sh->overlap_free, 4);
+    sh->abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_b0);
+    tma_prefetch_desc(&tm_b0_sf);
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_a_sf);
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc(&sh->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  if (warp == 0) count_tiles(sh, nseg, n_tiles);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  const int total_units = sh->tile_prefix[nseg] * n_tiles;
+  const uint32_t tmem_base = sh->tmem_base;
+  volatile int* abort_flag = &sh->abort_flag;
+  const int first = blockIdx.x, step = gridDim.x;
+
+  if (warp == 0) {
+    // ---- TMA producer --------------------------------------------------------------------
+    if (lane == 0) {
+      auto weights = [&](int stage, const Unit4& u, int kb) {
+        const int e = (sh->seg[u.seg0].expert & 0xffff) - args.expert_base;
+        unsigned char* sb = tiles + (size_t)stage * kStageCodes1 + kCodeBytes;
+        unsigned char* sf = scales_s + (size_t)stage * kStageScales1 + kScaleABytes;
+        uint64_t* bar = &sh->full[stage];
+        const int row = u.n_tile * kCols, tile = e * args.wn_tiles + (kGated ? u.n_tile : 2 * u.n_tile);
+        mbar_expect_tx(bar, kStageBytes1);
+        tma_load_3d(sb, &tm_b0, bar, kb * (kKStage / 2), row, e);
+        tma_load_3d(sb + kCodeBytes, kGated ? &tm_b1 : &tm_b0, bar, kb * (kKStage / 2), kGated ? row : row + 128, e);
+        tma_load_3d(sf, &tm_b0_sf, bar, 0, kb * 2, tile);
+        // (linear: behind an odd number of tiles the next expert's bytes or the fill value; they scale
+        // columns that are not stored)
+        tma_load_3d(sf + 1024, kGated ? &tm_b1_sf : &tm_b0_sf, bar, 0, kb * 2, kGated ? tile : tile + 1);
+      };
+      auto rows = [&](int stage, const Unit4& u, int kb) {
+        const AxmSegment sg = sh->seg[u.seg];
+        uint64_t* bar = &sh->full[stage];
+        tma_load_3d(tiles + (size_t)stage * kStageCodes1, &tm_a, bar, kb * (kKStage / 2), sg.out_row0 + u.m_tile * 128, 0);
+        tma_load_3d(scales_s + (size_t)stage * kStageScales1, &tm_a_sf, bar, 0, kb * 2,
+                    sg.out_row0 / 128 + args.seg_base + u.seg + u.m_tile);
+      };
+      // the first ring: weights, then, once the kernel before is done, the rows
+      int ahead = 0;
+      for (int unit = first; ahead < kStages1 && unit < total_units; unit += step) {
+        const Unit4 u = decode1(sh, n_tiles, unit);
+        for (int kb = 0; kb < k_blocks && ahead < kStages1; ++kb, ++ahead) weights(ahead, u, kb);
+      }
+      wait_for_previous();
+      int at = 0, stage = 0;  // stages of the first ring that have their rows
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int unit = first; ok && unit < total_units; unit += step) {
+        const Unit4 u = decode1(sh, n_tiles, unit);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (at < ahead) {
+            ++at;
+          } else {
+            if (!mbar_wait(&sh->empty[stage], phase ^ 1u, abort_flag)) {
+              ok = false;
+              break;
+            }
+            weights(stage, u, kb);
+          }
+          rows(stage, u, kb);
+          if (++stage == kStages1) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer (the whole warp, one elected lane issues) -----------------------------------
+    const uint64_t codes0 = make_smem_desc(smem_u32(tiles), 16, 1024);
+    const uint64_t scales0 = scale_desc(smem_u32(scales_s));
+    int stage = 0;
+    uint32_t phase = 0;
+    int tile = 0;
+    bool ok = true;
+    for (int unit = first; ok && unit < total_units; unit += step, ++tile) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&sh->overlap_free, (uint32_t)(tile & 1) ^ 1u, abort_flag))) break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + ((tile & 1) ? kAcc1 : 0u);
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh->full[stage], phase, abort_flag))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t da = codes0 + (uint64_t)(stage * (kStageCodes1 / 16));
+        const uint64_t db = da + kCodeBytes / 16;
+        const uint64_t sf = scales0 + (uint64_t)(stage * (kStageScales1 / 16));
+        if (elect_one()) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            tc_cp1_scales(tmem_base + kSfA + 4 * c, sf + 32 * c);
+            tc_cp1_scales(tmem_base + kSfB + 8 * c, sf + kScaleABytes / 16 + 32 * c);
+            tc_cp1_scales(tmem_base + kSfB + 8 * c + 4, sf + (kScaleABytes + 1024) / 16 + 32 * c);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            tc_mma1_mx4(d_tmem, da + (uint64_t)(j * 2), db + (uint64_t)(j * 2), mx4_instr_desc1(j & 1),
+                        tmem_base + kSfA + 4 * (j >> 1), tmem_base + kSfB + 8 * (j >> 1), (kb > 0 || j > 0) ? 1u : 0u);
+          tc_commit(&sh->empty[stage]);
+        }
+        __syncwarp();
+        if (++stage == kStages1) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      if (elect_one()) tc_commit(&sh->tmem_full[tile & 1]);
+      __syncwarp();
+    }
+  } else {
+    // ---- epilogue --------------------------------------------------------------------------------
+    wait_for_previous();  // outputs and scratch of the kernels before
+    int tile = 0;
+    for (int unit = first; unit < total_units; unit += step, ++tile) {
+      const Unit4 u = decode1(sh, n_tiles, unit);
+      if (!__all_sync(0xffffffffu, mbar_wait(&sh->tmem_full[tile & 1], (uint32_t)((tile >> 1) & 1), abort_flag))) break;
+      tc_fence_after();
+      drain_tile<kMode>(args, u, sh->seg[u.seg], tmem_base, tile & 1, n_tiles, [&] { mbar_arrive(&sh->overlap_free); });
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (sh->abort_flag != 0) {
+    long long t0 = clock64();
+    while (clock64() - t0 < 4000000LL) {
+    }
+    if (threadIdx.x == 0 && args.status != nullptr) atomicExch(args.status, kGated ? 15 : 16);
+  }
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
 // ---- host side -----------------------------------------------------------------------------
 
 // Codes: rows of k / 2 bytes, a box of 128 bytes x 128 rows, 128-byte swizzle.
@@ -460,9 +698,16 @@ int map_scales(CUtensorMap* m, const void* base, uint64_t tiles, int k) {
 }
 
 template <int kMode>
-int launch_pair(const CUtensorMap& a, const CUtensorMap& a_sf, const CUtensorMap& b0, const CUtensorMap& b1,
-                const CUtensorMap& b0_sf, const CUtensorMap& b1_sf, const Mx4Args& args, cudaStream_t st) {
-  static SmemLimitCache smem = {};
+int launch_tiles(const CUtensorMap& a, const CUtensorMap& a_sf, const CUtensorMap& b0, const CUtensorMap& b1,
+                const CUtensorMap& b0_sf, const CUtensorMap& b1_sf, const Mx4Args& args, bool single, cudaStream_t st) {
+  static SmemLimitCache smem = {}, smem1 = {};
+  if (single) {
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(mx4_gemm_single_kernel<kMode>), kMx4SmemBytes1, &smem1,
+                                     "mx4_gemm_single_kernel"))
+      return rc;
+    return launch_overlapping("mx4_gemm_single_kernel", mx4_gemm_single_kernel<kMode>, sm_count(), kThreads4, kMx4SmemBytes1,
+                              st, a, a_sf, b0, b1, b0_sf, b1_sf, args);
+  }
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(mx4_gemm_pair_kernel<kMode>), kMx4SmemBytes, &smem,
                                    "mx4_gemm_pair_kernel"))
     return rc;
@@ -502,7 +747,7 @@ int launch_mx4_linear(const Mx4Rows& r, const void* a_codes, const void* a_scale
   ga.out_bf16 = out_bf16 ? 1 : 0;
   ga.wn_tiles = wn;
   ga.out = out;
-  return launch_pair<kModeLinear>(a, a_sf, b, b, b_sf, b_sf, ga, st);
+  return launch_tiles<kModeLinear>(a, a_sf, b, b, b_sf, b_sf, ga, r.kernel == kMx4Single, st);
 }
 
 int launch_mx4_gated(const Mx4Rows& r, const void* a_codes, const void* a_scales, const AxmMx4Experts* w, int experts,
@@ -522,7 +767,7 @@ int launch_mx4_gated(const Mx4Rows& r, const void* a_codes, const void* a_scales
   ga.wn_tiles = wn;
   ga.out = h_codes;
   ga.out_scales = static_cast<uint8_t*>(h_scales);
-  return launch_pair<kModeGated>(a, a_sf, g, u, g_sf, u_sf, ga, st);
+  return launch_tiles<kModeGated>(a, a_sf, g, u, g_sf, u_sf, ga, r.kernel == kMx4Single, st);
 }
 
 }  // namespace axm

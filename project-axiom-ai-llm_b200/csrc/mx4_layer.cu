@@ -103,7 +103,7 @@ FfnWs carve_expert_ffn(const AxmMoeDesc* d, int rows, int num_segments, void* ba
 // Both products of the feed-forward over one range of the table.
 int launch_ffn(const Mx4Rows& r, const FfnWs& w, const AxmMx4Experts* experts, int num_experts, int d, int f, void* o,
                bool o_bf16, cudaStream_t st) {
-  if (r.few) {
+  if (r.kernel == kMx4Few) {
     if (int rc = launch_mx4_gated_few(r, w.x_codes, w.x_scales, experts, num_experts, d, f, w.h_codes, w.h_scales, st)) return rc;
     return launch_mx4_linear_few(r, w.h_codes, w.h_scales, experts->down_codes, experts->down_scales, num_experts, f, d, o,
                                  o_bf16, st);
@@ -188,12 +188,13 @@ extern "C" int axm_mx4_linear(const void* x, int32_t x_dtype, int64_t ld, int32_
   if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
   if (int rc = require_device()) return rc;
   const LinearWs w = carve_linear(tokens, k, workspace);
-  const int tile = mx4_tile_rows(tokens, 1, tokens);
-  const Mx4Rows rows = {nullptr, 1, tokens, 1, 0, 0, tile ? tile : 128, tile != 0, w.status, w.few.partial, w.few.counters};
+  int tile;
+  const int kernel = mx4_choose(tokens, 1, tokens, &tile);
+  const Mx4Rows rows = {nullptr, 1, tokens, 1, 0, 0, tile, kernel, w.status, w.few.partial, w.few.counters};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Mx4Gather from = {nullptr, 1, tokens, 1};
   if (int rc = launch_mx4_quantize_rows(x, x_dtype, ld, from, rows, k, w.codes, w.scales, st)) return rc;
-  return (rows.few ? launch_mx4_linear_few : launch_mx4_linear)(rows, w.codes, w.scales, w_codes, w_scales, 1, k,
+  return (kernel == kMx4Few ? launch_mx4_linear_few : launch_mx4_linear)(rows, w.codes, w.scales, w_codes, w_scales, 1, k,
                                                                            n, out, out_dtype == AXM_DTYPE_BF16, st);
 }
 
@@ -225,8 +226,9 @@ extern "C" int axm_mx4_expert_ffn(const AxmMoeDesc* desc, const void* x, int32_t
   if (int rc = require_device()) return rc;
   const int D = desc->d_model, F = desc->d_ff;
   const FfnWs w = carve_expert_ffn(desc, rows, num_segments, workspace);
-  const int tile = mx4_tile_rows(rows, num_segments, desc->tokens);
-  const Mx4Rows r = {segments, num_segments, rows, num_segments, 0, 0, tile ? tile : 128, tile != 0, w.status, w.few.partial, w.few.counters};
+  int tile;
+  const int kernel = mx4_choose(rows, num_segments, desc->tokens, &tile);
+  const Mx4Rows r = {segments, num_segments, rows, num_segments, 0, 0, tile, kernel, w.status, w.few.partial, w.few.counters};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Mx4Gather from = {nullptr, 1, rows, 1};
   if (int rc = launch_mx4_quantize_rows(x, AXM_DTYPE_BF16, D, from, r, D, w.x_codes, w.x_scales, st)) return rc;
@@ -274,8 +276,9 @@ extern "C" int axm_moe_forward_mx4(const AxmMoeDesc* desc, const AxmMoeTensors* 
     return rc;
   const int rows = T * (k + S);
   // one kind of kernel and of scale tile for the whole table: the routed experts'
-  const int tile = mx4_tile_rows(rows, E + S, T);
-  Mx4Rows r = {w.segments, E + S, rows, E + S, 0, 0, tile ? tile : 128, tile != 0, nullptr, w.ffn.few.partial, w.ffn.few.counters};
+  int tile;
+  const int kernel = mx4_choose(rows, E + S, T, &tile);
+  Mx4Rows r = {w.segments, E + S, rows, E + S, 0, 0, tile, kernel, nullptr, w.ffn.few.partial, w.ffn.few.counters};
   const Mx4Gather from = {row_src, k, T * k, T};
   if ((rc = launch_mx4_quantize_rows(t->x, AXM_DTYPE_BF16, D, from, r, D, w.ffn.x_codes, w.ffn.x_scales, st))) return rc;
   r.status = w.ffn.status;
