@@ -71,6 +71,7 @@ struct FewArgs {
   int num_segments;
   int rows_total;
   int seg_base;
+  int experts;
   int expert_base;
   int n_total;
   int k_total;
@@ -179,7 +180,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
   // The segment table is older than the kernel before this one (see the launch), so it may be read
   // at once.
   for (int s = threadIdx.x; s < nseg; s += kThreadsF)
-    sh->seg[s] = args.segments != nullptr ? args.segments[s] : AxmSegment{0, 0, args.rows_total, 0};
+    sh->seg[s] = product_segment(args.segments, s, args.rows_total, args.expert_base, args.experts);
   if (threadIdx.x == 32) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sh->full[i], 1);
@@ -584,6 +585,7 @@ int launch_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, cons
   ga.num_segments = r.segments != nullptr ? r.num_segments : 1;
   ga.rows_total = r.rows;
   ga.seg_base = r.seg_base;
+  ga.experts = experts;
   ga.expert_base = r.expert_base;
   ga.status = r.status;
   ga.n_total = n;

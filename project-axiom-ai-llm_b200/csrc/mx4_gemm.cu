@@ -70,8 +70,9 @@ struct Mx4Args {
   int num_segments;
   int n_total;       // Linear: columns of out; Gated: columns of h
   int k_total;
-  int rows_total;    // without a segment table: the rows of the one segment, expert 0
+  int rows_total;    // of the operand and of the output; without a segment table: of the one segment
   int seg_base;      // index of segments[0] in the layer's whole table (scale tiles count from there)
+  int experts;
   int expert_base;   // expert id of the first weight matrix
   int out_bf16;      // Linear
   int wn_tiles;      // 128-row tiles of one expert's weights
@@ -276,7 +277,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
   const int nseg = args.num_segments;
 
   for (int s = threadIdx.x; s < nseg; s += kThreads4)
-    sh->seg[s] = args.segments != nullptr ? args.segments[s] : AxmSegment{0, 0, args.rows_total, 0};
+    sh->seg[s] = product_segment(args.segments, s, args.rows_total, args.expert_base, args.experts);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages4; ++i) {
       mbar_init(&sh->full[i], 1);
@@ -523,7 +524,7 @@ mx4_gemm_single_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_co
   // the segment table is older than the kernel before this one, which has waited for everything before
   // itself
   for (int s = threadIdx.x; s < nseg; s += kThreads4)
-    sh->seg[s] = args.segments != nullptr ? args.segments[s] : AxmSegment{0, 0, args.rows_total, 0};
+    sh->seg[s] = product_segment(args.segments, s, args.rows_total, args.expert_base, args.experts);
   if (threadIdx.x == 32) {
     for (int i = 0; i < kStages1; ++i) {
       mbar_init(&sh->full[i], 1);
@@ -742,6 +743,7 @@ int launch_mx4_linear(const Mx4Rows& r, const void* a_codes, const void* a_scale
   if ((rc = map_codes(&b, w_codes, experts, n, k))) return rc;
   if ((rc = map_scales(&b_sf, w_scales, (uint64_t)experts * wn, k))) return rc;
   Mx4Args ga = mx4_args(r);
+  ga.experts = experts;
   ga.n_total = n;
   ga.k_total = k;
   ga.out_bf16 = out_bf16 ? 1 : 0;
@@ -762,6 +764,7 @@ int launch_mx4_gated(const Mx4Rows& r, const void* a_codes, const void* a_scales
   if ((rc = map_scales(&g_sf, w->gate_scales, (uint64_t)experts * wn, d))) return rc;
   if ((rc = map_scales(&u_sf, w->up_scales, (uint64_t)experts * wn, d))) return rc;
   Mx4Args ga = mx4_args(r);
+  ga.experts = experts;
   ga.n_total = f;
   ga.k_total = d;
   ga.wn_tiles = wn;
