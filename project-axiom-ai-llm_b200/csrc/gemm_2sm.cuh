@@ -1,8 +1,7 @@
 // Pieces shared by the kernels that run on CTA pairs (thread-block clusters of two,
 // tcgen05.mma.cta_group::2): stage geometry, the shared-memory control block and the PTX
-// wrappers.  No cluster multicast: every CTA issues its own TMA loads, and the leader
-// signals the peer's barriers with ordinary tcgen05.commit instructions addressed to the
-// peer's shared memory.
+// wrappers.  No load is multicast: every CTA issues its own TMA loads.  The leader signals both
+// CTAs' barriers with one tcgen05.commit (the commit's own multicast mask, tc_commit2_both).
 #pragma once
 
 #include "gemm_common.cuh"

@@ -3,9 +3,8 @@
 // own 128 activation rows and only HALF of the weight tile (128 of the 256 columns);
 // the tensor core of the leader CTA reads both halves, so the shared-memory fill per
 // FLOP drops from 48 KB to 32 KB per k-block and the pipeline gets six stages.
-// No cluster multicast is used anywhere: every CTA issues its own TMA loads, and the
-// leader signals the peer's barriers with ordinary (non-multicast) tcgen05.commit
-// instructions addressed to the peer's shared memory.
+// No load is multicast: every CTA issues its own TMA loads.  The leader signals both CTAs'
+// barriers with one tcgen05.commit.
 //
 // Same operator as grouped_ffn.cu (core/src/CUDA/kernel/moe_router.cu:155-190 of the
 // reference engine); same weight layouts consumed as stored (MN-major B operand).

@@ -24,6 +24,8 @@
 //
 // The weights do not depend on the kernel before: the producer asks for its first stages' weights
 // before it waits for that kernel (programmatic dependent launch), then for the activations.
+// Measured: one token 4096 -> 14336 10.9 us with its quantisation; one token through two experts 4096 x 14336
+// gated 26.5 us (125 MB), linear 23.0 us (62 MB), overlapping by 8; 16 tokens in all 126 us (742 MB, 5.9 TB/s).
 #include "gemm_2sm.cuh"
 #include "microscale.cuh"
 

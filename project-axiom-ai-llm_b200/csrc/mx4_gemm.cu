@@ -25,6 +25,10 @@
 // The accumulators overlap: the first is columns 0..255, the second 232..487, scales 488..511.
 // The epilogue takes the 32-column blocks that hold the shared columns first and then lets the
 // next tile's MMAs start; everything else of it runs under them.
+//
+// Measured: 8192 rows 4096 -> 14336 185 us (5.2 PFLOP/s) in a short run, 8 experts 4096 x 14336 over 16384 rows
+// gated 720 us, linear 344 us (5.4 and 5.6 PFLOP/s); back to back the power cap holds them to 4.0-4.8.  A stage took
+// 630 cycles where its MMAs take 511 (8192 rows, 14336 -> 4096).
 #include <mutex>
 
 #include "gemm_2sm.cuh"
