@@ -85,7 +85,7 @@ mx_quantize_rows_kernel(const T* __restrict__ x, long long ld, Mx4Gather from, i
   for (long long row_at = (long long)blockIdx.x * rows_per_cta + ((warp >> log_wpr) << log_rpw); row_at < rows;
        row_at += (long long)gridDim.x * rows_per_cta) {
     const int row = (int)row_at + group;
-    const bool there = row < rows;
+    const bool there = row_at + group < rows;
     long long src = there ? row : -1;
     if (there && row >= from.tail_row0) {
       src = (row - from.tail_row0) % from.tail_mod;
@@ -201,7 +201,7 @@ mx_dequantize_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __re
   for (long long row_at = (long long)blockIdx.x * rows_per_cta + ((warp >> log_wpr) << log_rpw); row_at < rows;
        row_at += (long long)gridDim.x * rows_per_cta) {
     const int row = (int)row_at + group;
-    bool there = row < rows;
+    bool there = row_at + group < rows;
     const uint8_t* in = codes + (size_t)row * (kBits == 4 ? k >> 1 : k);
     const uint8_t* sc = scales;
     T* to = out + (size_t)row * ld;

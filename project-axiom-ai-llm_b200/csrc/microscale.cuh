@@ -201,7 +201,8 @@ __device__ __forceinline__ RowSegment segment_of_row(const AxmSegment* segments,
     rows = __shfl_sync(0xffffffffu, e.z, at);
     if (at < 31) break;
   }
-  if (row - r.first >= rows) r.seg = -1;
+  // (a start before the first row would count tiles that the scale buffer does not have)
+  if (r.first < 0 || row - r.first >= rows) r.seg = -1;
   return r;
 }
 

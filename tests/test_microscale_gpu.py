@@ -652,3 +652,20 @@ def test_training_step_of_the_layer(ms, axm, cuda_device, t, d, f, e, k, shared)
     b.backward(y, d_out)
     a.backward(x, d_out)
     assert torch.equal(a.out, out8) and torch.equal(a.d_x, got["d_x"]) and torch.equal(a.d_w_down, got["d_w_down"])
+
+
+def test_rows_of_a_segment_that_starts_before_the_first(ms, axm, cuda_device):
+    """Such a segment has no tiles: its rows get codes and no scale bytes, nothing is written behind the
+    scale buffer (one tile, 1024 bytes; row 1 of this one would be in its second tile), and reading leaves them as they are."""
+    x = torch.randn(2, 64, device=cuda_device).to(BF16)
+    segs = torch.tensor([(-127, -127, 129, 0)], dtype=torch.int32, device=cuda_device)
+    scales = torch.full((4 * 1024,), 77, dtype=torch.uint8, device=cuda_device)
+    codes = torch.empty(2, 32, dtype=torch.uint8, device=cuda_device)
+    lib, stream = axm.load(), axm.current_stream()
+    axm.check(lib.axm_mx4_quantize_rows(x.data_ptr(), axm.DTYPE_BF16, 64, None, 1, 2, 64, segs.data_ptr(), 1,
+                                        codes.data_ptr(), scales.data_ptr(), stream))
+    assert (scales == 77).all()
+    out = torch.full((2, 64), 3.0, dtype=BF16, device=cuda_device)
+    axm.check(lib.axm_mx4_dequantize_rows(codes.data_ptr(), scales.data_ptr(), 2, 64, segs.data_ptr(), 1, out.data_ptr(),
+                                          axm.DTYPE_BF16, 64, stream))
+    assert (out == 3).all()
