@@ -693,10 +693,11 @@ typedef struct AxmMx4Experts {
 } AxmMx4Experts;
 
 /* The expert feed-forward from 4-bit weights: o = q4(silu(g) u) . Wd[e]^T,
- * g = q4(x) . Wg[e]^T, u = q4(x) . Wu[e]^T over the rows of each segment (a_row0 == out_row0;
- * desc->tokens, the most rows a segment is expected to have, only guides the choice of kernel).  x [rows][D] bf16, o [rows][D] bf16 or fp32; rows outside every
- * segment of o are left as they are.  desc gives tokens, d_model and d_ff (multiples of 32) and
- * num_experts.  Workspace as for axm_mx4_linear. */
+ * g = q4(x) . Wg[e]^T, u = q4(x) . Wu[e]^T over the rows of each segment (a_row0 == out_row0).
+ * x [rows][D] bf16, o [rows][D] bf16 or fp32; rows outside every segment of o are left as they
+ * are.  desc gives d_model and d_ff (multiples of 32), num_experts, and in tokens the most rows a
+ * segment is expected to have (it only guides the choice of kernel; 0: not known).
+ * Workspace as for axm_mx4_linear. */
 AXM_API int axm_mx4_expert_ffn_workspace_bytes(const AxmMoeDesc* desc, int32_t rows, int32_t num_segments,
                                                size_t* bytes);
 AXM_API int axm_mx4_expert_ffn(const AxmMoeDesc* desc, const void* x, int32_t rows,

@@ -222,7 +222,6 @@ extern "C" int axm_mx4_expert_ffn(const AxmMoeDesc* desc, const void* x, int32_t
   if (o_dtype != AXM_DTYPE_BF16 && o_dtype != AXM_DTYPE_FP32) return fail(AXM_ERR_ARGUMENT, "%s: o_dtype %d unknown", what, o_dtype);
   if (off16(x) || off16(o)) return fail(AXM_ERR_ARGUMENT, "%s: x and o must be 16-byte aligned", what);
   if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
-  if (desc->tokens == 0) return AXM_OK;
   if (int rc = require_device()) return rc;
   const int D = desc->d_model, F = desc->d_ff;
   const FfnWs w = carve_expert_ffn(desc, rows, num_segments, workspace);

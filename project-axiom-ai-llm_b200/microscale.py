@@ -255,7 +255,8 @@ def _expert_table(gate, up, down):
 
 class Mx4ExpertFfn(_Workspace):
     """The expert feed-forward from 4-bit weights over up to `rows` rows in up to `segments`
-    segments (default: one per expert) of at most `tokens` rows each."""
+    segments (default: one per expert); `tokens`, the most rows a segment is expected to have, guides the
+    choice of kernel."""
 
     def __init__(self, gate, up, down, rows, tokens, segments=None):
         self.lib = _pkg.load()

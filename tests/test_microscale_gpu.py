@@ -669,3 +669,20 @@ def test_rows_of_a_segment_that_starts_before_the_first(ms, axm, cuda_device):
     axm.check(lib.axm_mx4_dequantize_rows(codes.data_ptr(), scales.data_ptr(), 2, 64, segs.data_ptr(), 1, out.data_ptr(),
                                           axm.DTYPE_BF16, 64, stream))
     assert (out == 3).all()
+
+
+@pytest.mark.parametrize("counts", [[50, 3, 0, 17], [200, 1, 2, 5, 0, 9, 3, 4], [130, 140, 150, 160]])
+def test_expert_ffn_with_more_rows_than_expected(ms, cuda_device, counts):
+    """tokens only guides the choice of kernel: 0 and 1 give what the true number gives, but for sums in
+    another order and the single roundings of h that fall the other way (as in the test above)."""
+    e, d, f = len(counts), 64, 96
+    q = [ms.quantize_weights(torch.randn(e, k, n, device=cuda_device) * 0.2) for k, n in ((d, f), (d, f), (f, d))]
+    segs, rows = table(counts, cuda_device)
+    x = torch.randn(rows, d, device=cuda_device).to(BF16)
+    out = []
+    for tokens in (rows, 1, 0):
+        plan = ms.Mx4ExpertFfn(*q, rows=rows, tokens=tokens)
+        out.append(plan.forward(x, segs, out=torch.full((rows, d), float("nan"), device=cuda_device)))
+        assert plan.status() == 0
+    for o in out[1:]:
+        assert (o - out[0]).norm() <= 0.01 * out[0].norm()
