@@ -67,7 +67,8 @@ enum {
   /* Training step on one GPU: what the backward pass needs of the forward pass is kept in 8 bits
    * (the gate's and the up projection's outputs and the expert rows; the format of axm_mx8_*), the
    * rest is rebuilt: 2 F + D bytes a row and 3 % where the plain form keeps 6 F + 6 D.  Gradients are
-   * those of the kept values.  d_model and d_ff must be multiples of 32. */
+   * those of the kept values.  x has to hold the same values in both calls.  d_model and d_ff must be
+   * multiples of 32; the sharded training step refuses the flag. */
   AXM_FLAG_SAVE_8BIT = 8
 };
 
@@ -646,7 +647,8 @@ AXM_API int axm_mx4_weights_bytes(int32_t experts, int32_t k, int32_t n, size_t*
 
 /* Rows of a matrix (row stride ld elements: a multiple of 16 bytes) to 4 bits.  Row r is read
  * from source row row_src[r] / row_div (row_src NULL: r; row_src[r] < 0: zeros), so that the
- * layer's permutation can be applied on the way (axm_moe_permute's row_src with row_div = k).
+ * layer's permutation can be applied on the way (axm_moe_permute's row_src with row_div = k); the
+ * source rows it names must exist.
  * segments NULL: all rows form one segment; rows outside every segment get no scale bytes. */
 AXM_API int axm_mx4_quantize_rows(const void* x, int32_t x_dtype, int64_t ld, const int32_t* row_src,
                                   int32_t row_div, int32_t rows, int32_t k, const AxmSegment* segments,
@@ -736,7 +738,8 @@ AXM_API int axm_mx8_checkpoint_bytes(int32_t rows, int32_t d_ff, size_t* code_by
  * Gradients are bf16 or fp32 (grad_dtype, all of them alike), in the layouts of what they belong to;
  * the three weight gradients may all be NULL.  h, d_g, d_u [rows][F] bf16 are scratch of the call.
  * Tables as for axm_moe_expert_ffn_backward: a_row0 == out_row0, every expert once, segments
- * padded to multiples of 64 rows with zero rows of x and d_o.  d_ff is a multiple of 32, d_model of 8.
+ * padded to multiples of 64 rows with zero rows of x and d_o (the gradients of experts that a
+ * table leaves out, and of all with num_segments 0, are not written).  d_ff is a multiple of 32, d_model of 8.
  * status: an optional int32 device word that receives a non-zero code when a bounded wait gave up. */
 AXM_API int axm_mx8_expert_ffn_train(const AxmMoeDesc* desc, const void* x, int32_t rows,
                                      const AxmSegment* segments, int32_t num_segments, const void* w_gate,

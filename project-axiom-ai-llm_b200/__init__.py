@@ -375,8 +375,10 @@ class MoeTrainLayer:
         self.desc = make_desc(tokens, D, F, E, top_k, S, rdt, FLAG_RESIDUAL | (FLAG_SAVE_8BIT if save_8bit else 0))
         dev = torch.device(device)
         kept, shared = train_split_bytes(self.desc)
-        if scratch is not None and scratch.numel() < shared:
-            raise ValueError(f"scratch has {scratch.numel()} bytes, {shared} are needed")
+        if scratch is not None and (scratch.dtype != torch.uint8 or scratch.numel() < shared or not scratch.is_contiguous() or
+                                    scratch.device.type != dev.type):
+            raise ValueError(f"scratch: {shared} contiguous bytes on {dev} are needed, not {scratch.numel()} of "
+                             f"{scratch.dtype} on {scratch.device}")
         self.scratch = scratch
         self.workspace = torch.empty(kept + shared if scratch is None else kept, dtype=torch.uint8, device=dev)
         f32 = torch.float32

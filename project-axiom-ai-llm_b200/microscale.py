@@ -53,6 +53,23 @@ def _rows_of(x):
     return rows, k, ld if rows > 1 else max(ld, k)
 
 
+def _check_index(t, width, device, what):
+    """An int32 device tensor as the kernels read it: [n], or [n][width].  (None: not given.)"""
+    if t is None:
+        return
+    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or \
+            (t.dim() != 1 if width is None else t.dim() != 2 or t.shape[1] != width):
+        raise ValueError(f"{what}: a contiguous int32 {'[n]' if width is None else f'[n][{width}]'} on {device} is needed, "
+                         f"not {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _check_out(out, shape, device, dtype=None):
+    if tuple(out.shape) != tuple(shape) or not out.is_contiguous() or out.device != device or \
+            (dtype is not None and out.dtype != dtype):
+        raise ValueError(f"out: a contiguous {'' if dtype is None else dtype} {tuple(shape)} on {device} is needed, "
+                         f"not {out.dtype} {tuple(out.shape)} on {out.device}")
+
+
 def _address(t):
     return None if t is None else t.data_ptr()
 
@@ -116,8 +133,10 @@ def quantize_rows(x, segments=None, row_src=None, row_div=1):
     rows, k, ld = _rows_of(x)
     nseg = 0
     if row_src is not None:
+        _check_index(row_src, None, x.device, "row_src")
         rows = row_src.numel()
     if segments is not None:
+        _check_index(segments, 4, x.device, "segments")
         nseg = segments.shape[0]
     # the sizes of axm_mx4_rows_bytes; sizes that it refuses are refused by the call below
     at = (rows * (k // 2) + 255) & -256
@@ -208,6 +227,7 @@ class _Workspace:
     def _scratch(self, size, device):
         self.device = device
         self.workspace = torch.empty(max(size, 256), dtype=torch.uint8, device=device)
+        self.workspace[:4].zero_()  # the status word, until the first call
 
     def status(self):
         """Reads the status word of the last call (synchronises): 0, or the code of a kernel whose
@@ -235,8 +255,8 @@ class Mx4Linear(_Workspace):
             raise ValueError(f"x {tuple(x.shape)} on {x.device}: up to {self.tokens} rows of {w.k} on {device}")
         if out is None:
             out = torch.empty((rows, w.n), dtype=dtype, device=device)
-        elif out.shape != (rows, w.n) or not out.is_contiguous() or out.device != device:
-            raise ValueError("out must be a contiguous [rows][N] matrix beside x")
+        else:
+            _check_out(out, (rows, w.n), device)
         status = self.lib.axm_mx4_linear(x.data_ptr(), _dtype(x.dtype), ld, rows, k, w.n, w.codes.data_ptr(),
                                          w.scales.data_ptr(), out.data_ptr(), _dtype(out.dtype),
                                          self.workspace.data_ptr(), self.workspace.numel(),
@@ -250,6 +270,9 @@ def _expert_table(gate, up, down):
     if (gate.experts, gate.k, gate.n) != (up.experts, up.k, up.n) or \
             (down.experts, down.k, down.n) != (gate.experts, gate.n, gate.k):
         raise ValueError("gate and up are [E][F][D/2], down is [E][D][F/2]")
+    for w in (up, down):
+        if w.device != gate.device:
+            raise ValueError(f"weights on {gate.device} and {w.device}: one device is needed")
     return _pkg.Mx4ExpertWeights(*(t.data_ptr() for w in (gate, up, down) for t in (w.codes, w.scales)))
 
 
@@ -276,13 +299,13 @@ class Mx4ExpertFfn(_Workspace):
         dev = self.device
         if rows > self.rows or d != self.desc.d_model or not x.is_contiguous() or x.dtype != torch.bfloat16 or x.device != dev:
             raise ValueError(f"x: up to {self.rows} contiguous bf16 rows of {self.desc.d_model} on {dev}")
-        if segments.dtype != torch.int32 or segments.shape[1:] != (4,) or not segments.is_contiguous() or \
-                segments.device != dev or segments.shape[0] > self.segments:
-            raise ValueError(f"segments: a contiguous int32 table of up to {self.segments} x 4 on {dev}")
+        _check_index(segments, 4, dev, "segments")
+        if segments.shape[0] > self.segments:
+            raise ValueError(f"segments: {segments.shape[0]}, up to {self.segments} were announced")
         if out is None:
             out = torch.empty(rows, d, dtype=dtype, device=dev)
-        elif out.shape != x.shape or not out.is_contiguous() or out.device != dev:
-            raise ValueError("out must be a contiguous matrix like x")
+        else:
+            _check_out(out, x.shape, dev)
         _pkg.check(self.lib.axm_mx4_expert_ffn(ctypes.byref(self.desc), x.data_ptr(), rows, segments.data_ptr(),
                                                segments.shape[0], ctypes.byref(self.table), out.data_ptr(),
                                                _dtype(out.dtype), self.workspace.data_ptr(), self.workspace.numel(),
@@ -303,6 +326,16 @@ class Mx4MoeLayer(_Workspace):
         if weights.get("shared_gate") is not None:
             self.shared = _expert_table(weights["shared_gate"], weights["shared_up"], weights["shared_down"])
             shared = weights["shared_gate"].experts
+            if (weights["shared_gate"].k, weights["shared_gate"].n) != (gate.k, gate.n):
+                raise ValueError("shared experts have the routed experts' sizes")
+        bias = weights.get("router_bias")
+        for t in [wr, gate, weights.get("shared_gate"), bias]:
+            if t is not None and t.device != gate.device:
+                raise ValueError(f"weights on {gate.device} and {t.device}: one device is needed")
+        if not wr.is_contiguous() or wr.dtype not in _DTYPES:
+            raise ValueError("router_w: a contiguous bf16 or fp32 matrix is needed")
+        if bias is not None and (bias.numel() != gate.experts or not bias.is_contiguous() or bias.dtype != torch.float32):
+            raise ValueError(f"router_bias: {gate.experts} contiguous fp32 values are needed")
         if wr.shape != (gate.k, gate.experts):
             raise ValueError(f"router_w {tuple(wr.shape)}: [D][E] = {(gate.k, gate.experts)} is needed")
         flags = (_pkg.FLAG_RESIDUAL if residual else 0) | (_pkg.FLAG_HIST_ACCUMULATE if hist_accumulate else 0)
@@ -325,6 +358,8 @@ class Mx4MoeLayer(_Workspace):
             raise ValueError(f"x: contiguous bf16 {(self.T, self.D)} on {dev}")
         if out is None:
             out = torch.empty_like(x)
+        else:
+            _check_out(out, x.shape, dev, torch.bfloat16)
         t = _pkg.MoeTensors()
         t.x, t.out, t.router_w = x.data_ptr(), out.data_ptr(), self.w["router_w"].data_ptr()
         if self.w.get("router_bias") is not None:
@@ -362,6 +397,11 @@ class Mx8TrainFfn:
         _bytes(self.lib.axm_mx8_checkpoint_bytes, rows, f)  # refuses sizes that cannot be kept
         self.checkpoint = [torch.empty(rows, n, dtype=torch.uint8, device=dev) for n in (f, f // 32, f, f // 32)]
         self.keep = _pkg.Mx8Checkpoint(*(t.data_ptr() for t in self.checkpoint))
+        if scratch is not None:
+            if len(scratch) != 3:
+                raise ValueError("scratch: three matrices are needed")
+            for t in scratch:
+                _check_out(t, (rows, f), dev, torch.bfloat16)
         self.scratch = scratch or [torch.empty(rows, f, dtype=torch.bfloat16, device=dev) for _ in range(3)]
         self.status_word = torch.zeros(1, dtype=torch.int32, device=dev)
         self.saved = None
@@ -379,10 +419,11 @@ class Mx8TrainFfn:
     @_on_its_device
     def forward(self, x, segments, out=None):
         self._check(x, "x")
-        if segments.dtype != torch.int32 or segments.shape[1:] != (4,) or not segments.is_contiguous() or segments.device != x.device:
-            raise ValueError("segments: a contiguous int32 table n x 4 beside x")
+        _check_index(segments, 4, x.device, "segments")
         if out is None:
             out = torch.empty(x.shape, dtype=self.dtype, device=x.device)
+        else:
+            _check_out(out, x.shape, x.device)
         p = _address
         _pkg.check(self.lib.axm_mx8_expert_ffn_train(
             ctypes.byref(self.desc), p(x), x.shape[0], p(segments), segments.shape[0], *map(p, self.weights),
@@ -402,9 +443,10 @@ class Mx8TrainFfn:
             raise ValueError(f"d_o {tuple(d_o.shape)} is not like x {tuple(x.shape)}")
         p = _address
         grads = {"d_x": torch.empty(x.shape, dtype=self.dtype, device=x.device)}
-        if weight_grads:
+        if weight_grads:  # experts that the table leaves out are not written: zero
+            make = torch.empty if segments.shape[0] >= self.desc.num_experts else torch.zeros
             for n, w in zip(("d_gate", "d_up", "d_down"), self.weights):
-                grads[n] = torch.empty(w.shape, dtype=self.dtype, device=x.device)
+                grads[n] = make(w.shape, dtype=self.dtype, device=x.device)
         _pkg.check(self.lib.axm_mx8_expert_ffn_backward(
             ctypes.byref(self.desc), p(x), x.shape[0], p(segments), segments.shape[0], ctypes.byref(self.keep), p(d_o),
             *map(p, self.weights), *map(p, self.scratch), p(grads["d_x"]), p(grads.get("d_gate")),

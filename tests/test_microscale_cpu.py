@@ -260,3 +260,72 @@ def test_training_step_workspaces(lib, axm):
             assert call(ctypes.byref(d), ctypes.byref(t), k, kb, sc, sb, None) == axm.AXM_ERR_WORKSPACE
         if not torch.cuda.is_available():
             assert call(ctypes.byref(d), ctypes.byref(t), FAKE, kept, FAKE, scratch, None) == axm.AXM_ERR_DEVICE
+
+
+def test_index_and_out_checks():
+    """What the calls of the Python layer refuse before they hand an address to the library."""
+    ms = importlib.import_module("project_axiom_ai_llm_b200.microscale")
+    dev = torch.device("cpu")
+    ms._check_index(None, 4, dev, "segments")
+    ms._check_index(torch.zeros(3, 4, dtype=torch.int32), 4, dev, "segments")
+    ms._check_index(torch.zeros(3, dtype=torch.int32), None, dev, "row_src")
+    for t, width in [(torch.zeros(3, 4), 4), (torch.zeros(3, 4, dtype=torch.int64), 4), (torch.zeros(3, 5, dtype=torch.int32), 4),
+                     (torch.zeros(12, dtype=torch.int32), 4), (torch.zeros(4, 3, dtype=torch.int32).t(), 4),
+                     (torch.zeros(3, dtype=torch.int64), None), (torch.zeros(6, dtype=torch.int32)[::2], None),
+                     (torch.zeros(3, 1, dtype=torch.int32), None), (torch.zeros(3, 4, dtype=torch.int32, device="meta"), 4)]:
+        with pytest.raises(ValueError):
+            ms._check_index(t, width, dev, "table")
+    bf16 = torch.bfloat16
+    ms._check_out(torch.zeros(3, 8, dtype=bf16), (3, 8), dev, bf16)
+    for t in [torch.zeros(3, 8), torch.zeros(2, 8, dtype=bf16), torch.zeros(3, 16, dtype=bf16)[:, ::2],
+              torch.zeros(3, 8, dtype=bf16, device="meta")]:
+        with pytest.raises(ValueError):
+            ms._check_out(t, (3, 8), dev, bf16)
+
+
+def test_weights_of_other_sizes_or_devices():
+    ms = importlib.import_module("project_axiom_ai_llm_b200.microscale")
+
+    def weights(e, k, n, device="cpu"):
+        return ms.Mx4Weights(torch.empty(e, n, k // 2, dtype=torch.uint8, device=device),
+                             torch.empty(16, dtype=torch.uint8, device=device), e, k, n)
+
+    a, d = weights(4, 64, 96), weights(4, 96, 64)
+    with pytest.raises(ValueError):
+        ms._expert_table(a, a, a)
+    with pytest.raises(ValueError):
+        ms._expert_table(a, a, weights(4, 96, 64, "meta"))
+    base = dict(router_w=torch.zeros(64, 4), gate=a, up=a, down=d)
+    small, small_d = weights(1, 64, 32), weights(1, 32, 64)
+    for change in [dict(shared_gate=small, shared_up=small, shared_down=small_d), dict(router_w=torch.zeros(4, 64).t()),
+                   dict(router_w=torch.zeros(64, 4, dtype=torch.float64)), dict(router_w=torch.zeros(64, 4, device="meta")),
+                   dict(router_bias=torch.zeros(3)), dict(router_bias=torch.zeros(4, dtype=torch.bfloat16)),
+                   dict(router_w=torch.zeros(64, 5))]:
+        with pytest.raises(ValueError):
+            ms.Mx4MoeLayer({**base, **change}, tokens=4, top_k=2)
+
+
+def test_training_scratch_refused(axm):
+    w = dict(router_w=torch.zeros(64, 4), w_gate=torch.zeros(4, 64, 96, dtype=torch.bfloat16))
+    need = axm.train_split_bytes(axm.make_desc(8, 64, 96, 4, 2, flags=axm.FLAG_RESIDUAL | axm.FLAG_SAVE_8BIT))[1]
+    for scratch in [torch.empty(need - 1, dtype=torch.uint8), torch.empty(need, dtype=torch.float32),
+                    torch.empty(2 * need, dtype=torch.uint8)[::2], torch.empty(need, dtype=torch.uint8, device="meta")]:
+        with pytest.raises(ValueError):
+            axm.MoeTrainLayer(w, 8, 2, device="cpu", save_8bit=True, scratch=scratch)
+
+
+def test_sharded_training_refuses_8_bits(lib, axm):
+    """On the host, with a layout that the same call accepts without the flag."""
+    world, e, d, f, t, k = 2, 8, 256, 512, 64, 2
+    lo, n, zero = axm.EpLayout(), ctypes.c_size_t(0), ctypes.c_size_t(0)
+    cap = t * k * world + 63 * (e // world)
+    assert lib.axm_ep_region_bytes(world, e, d, t * k, cap, ctypes.byref(lo), ctypes.byref(n)) == axm.AXM_OK
+    lo.rank, lo.row_align = 0, 64
+
+    def call(flags):
+        desc = axm.make_desc(t, d, f, e, k, flags=flags)
+        return lib.axm_moe_ep_train_workspace_bytes(ctypes.byref(lo), ctypes.byref(desc), ctypes.byref(n), ctypes.byref(zero))
+
+    assert call(axm.FLAG_RESIDUAL) == axm.AXM_OK
+    assert call(axm.FLAG_RESIDUAL | axm.FLAG_SAVE_8BIT) == axm.AXM_ERR_ARGUMENT
+    assert b"AXM_FLAG_SAVE_8BIT" in lib.axm_last_error()

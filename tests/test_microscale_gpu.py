@@ -686,3 +686,42 @@ def test_expert_ffn_with_more_rows_than_expected(ms, cuda_device, counts):
         assert plan.status() == 0
     for o in out[1:]:
         assert (o - out[0]).norm() <= 0.01 * out[0].norm()
+
+
+def test_train_step_with_experts_left_out(ms, cuda_device):
+    """Weight gradients of experts that the table does not name are zero, with a table of no segments all."""
+    w = [torch.randn(3, a, b, device=cuda_device).to(BF16) for a, b in ((64, 32), (64, 32), (32, 64))]
+    x = torch.randn(64, 64, device=cuda_device).to(BF16)
+    plan = ms.Mx8TrainFfn(*w, rows=64)
+    for table_rows, left in (([(0, 0, 64, 1)], [0, 2]), ([], [0, 1, 2])):
+        for _ in range(3):  # the allocator hands out used memory
+            torch.full((1 << 20,), float("nan"), device=cuda_device)
+        segs = torch.tensor(table_rows, dtype=torch.int32, device=cuda_device).reshape(-1, 4)
+        plan.forward(x, segs)
+        g = plan.backward(x)
+        assert all((g[k][left] == 0).all() for k in ("d_gate", "d_up", "d_down"))
+        assert all(torch.isfinite(g[k].float()).all() for k in ("d_gate", "d_up", "d_down"))
+
+
+def test_status_before_the_first_call(ms, cuda_device):
+    junk = [torch.full((1 << 22,), 0x5a, dtype=torch.uint8, device=cuda_device) for _ in range(4)]
+    del junk
+    w = ms.quantize_weights(torch.ones(1, 64, 64, device=cuda_device))
+    plan = ms.Mx4Linear(w, 4)
+    assert plan.status() == 0
+    plan.forward(torch.empty(0, 64, dtype=BF16, device=cuda_device))
+    assert plan.status() == 0
+
+
+def test_calls_with_wrong_indexes_are_refused(ms, cuda_device):
+    """On the host, before a launch."""
+    x = torch.zeros(4, 64, dtype=BF16, device=cuda_device)
+    with pytest.raises(ValueError):
+        ms.quantize_rows(x, row_src=torch.zeros(4, dtype=torch.int64, device=cuda_device))
+    with pytest.raises(ValueError):
+        ms.quantize_rows(x, row_src=torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        ms.quantize_rows(x, segments=torch.zeros(1, 4, dtype=torch.int64, device=cuda_device))
+    w = ms.quantize_weights(torch.ones(1, 64, 64, device=cuda_device))
+    with pytest.raises(ValueError):
+        ms.Mx4Linear(w, 4).forward(x, out=torch.zeros(64, 4, dtype=BF16, device=cuda_device).t())
