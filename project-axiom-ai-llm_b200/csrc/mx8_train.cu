@@ -20,7 +20,7 @@ int check_call(const AxmMoeDesc* d, int32_t rows, const AxmSegment* segments, in
   if (rows < 0) return fail(AXM_ERR_ARGUMENT, "%s: %d rows", what, rows);
   if (num_segments < 0 || num_segments > kMaxSegments)
     return fail(AXM_ERR_ARGUMENT, "%s: num_segments %d not in 0..%d", what, num_segments, kMaxSegments);
-  if (rows == 0) return AXM_OK;  // matrices without rows may have no address
+  if (rows == 0 || num_segments == 0) return AXM_OK;  // matrices without rows and empty tables may have no address
   if (!segments || !keep || !keep->gate_codes || !keep->gate_scales || !keep->up_codes || !keep->up_scales)
     return fail(AXM_ERR_ARGUMENT, "%s: null pointer", what);
   if (off16(keep->gate_codes) || off16(keep->up_codes))

@@ -138,6 +138,8 @@ def quantize_rows(x, segments=None, row_src=None, row_div=1):
     if segments is not None:
         _check_index(segments, 4, x.device, "segments")
         nseg = segments.shape[0]
+        if nseg == 0:  # an empty tensor has no address, which would mean that all rows form one segment
+            raise ValueError("segments: an empty table")
     # the sizes of axm_mx4_rows_bytes; sizes that it refuses are refused by the call below
     at = (rows * (k // 2) + 255) & -256
     size = at + (rows // 128 + (nseg or 1)) * ((k + 255) >> 8) * 1024

@@ -329,3 +329,12 @@ def test_sharded_training_refuses_8_bits(lib, axm):
     assert call(axm.FLAG_RESIDUAL) == axm.AXM_OK
     assert call(axm.FLAG_RESIDUAL | axm.FLAG_SAVE_8BIT) == axm.AXM_ERR_ARGUMENT
     assert b"AXM_FLAG_SAVE_8BIT" in lib.axm_last_error()
+
+
+def test_train8_empty_table_without_an_address(lib, axm):
+    """Zero segments: nothing to do, with rows and with a table that has no address (an empty tensor's)."""
+    desc, keep = axm.make_desc(64, 64, 64, 2, 1), axm.Mx8Checkpoint(*[FAKE] * 4)
+    assert lib.axm_mx8_expert_ffn_train(ctypes.byref(desc), FAKE, 64, None, 0, FAKE, FAKE, FAKE, ctypes.byref(keep), FAKE, FAKE,
+                                        0, None, None) == axm.AXM_OK
+    assert lib.axm_mx8_expert_ffn_backward(ctypes.byref(desc), FAKE, 64, None, 0, ctypes.byref(keep), FAKE, FAKE, FAKE, FAKE,
+                                           FAKE, FAKE, FAKE, FAKE, None, None, None, 0, None, None) == axm.AXM_OK

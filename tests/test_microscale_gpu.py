@@ -725,3 +725,5 @@ def test_calls_with_wrong_indexes_are_refused(ms, cuda_device):
     w = ms.quantize_weights(torch.ones(1, 64, 64, device=cuda_device))
     with pytest.raises(ValueError):
         ms.Mx4Linear(w, 4).forward(x, out=torch.zeros(64, 4, dtype=BF16, device=cuda_device).t())
+    with pytest.raises(ValueError):
+        ms.quantize_rows(x, segments=torch.zeros(0, 4, dtype=torch.int32, device=cuda_device))
