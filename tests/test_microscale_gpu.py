@@ -727,3 +727,90 @@ def test_calls_with_wrong_indexes_are_refused(ms, cuda_device):
         ms.Mx4Linear(w, 4).forward(x, out=torch.zeros(64, 4, dtype=BF16, device=cuda_device).t())
     with pytest.raises(ValueError):
         ms.quantize_rows(x, segments=torch.zeros(0, 4, dtype=torch.int32, device=cuda_device))
+
+
+def room(bytes_needed):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < bytes_needed:
+        pytest.skip(f"{bytes_needed >> 30} GB of free memory are needed")
+
+
+@pytest.fixture
+def give_back():
+    yield
+    torch.cuda.empty_cache()
+
+
+def test_rows_past_32_bits(ms, cuda_device, give_back):
+    """More than 2^32 values: the last rows are what they are alone."""
+    room(45 << 30)
+    rows, k = (1 << 20) + 4099, 4096
+    x = torch.empty(rows, k, dtype=BF16, device=cuda_device).normal_(generator=generator(cuda_device, 1))
+    tail = x[-700:].contiguous()
+    back = ms.dequantize_rows(ms.quantize_rows(x))
+    assert torch.equal(back[-700:], ms.dequantize_rows(ms.quantize_rows(tail)))
+    del back
+    codes, scales = ms.quantize_rows8(x)
+    alone = ms.quantize_rows8(tail)
+    assert torch.equal(codes[-700:], alone[0]) and torch.equal(scales[-700:], alone[1])
+    assert torch.equal(ms.dequantize_rows8(codes, scales)[-700:], ms.dequantize_rows8(*alone))
+
+
+def test_weights_past_32_bits(ms, cuda_device, give_back):
+    room(30 << 30)
+    w = torch.empty(17, 16384, 16384, dtype=BF16, device=cuda_device).normal_(generator=generator(cuda_device, 2))
+    back, alone = ms.dequantize_weights(ms.quantize_weights(w)), ms.dequantize_weights(ms.quantize_weights(w[16:].contiguous()))
+    assert torch.equal(back[16], alone[0])
+
+
+def test_linear_past_32_bits(ms, cuda_device, give_back):
+    """An output of more than 2^32 values; one stage of the reduction, so rows alone give the same bits."""
+    room(25 << 30)
+    rows, k, n = 300007, 64, 14400
+    w = ms.quantize_weights(torch.randn(1, k, n, device=cuda_device))
+    x = torch.empty(rows, k, dtype=BF16, device=cuda_device).normal_(generator=generator(cuda_device, 3))
+    plan = ms.Mx4Linear(w, rows)
+    out = plan.forward(x)
+    assert plan.status() == 0
+    assert torch.equal(out[-1031:], plan.forward(x[-1031:].contiguous()))
+
+
+def test_train_step_past_32_bits(ms, cuda_device, give_back):
+    """Checkpoints of more than 2^32 codes: the last expert's rows and gradients are what they are alone."""
+    room(75 << 30)
+    d, f, first, last = 64, 4096, 1 << 20, 4096
+    g = generator(cuda_device, 4)
+    w = [torch.empty(2, a, b, device=cuda_device).normal_(0, 0.1, generator=g).to(BF16) for a, b in ((d, f), (d, f), (f, d))]
+    x, d_o = (torch.empty(first + last, d, dtype=BF16, device=cuda_device).normal_(generator=g) for _ in range(2))
+
+    def run(w, x, d_o, counts):
+        segs, rows = table(counts, cuda_device)
+        plan = ms.Mx8TrainFfn(*w, rows=rows)
+        o, grads = plan.forward(x, segs), plan.backward(d_o)
+        assert plan.status() == 0
+        return o, grads
+
+    o, grads = run(w, x, d_o, [first, last])
+    o = o[-last:].clone()
+    grads = {"d_x": grads["d_x"][-last:].clone(), **{n: grads[n][1].clone() for n in ("d_gate", "d_up", "d_down")}}
+    alone, want = run([t[1:].contiguous() for t in w], x[-last:].contiguous(), d_o[-last:].contiguous(), [last])
+    assert torch.equal(o, alone) and torch.equal(grads["d_x"], want["d_x"])
+    assert all(torch.equal(grads[n], want[n][0]) for n in ("d_gate", "d_up", "d_down"))
+
+
+def test_two_streams_at_once(ms, cuda_device):
+    """Calls with workspaces of their own run side by side without touching one another's results."""
+    w = ms.quantize_weights(torch.randn(1, 512, 1024, device=cuda_device))
+    xs = [torch.randn(t, 512, device=cuda_device).to(BF16) for t in (1, 300)]
+    plans = [ms.Mx4Linear(w, 300) for _ in xs]
+    want = [p.forward(x) for p, x in zip(plans, xs)]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(50):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(plans[i].forward(xs[i]))
+    torch.cuda.synchronize()
+    for i, p in enumerate(plans):
+        assert p.status() == 0 and all(torch.equal(g, want[i]) for g in got[i])
