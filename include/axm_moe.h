@@ -636,7 +636,7 @@ AXM_API int axm_moe_ep_forward_host(const AxmEpLayout* layout, const AxmMoeDesc*
  * segment s are in the tiles from out_row0 / 128 + s on.  8-bit codes are [rows][K], their
  * scale bytes [rows][K/32].  K is a multiple of 32, N a multiple of 8; matrices, codes and
  * tile-ordered scales are 16-byte aligned.  Tables must be ordered by out_row0, their rows
- * disjoint and inside `rows`. */
+ * disjoint and inside `rows`; entries without rows may start anywhere in that order. */
 enum { AXM_DTYPE_BF16 = 0, AXM_DTYPE_FP32 = 1 };
 
 /* Bytes of the codes and of the tile-ordered scales.  num_segments 0: no table. */

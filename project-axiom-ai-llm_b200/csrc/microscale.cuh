@@ -179,8 +179,9 @@ __device__ __forceinline__ float2 mx8_unpack2(uint32_t two) {
   return f;
 }
 
-// The segment that output row `row` belongs to (the last one that starts at or before it and has
-// rows), and its first row; tables are ordered by out_row0.  -1: the row is behind its segment's end.
+// The segment that output row `row` belongs to: the last entry with rows that starts at or before it (tables
+// are ordered by out_row0; entries without rows may start anywhere, inside another's rows too), and its
+// first row.  -1: the row is behind that segment's end.
 // By a whole warp: 32 entries at a time, all loads of a round at once (a binary search is a chain of
 // dependent loads, 3 us for 64 segments, which every row of a small call waited for).
 struct RowSegment {
@@ -192,14 +193,14 @@ __device__ __forceinline__ RowSegment segment_of_row(const AxmSegment* segments,
   int rows = 0;
   for (int s0 = 0; s0 < n; s0 += 32) {
     const int4 e = s0 + lane < n ? __ldg(reinterpret_cast<const int4*>(segments) + s0 + lane) : make_int4(0, 0x7fffffff, 0, 0);
-    // segments without rows share their start with the next one: the last of them is found
-    const uint32_t here = __ballot_sync(0xffffffffu, e.y <= row);
-    if (here == 0) break;
-    const int at = 31 - __clz(here);
-    r.seg = s0 + at;
-    r.first = __shfl_sync(0xffffffffu, e.y, at);
-    rows = __shfl_sync(0xffffffffu, e.z, at);
-    if (at < 31) break;
+    const uint32_t here = __ballot_sync(0xffffffffu, e.y <= row && e.z > 0);
+    if (here != 0) {
+      const int at = 31 - __clz(here);
+      r.seg = s0 + at;
+      r.first = __shfl_sync(0xffffffffu, e.y, at);
+      rows = __shfl_sync(0xffffffffu, e.z, at);
+    }
+    if (__any_sync(0xffffffffu, e.y > row)) break;  // all further entries start behind the row
   }
   // (a start before the first row would count tiles that the scale buffer does not have)
   if (r.first < 0 || row - r.first >= rows) r.seg = -1;
