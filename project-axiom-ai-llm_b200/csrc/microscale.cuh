@@ -183,7 +183,8 @@ __device__ __forceinline__ float2 mx8_unpack2(uint32_t two) {
 // are ordered by out_row0; entries without rows may start anywhere, inside another's rows too), and its
 // first row.  -1: the row is behind that segment's end.
 // By a whole warp: 32 entries at a time, all loads of a round at once (a binary search is a chain of
-// dependent loads, 3 us for 64 segments, which every row of a small call waited for).
+// dependent loads, 3 us for 64 segments, which every row of a small call waited for).  Loads of four
+// bytes: a table is an array of int32 and starts at any multiple of four.
 struct RowSegment {
   int seg, first;
 };
@@ -192,15 +193,17 @@ __device__ __forceinline__ RowSegment segment_of_row(const AxmSegment* segments,
   RowSegment r = {-1, 0};
   int rows = 0;
   for (int s0 = 0; s0 < n; s0 += 32) {
-    const int4 e = s0 + lane < n ? __ldg(reinterpret_cast<const int4*>(segments) + s0 + lane) : make_int4(0, 0x7fffffff, 0, 0);
-    const uint32_t here = __ballot_sync(0xffffffffu, e.y <= row && e.z > 0);
+    const bool there = s0 + lane < n;
+    const int start = there ? __ldg(&segments[s0 + lane].out_row0) : 0x7fffffff;
+    const int count = there ? __ldg(&segments[s0 + lane].rows) : 0;
+    const uint32_t here = __ballot_sync(0xffffffffu, start <= row && count > 0);
     if (here != 0) {
       const int at = 31 - __clz(here);
       r.seg = s0 + at;
-      r.first = __shfl_sync(0xffffffffu, e.y, at);
-      rows = __shfl_sync(0xffffffffu, e.z, at);
+      r.first = __shfl_sync(0xffffffffu, start, at);
+      rows = __shfl_sync(0xffffffffu, count, at);
     }
-    if (__any_sync(0xffffffffu, e.y > row)) break;  // all further entries start behind the row
+    if (__any_sync(0xffffffffu, start > row)) break;  // all further entries start behind the row
   }
   // (a start before the first row would count tiles that the scale buffer does not have)
   if (r.first < 0 || row - r.first >= rows) r.seg = -1;

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import microscale_ref as ref
-from test_microscale_gpu import awkward, exact_expert_weights, ffn_reference, held_float, held_operand, same
+from test_microscale_gpu import awkward, exact_expert_weights, ffn_reference, held_float, held_operand, same, table
 
 pytestmark = pytest.mark.gpu
 BF16, FP32 = torch.bfloat16, torch.float32
@@ -53,3 +53,23 @@ def test_entries_without_rows(ms, cuda_device, name):
     got = plan.forward(x, segs, out=torch.full((rows, d), float("nan"), device=cuda_device))
     assert plan.status() == 0
     assert ((got.double() - o).abs() <= slack).all()
+
+
+@pytest.mark.parametrize("counts", [[5, 0, 3], [60, 70], [300, 0, 290]])
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_tables_at_any_address(ms, cuda_device, counts, offset):
+    """A table is an array of int32: it may be a slice that starts anywhere in another tensor (few-rows,
+    one-CTA and pair kernels; the 8-bit training calls)."""
+    segs, rows = table(counts, cuda_device, 64)
+    moved = torch.full((segs.numel() + 8,), -7, dtype=torch.int32, device=cuda_device)[offset:offset + segs.numel()].view(-1, 4)
+    moved.copy_(segs)
+    assert moved.data_ptr() % 16 == 4 * offset and moved.is_contiguous()
+    x = torch.randn(rows, 64, device=cuda_device).to(BF16)
+    assert torch.equal(ms.dequantize_rows(ms.quantize_rows(x, segments=moved)), ms.dequantize_rows(ms.quantize_rows(x, segments=segs)))
+    w = [torch.randn(3, *kn, device=cuda_device).to(BF16) for kn in ((64, 96), (64, 96), (96, 64))]
+    plan = ms.Mx4ExpertFfn(*(ms.quantize_weights(t) for t in w), rows=rows, tokens=rows)
+    assert torch.equal(plan.forward(x, moved), plan.forward(x, segs)) and plan.status() == 0
+    plan = ms.Mx8TrainFfn(*w, rows=rows)
+    want = [plan.forward(x, segs), *plan.backward(x).values()]
+    got = [plan.forward(x, moved), *plan.backward(x).values()]
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and plan.status() == 0
