@@ -15,6 +15,7 @@
 // matrix edge.  All waits are bounded; a wait that gives up winds both CTAs down and sets
 // the status word to 9.
 #include "gemm_2sm.cuh"
+#include "microscale.cuh"
 
 namespace axm {
 
@@ -45,6 +46,8 @@ struct Wgrad2Args {
   int units_before[kWgradProblems + 1];
   int* status;
   int overlap;  // see launch_overlapping
+  int rows_checked;  // training step with 8-bit checkpoints: as in the other products' arguments
+  int experts;
 };
 // The maps of a launch's problems: A, B and the gradient.
 struct Wgrad2Maps {
@@ -121,7 +124,8 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ Wgrad2Maps maps, const __grid_c
     tmem_relinquish2();
   }
   if (args.overlap) wait_for_previous();
-  for (int s = threadIdx.x; s < nseg; s += kGemmThreads) sh->seg[s] = args.segments[s];
+  for (int s = threadIdx.x; s < nseg; s += kGemmThreads)
+    sh->seg[s] = args.rows_checked > 0 ? product_segment(args.segments, s, args.rows_checked, 0, args.experts) : args.segments[s];
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // barriers of both CTAs are initialised before anyone signals across
@@ -249,7 +253,7 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ Wgrad2Maps maps, const __grid_c
           // swizzle of the output map (and free of bank conflicts); one TMA store per block.
           if (lane == 0) bulk_wait_read();  // the previous block's store has read the buffer
           __syncwarp();
-          if (n0 + c0 < args.n_total[u.problem] && block_row0 < args.m_total[u.problem]) {
+          if (n0 + c0 < args.n_total[u.problem] && block_row0 < args.m_total[u.problem] && (sg.expert & 0xffff) < args.experts) {
             if constexpr (kBf16) {  // rows of 64 bytes, the 64-byte swizzle of the bf16 output map
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
@@ -329,6 +333,8 @@ static int launch_wgrad_as(const AxmSegment* segments, int32_t num_segments, int
   wa.num_problems = num_problems;
   wa.status = status;
   wa.overlap = overlap ? 1 : 0;
+  wa.rows_checked = overlap ? rows_total : 0;
+  wa.experts = experts;
   for (int p = 0; p < num_problems; ++p) {
     const WgradProblem& w = problems[p];
     int rc;

@@ -59,6 +59,9 @@ struct Gemm2Args {
   int k_splits;
   long long split_stride;
   int out_bf16;  // kModeDown, kModeDX: bf16 rows instead of fp32
+  // Training step with 8-bit checkpoints: rows of the operands and outputs, inside which the table's
+  // entries are kept whatever it says (product_segment).  0: the table is taken as it is.
+  int rows_checked;
   // kModeSwiGLU8 (written) and kModeDH8 (read): e4m3 codes [rows][F], scale bytes [rows][F / 32]
   uint8_t* codes_g;
   uint8_t* codes_u;
@@ -226,7 +229,9 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
     tmem_relinquish2();
   }
   if (args.overlap) wait_for_previous();
-  for (int s = threadIdx.x; s < nseg; s += gemm2_threads(kMode)) sh->seg[s] = args.segments[s];
+  for (int s = threadIdx.x; s < nseg; s += gemm2_threads(kMode))
+    sh->seg[s] = args.rows_checked > 0 ? product_segment(args.segments, s, args.rows_checked, 0, args.routed_experts)
+                                       : args.segments[s];
   __syncthreads();
   if (warp == 0) count_tiles(sh, nseg, n_tiles);
   tc_fence_before();
@@ -964,8 +969,9 @@ int launch_bwd_dx_2sm(const AxmMoeDesc* d, const AxmSegment* segments, int32_t n
   ga.two_term = 0;
   ga.k_splits = 1;
   ga.split_stride = 0;
-  if (overlap) {
+  if (overlap) {  // the training step with 8-bit checkpoints
     ga.overlap = 1;
+    ga.rows_checked = rows_total;
     return launch_overlapping("grouped_gemm_2sm_kernel<dX>", grouped_gemm_2sm_kernel<kModeDX>, grid, kGemmThreads,
                               kGemm2SmemBytes, st, m_dg, m_du, m_wg, m_wu, m_wg, m_wu, m_dg, m_dg, m_dg, m_dg, ga);
   }
@@ -1010,6 +1016,7 @@ int launch_train8_forward(const AxmMoeDesc* d, const AxmSegment* segments, int32
   ga.scales_g = static_cast<uint8_t*>(keep->gate_scales);
   ga.scales_u = static_cast<uint8_t*>(keep->up_scales);
   ga.overlap = 1;
+  ga.rows_checked = rows_total;
   if ((rc = launch_overlapping("grouped_gemm_2sm_kernel<swiglu, 8 bits>", grouped_gemm_2sm_kernel<kModeSwiGLU8>, grid,
                                gemm2_threads(kModeSwiGLU8), kGemm2SmemBytes, st, a1, a1, g, u, g, u, a1, a1, a1, a1, ga)))
     return rc;
@@ -1060,6 +1067,7 @@ int launch_train8_dh(const AxmMoeDesc* d, const AxmSegment* segments, int32_t nu
   ga.scales_g = static_cast<uint8_t*>(keep->gate_scales);
   ga.scales_u = static_cast<uint8_t*>(keep->up_scales);
   ga.overlap = 1;
+  ga.rows_checked = rows_total;
   return launch_overlapping("grouped_gemm_2sm_kernel<dH, 8 bits>", grouped_gemm_2sm_kernel<kModeDH8>, grid, gemm2_threads(kModeDH8),
                             kGemm2DhSmemBytes, st, m_do, m_do, m_wd, m_wd, m_wd, m_wd, m_h, m_h, m_dg, m_du, ga);
 }

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import microscale_ref as ref
-from test_microscale_gpu import awkward, exact_expert_weights, ffn_reference, held_float, held_operand, same, table
+from test_microscale_gpu import awkward, exact_expert_weights, ffn_reference, generator, held_float, held_operand, same, table
 
 pytestmark = pytest.mark.gpu
 BF16, FP32 = torch.bfloat16, torch.float32
@@ -73,3 +73,52 @@ def test_tables_at_any_address(ms, cuda_device, counts, offset):
     want = [plan.forward(x, segs), *plan.backward(x).values()]
     got = [plan.forward(x, moved), *plan.backward(x).values()]
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and plan.status() == 0
+
+
+def test_training_tables_that_do_not_fit(ms, axm, cuda_device):
+    """The 8-bit training calls keep a table's entries inside `rows`: rows behind the matrices' end are cut
+    off, entries that start outside or name no expert are left out, everything else is as with the table
+    that fits.  Every buffer is a slice of one allocation, with 8 KiB around each that nothing may touch."""
+    dev, rows, d, f, e = cuda_device, 198, 64, 96, 4
+    fits = [(0, 0, 64, 0), (64, 64, 128, 2), (192, 192, 6, 1), (0, 0, 0, 3)]
+    padded = [(0, 0, 64, 0), (64, 64, 128, 2), (192, 192, 64, 1), (0, 0, 0, 3)]  # as if x were padded too
+    far = [(0, 0, 64, 0), (64, 64, 128, 2), (192, 192, 1 << 30, 1), (1 << 30, 1 << 30, 64, 3)]
+    before = [(0, 0, 64, 0), (64, 64, 128, 2), (192, 192, 70, 1), (-64, -64, 128, 3)]
+    unknown = fits + [(0, 0, 64, e), (64, 64, 64, 0xffff), (0, 0, 128, -1), (rows, rows, 64, 3), (64, 64, -64, 7)]
+    g = generator(dev, 1)
+    whole = dict(x=(rows, d, BF16), d_o=(rows, d, BF16), wg=(e * d, f, BF16), wu=(e * d, f, BF16), wd=(e * f, d, BF16),
+                 gc=(rows, f, torch.uint8), gs=(rows, f // 32, torch.uint8), uc=(rows, f, torch.uint8), us=(rows, f // 32, torch.uint8),
+                 h=(rows, f, BF16), dg=(rows, f, BF16), du=(rows, f, BF16))
+    lib, stream, desc = axm.load(), axm.current_stream(), axm.make_desc(rows, d, f, e, 1)
+    gap = 8192
+    for dtype, code in ((BF16, axm.DTYPE_BF16), (FP32, axm.DTYPE_FP32)):
+        shapes = {**whole, "o": (rows, d, dtype), "d_x": (rows, d, dtype), "dwg": (e * d, f, dtype), "dwu": (e * d, f, dtype), "dwd": (e * f, d, dtype)}
+        inputs = {n: torch.empty(shapes[n][:2], device=dev).normal_(0, 0.3, generator=g).to(BF16) for n in ("x", "d_o", "wg", "wu", "wd")}
+        want = None
+        for name, entries_ in (("fits", fits), ("padded", padded), ("far", far), ("before", before), ("unknown", unknown)):
+            at, places = gap, {}
+            for n, (r, c, t) in shapes.items():
+                size = r * c * t.itemsize
+                places[n] = (at, size)
+                at = (at + size + 255 & -256) + gap
+            pool = torch.full((at,), 0x5a, dtype=torch.uint8, device=dev)
+            v = {n: pool[a:a + s].view(shapes[n][2]).view(shapes[n][:2]) for n, (a, s) in places.items()}
+            for n in inputs:
+                v[n].copy_(inputs[n])
+            free = torch.ones(at, dtype=torch.bool, device=dev)
+            for a, s in places.values():
+                free[a:a + s] = False
+            segs = torch.tensor(entries_, dtype=torch.int32, device=dev)
+            keep = axm.Mx8Checkpoint(*(v[n].data_ptr() for n in ("gc", "gs", "uc", "us")))
+            status = torch.zeros(1, dtype=torch.int32, device=dev)
+            p = {n: t.data_ptr() for n, t in v.items()}
+            axm.check(lib.axm_mx8_expert_ffn_train(desc, p["x"], rows, segs.data_ptr(), len(entries_), p["wg"], p["wu"], p["wd"], keep,
+                                                   p["h"], p["o"], code, status.data_ptr(), stream))
+            axm.check(lib.axm_mx8_expert_ffn_backward(desc, p["x"], rows, segs.data_ptr(), len(entries_), keep, p["d_o"], p["wg"], p["wu"],
+                                                      p["wd"], p["h"], p["dg"], p["du"], p["d_x"], p["dwg"], p["dwu"], p["dwd"], code,
+                                                      status.data_ptr(), stream))
+            assert int(status.item()) == 0 and (pool[free] == 0x5a).all(), name
+            got = {n: pool[a:a + s].clone() for n, (a, s) in places.items()}
+            want = got if want is None else want
+            assert all(torch.equal(got[n], want[n]) for n in got), (name, [n for n in got if not torch.equal(got[n], want[n])])
+            assert torch.isfinite(v["d_x"].float()).all() and (v["dwg"].view(e, d, f)[3] == 0).all()
