@@ -244,6 +244,23 @@ mx_dequantize_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __re
       for (int i = 0; i < kAhead; ++i) {
         const int k0 = (run0 + i * wpr) * 512 + in_row * 16;
         if (!there || k0 >= k) break;
+        if constexpr (kBits == 8 && sizeof(T) == 4) {
+          // one by one: e4m3 under the smallest scales has values (from 2^-136 on) that bf16 has not
+          const float f = mx_scale_value(s[i]);
+          const uint32_t word[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 two = mx8_unpack2((word[2 * h + (j >> 1)] >> (16 * (j & 1))) & 0xffffu);
+              v[2 * j] = __float_as_uint(two.x * f);
+              v[2 * j + 1] = __float_as_uint(two.y * f);
+            }
+            store32<kWide>(to + k0 + 8 * h, v);
+          }
+          continue;
+        }
         const uint32_t f = mx_scale_bf16x2(s[i]);
         uint32_t w[8];
         if constexpr (kBits == 4) {
