@@ -274,6 +274,18 @@ mx_dequantize_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __re
           mx8_decode4(c[i].y, f, w[2], w[3]);
           mx8_decode4(c[i].z, f, w[4], w[5]);
           mx8_decode4(c[i].w, f, w[6], w[7]);
+          const uint32_t word[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+          uint32_t nan = 0;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) nan |= mx8_nan_codes(word[h]);
+          if (nan != 0) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const uint32_t n = mx8_nan_codes(word[h]);
+              w[2 * h] |= ((n & 0x80u) ? 0x7fc0u : 0u) | ((n & 0x8000u) ? 0x7fc00000u : 0u);
+              w[2 * h + 1] |= ((n & 0x800000u) ? 0x7fc0u : 0u) | ((n & 0x80000000u) ? 0x7fc00000u : 0u);
+            }
+          }
         }
         if constexpr (sizeof(T) == 2) {
           store32<kWide>(to + k0, w);

@@ -146,6 +146,12 @@ __device__ __forceinline__ void mx8_decode4(uint32_t codes, uint32_t scale2, uin
   }
 }
 
+// Bit 7 of every byte that is e4m3's NaN code (0x7f or 0xff), which mx8_decode4 takes for 480.  The library
+// writes none, codes from elsewhere may hold some.
+__device__ __forceinline__ uint32_t mx8_nan_codes(uint32_t codes) {
+  return ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
 // Four values to four e4m3 codes, value 0 in the lowest byte.
 __device__ __forceinline__ uint32_t mx8_pack4(float a, float b, float c, float d) {
   uint32_t r;

@@ -52,3 +52,12 @@ def test_4_bit_codes(ms, cuda_device):
     for out in (FP32, BF16):
         assert same(ms.dequantize_weights(q, out), want.to(out).transpose(1, 2))
         assert same(ms.dequantize_rows(rows, out), want[0].to(out))
+
+
+@pytest.mark.parametrize("k", [32, 96, 544])
+def test_8_bit_codes_that_stand_for_nan(ms, cuda_device, k):
+    """0x7f and 0xff read as NaN in either type; in bf16 every other code is rounded once."""
+    codes, scales, want = all_8_bit_codes(k, cuda_device)
+    assert torch.isnan(want).any()
+    assert same(ms.dequantize_rows8(codes, scales, FP32), want.float())
+    assert same(ms.dequantize_rows8(codes, scales, BF16), want.float().to(BF16))  # 64 to 32 bits is exact here
