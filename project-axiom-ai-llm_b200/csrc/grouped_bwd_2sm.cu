@@ -124,8 +124,10 @@ grouped_wgrad_2sm_kernel(const __grid_constant__ Wgrad2Maps maps, const __grid_c
     tmem_relinquish2();
   }
   if (args.overlap) wait_for_previous();
-  for (int s = threadIdx.x; s < nseg; s += kGemmThreads)
-    sh->seg[s] = args.rows_checked > 0 ? product_segment(args.segments, s, args.rows_checked, 0, args.experts) : args.segments[s];
+  for (int s = threadIdx.x; s < nseg; s += kGemmThreads) {
+    const AxmSegment sg = args.segments[s];
+    sh->seg[s] = args.rows_checked > 0 ? kept_inside(sg, args.rows_checked, 0, args.experts) : sg;
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // barriers of both CTAs are initialised before anyone signals across

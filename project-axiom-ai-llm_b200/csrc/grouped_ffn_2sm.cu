@@ -60,7 +60,7 @@ struct Gemm2Args {
   long long split_stride;
   int out_bf16;  // kModeDown, kModeDX: bf16 rows instead of fp32
   // Training step with 8-bit checkpoints: rows of the operands and outputs, inside which the table's
-  // entries are kept whatever it says (product_segment).  0: the table is taken as it is.
+  // entries are kept whatever it says (kept_inside).  0: the table is taken as it is.
   int rows_checked;
   // kModeSwiGLU8 (written) and kModeDH8 (read): e4m3 codes [rows][F], scale bytes [rows][F / 32]
   uint8_t* codes_g;
@@ -229,9 +229,10 @@ grouped_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_c
     tmem_relinquish2();
   }
   if (args.overlap) wait_for_previous();
-  for (int s = threadIdx.x; s < nseg; s += gemm2_threads(kMode))
-    sh->seg[s] = args.rows_checked > 0 ? product_segment(args.segments, s, args.rows_checked, 0, args.routed_experts)
-                                       : args.segments[s];
+  for (int s = threadIdx.x; s < nseg; s += gemm2_threads(kMode)) {
+    const AxmSegment sg = args.segments[s];
+    sh->seg[s] = args.rows_checked > 0 ? kept_inside(sg, args.rows_checked, 0, args.routed_experts) : sg;
+  }
   __syncthreads();
   if (warp == 0) count_tiles(sh, nseg, n_tiles);
   tc_fence_before();

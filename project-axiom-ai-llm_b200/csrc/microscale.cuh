@@ -218,17 +218,19 @@ __device__ __forceinline__ RowSegment segment_of_row(const AxmSegment* segments,
   return r;
 }
 
-// Entry s of a product's segment table (none: one segment of all rows), kept inside the buffers whatever
-// the table says: rows beyond `rows_total` are dropped, and a segment that starts outside or whose
-// expert is not one of this launch's has none.
+// A table's entry, kept inside the buffers whatever it says: rows beyond `rows_total` are dropped, and a
+// segment that starts outside or whose expert is not one of this launch's has none.
+__device__ __forceinline__ AxmSegment kept_inside(AxmSegment sg, int rows_total, int expert_base, int experts) {
+  const int e = (sg.expert & 0xffff) - expert_base;
+  const bool there = sg.out_row0 >= 0 && sg.out_row0 < rows_total && e >= 0 && e < experts;
+  sg.rows = there ? min(max(sg.rows, 0), rows_total - sg.out_row0) : 0;
+  return sg;
+}
+// Entry s of a product's segment table (none: one segment of all rows).
 __device__ __forceinline__ AxmSegment product_segment(const AxmSegment* segments, int s, int rows_total, int expert_base,
                                                       int experts) {
   if (segments == nullptr) return AxmSegment{0, 0, rows_total, expert_base};
-  AxmSegment sg = segments[s];
-  const int e = (sg.expert & 0xffff) - expert_base;
-  if (sg.out_row0 < 0 || sg.out_row0 >= rows_total || e < 0 || e >= experts || sg.rows < 0) sg.rows = 0;
-  sg.rows = min(sg.rows, max(rows_total - sg.out_row0, 0));
-  return sg;
+  return kept_inside(segments[s], rows_total, expert_base, experts);
 }
 
 #endif
