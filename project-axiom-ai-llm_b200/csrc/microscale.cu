@@ -329,7 +329,7 @@ mx4_quantize_weights_kernel(const T* __restrict__ w, int k, int n, uint8_t* __re
   // 16-byte piece p of column c sits at piece p ^ (c % 8): neither the column-wise stores nor the
   // row-wise loads of a warp meet in a bank
   __shared__ uint4 tile[kWeightsN * 8];
-  __shared__ uint8_t sc[kWeightsN][8];
+  __shared__ __align__(4) uint8_t sc[kWeightsN][8];  // read back four bytes at a time
   const int e = blockIdx.z, n0 = blockIdx.x * kWeightsN, k0 = blockIdx.y * kWeightsK;
   const int pair = threadIdx.x & 31, blk = threadIdx.x >> 5;
   const int col = n0 + 2 * pair, kk = k0 + blk * kMxBlock;
