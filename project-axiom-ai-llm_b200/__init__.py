@@ -373,10 +373,10 @@ class MoeTrainLayer:
         rdt = ROUTER_FP32 if wr.dtype == torch.float32 else ROUTER_BF16
         S = self.S = 0 if weights.get("shared_gate") is None else weights["shared_gate"].shape[0]
         self.desc = make_desc(tokens, D, F, E, top_k, S, rdt, FLAG_RESIDUAL | (FLAG_SAVE_8BIT if save_8bit else 0))
-        dev = torch.device(device)
+        dev = torch.empty(0, device=device).device  # with its index
         kept, shared = train_split_bytes(self.desc)
         if scratch is not None and (scratch.dtype != torch.uint8 or scratch.numel() < shared or not scratch.is_contiguous() or
-                                    scratch.device.type != dev.type):
+                                    scratch.device != dev):
             raise ValueError(f"scratch: {shared} contiguous bytes on {dev} are needed, not {scratch.numel()} of "
                              f"{scratch.dtype} on {scratch.device}")
         self.scratch = scratch
