@@ -50,7 +50,7 @@ def _rows_of(x):
     ld, one = x.stride()
     if one != 1 and k > 1:
         raise ValueError("a CUDA matrix with contiguous rows is needed")
-    return rows, k, ld if rows > 1 else max(ld, k)
+    return rows, k, ld if rows > 1 else k  # one row has no next one: its stride says nothing
 
 
 def _check_index(t, width, device, what):

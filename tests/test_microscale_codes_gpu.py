@@ -1,4 +1,5 @@
-"""Every code under the smallest, middle and largest scale bytes, as another program may have written them."""
+"""Every code under the smallest, middle and largest scale bytes, as another program may have written them; rows
+with any stride."""
 import importlib
 
 import pytest
@@ -61,3 +62,17 @@ def test_8_bit_codes_that_stand_for_nan(ms, cuda_device, k):
     assert torch.isnan(want).any()
     assert same(ms.dequantize_rows8(codes, scales, FP32), want.float())
     assert same(ms.dequantize_rows8(codes, scales, BF16), want.float().to(BF16))  # 64 to 32 bits is exact here
+
+
+@pytest.mark.parametrize("stride", [5, 4097])
+def test_one_row_with_any_stride(ms, cuda_device, stride):
+    """The stride of a single row is never used: a row cut out of a matrix of odd width is taken as it is."""
+    pool = torch.randn(2 * 4096, device=cuda_device).to(BF16)
+    x = torch.as_strided(pool, (1, 288), (stride, 1))
+    want = ms.dequantize_rows(ms.quantize_rows(x.clone()))
+    assert torch.equal(ms.dequantize_rows(ms.quantize_rows(x)), want)
+    assert torch.equal(ms.dequantize_rows8(*ms.quantize_rows8(x)), ms.dequantize_rows8(*ms.quantize_rows8(x.clone())))
+    out = torch.as_strided(torch.zeros_like(pool), (1, 288), (stride, 1))
+    assert torch.equal(ms.dequantize_rows(ms.quantize_rows(x), out=out), want)
+    plan = ms.Mx4Linear(ms.quantize_weights(torch.randn(1, 288, 72, device=cuda_device)), 4)
+    assert torch.equal(plan.forward(x), plan.forward(x.clone()))
