@@ -129,7 +129,8 @@ class Mx4Weights:
 
 @_on_its_device
 def quantize_rows(x, segments=None, row_src=None, row_div=1):
-    """x [rows][K] bf16 or fp32 to 4 bits; row_src: row r is read from x[row_src[r] // row_div]."""
+    """x [rows][K] bf16 or fp32 to 4 bits; row_src: row r is read from x[row_src[r] // row_div], which has to
+    exist (negative: zeros).  Rows that no segment covers cannot be read back."""
     rows, k, ld = _rows_of(x)
     nseg = 0
     if row_src is not None:
@@ -155,6 +156,7 @@ def quantize_rows(x, segments=None, row_src=None, row_div=1):
 
 @_on_its_device
 def dequantize_rows(q, dtype=torch.bfloat16, out=None):
+    """Rows that no segment covers are not written: without `out` they hold what the allocator gave."""
     buffer, rows, k, ld = q.buffer, q.rows, q.k, q.k
     device = buffer.device
     if out is None:
@@ -296,7 +298,8 @@ class Mx4ExpertFfn(_Workspace):
 
     @_on_its_device
     def forward(self, x, segments, out=None, dtype=torch.bfloat16):
-        """x [rows][D] bf16, segments int32 [n][4] {a_row0, out_row0, rows, expert} (device)."""
+        """x [rows][D] bf16, segments int32 [n][4] {a_row0, out_row0, rows, expert} (device).  Rows that no
+        segment covers are not written: without `out` they hold what the allocator gave."""
         rows, d, _ = _rows_of(x)
         dev = self.device
         if rows > self.rows or d != self.desc.d_model or not x.is_contiguous() or x.dtype != torch.bfloat16 or x.device != dev:
@@ -380,8 +383,9 @@ class Mx8TrainFfn:
     projection's outputs in 8 bits, backward(d_o) gives the gradients from them.
 
     gate, up [E][D][F] and down [E][F][D] bf16; up to `rows` rows, segments padded to 64 rows with zero
-    rows (the layer's training layout).  dtype: of o and of every gradient.  What is kept is in
-    `checkpoint`; `scratch` (h, dG, dU) holds nothing between calls and may be shared by objects of the
+    rows (the layer's training layout).  dtype: of o and of every gradient.  Rows that no segment covers are
+    not written: in o and d_x, when these are not the caller's, they hold what the allocator gave (the
+    gradients of experts that a table leaves out are zero).  What is kept is in `checkpoint`; `scratch` (h, dG, dU) holds nothing between calls and may be shared by objects of the
     same sizes that run one after the other on one stream."""
 
     def __init__(self, gate, up, down, rows, dtype=torch.bfloat16, scratch=None):
