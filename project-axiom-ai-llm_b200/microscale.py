@@ -384,9 +384,9 @@ class Mx8TrainFfn:
 
     gate, up [E][D][F] and down [E][F][D] bf16; up to `rows` rows, segments padded to 64 rows with zero
     rows (the layer's training layout).  dtype: of o and of every gradient.  Rows that no segment covers are
-    not written: in o and d_x, when these are not the caller's, they hold what the allocator gave (the
-    gradients of experts that a table leaves out are zero).  What is kept is in `checkpoint`; `scratch` (h, dG, dU) holds nothing between calls and may be shared by objects of the
-    same sizes that run one after the other on one stream."""
+    not written: d_x, and o without `out`, hold there what the allocator gave (the gradients of experts that
+    a table leaves out are zero).  What is kept is in `checkpoint`; `scratch` (h, dG, dU) holds nothing
+    between calls and may be shared by objects of the same sizes that run one after the other on one stream."""
 
     def __init__(self, gate, up, down, rows, dtype=torch.bfloat16, scratch=None):
         self.lib = _pkg.load()
