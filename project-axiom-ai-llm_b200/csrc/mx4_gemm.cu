@@ -449,9 +449,10 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
 
 // ---- the same tile on one CTA -----------------------------------------------------------------
 // For segments of up to about a hundred rows, whose time is the weights' way in: a pair's second CTA would
-// have no rows of its own there.  M = 128 rows, N = 256 weight rows, all of them staged by the CTA
-// itself: 51 KB a stage, four stages.  The first ring of weights is asked for before the kernel
-// before this one has finished (the weights do not depend on it).
+// have no rows of its own there; and for all segments where pairs are not wanted or cannot be scheduled.
+// M = 128 rows, N = 256 weight rows, all of them staged by the CTA itself: 51 KB a stage, four stages.  The
+// first ring of weights is asked for before the kernel before this one has finished (the weights do not
+// depend on it).
 constexpr int kStages1 = 4;
 constexpr int kStageCodes1 = 3 * kCodeBytes;
 constexpr int kStageScales1 = kScaleABytes + kScaleBBytes;
@@ -706,7 +707,12 @@ template <int kMode>
 int launch_tiles(const CUtensorMap& a, const CUtensorMap& a_sf, const CUtensorMap& b0, const CUtensorMap& b1,
                 const CUtensorMap& b0_sf, const CUtensorMap& b1_sf, const Mx4Args& args, bool single, cudaStream_t st) {
   static SmemLimitCache smem = {}, smem1 = {};
-  if (single) {
+  int grid = 0;
+  if (!single && use_2sm_kernels()) {
+    grid = grid_2sm();
+    if (grid < 0) return grid;
+  }
+  if (grid < 2) {  // few rows a segment, or no pairs: not wanted (AXM_GEMM_2SM=0) or not to be had on this device
     if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(mx4_gemm_single_kernel<kMode>), kMx4SmemBytes1, &smem1,
                                      "mx4_gemm_single_kernel"))
       return rc;
@@ -716,9 +722,6 @@ int launch_tiles(const CUtensorMap& a, const CUtensorMap& a_sf, const CUtensorMa
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(mx4_gemm_pair_kernel<kMode>), kMx4SmemBytes, &smem,
                                    "mx4_gemm_pair_kernel"))
     return rc;
-  const int grid = grid_2sm();
-  if (grid < 0) return grid;
-  if (grid < 2) return fail(AXM_ERR_DEVICE, "two-SM clusters cannot be scheduled on this device");
   mx4_gemm_pair_kernel<kMode><<<grid, kThreads4, kMx4SmemBytes, st>>>(a, a_sf, b0, b1, b0_sf, b1_sf, args);
   return check_launch("mx4_gemm_pair_kernel");
 }
