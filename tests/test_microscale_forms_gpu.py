@@ -45,7 +45,7 @@ def test_few_rows_instances(ms, cuda_device, counts, d, f):
     assert float(slack[:rows].norm()) < (0.02 if f < 4096 else 0.5) * float(o[:rows].norm())
 
 
-@pytest.mark.parametrize("t", [1, 23, 300])
+@pytest.mark.parametrize("t", [1, 23, 300, 1100])  # few-rows, one-CTA and pair kernels
 @pytest.mark.parametrize("residual,accumulate,biased,router,shared", [
     (False, False, False, FP32, 0), (True, True, False, FP32, 1), (True, False, True, FP32, 0), (True, False, False, BF16, 2),
     (False, True, True, BF16, 1)])
