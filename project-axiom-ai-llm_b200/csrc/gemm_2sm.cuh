@@ -79,13 +79,7 @@ __device__ __forceinline__ void tmem_relinquish2() {
 __device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }
-// arrives on the mbarrier at a shared::cluster address once the pair's MMAs issued so far are done
-__device__ __forceinline__ void tc_commit2(uint32_t bar_cluster_addr) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   bar_cluster_addr)
-               : "memory");
-}
-// The same for both CTAs of the pair with one instruction: the barrier at this offset in either.
+// Arrives, once the pair's MMAs issued so far are done, on the barrier at this offset in both CTAs.
 __device__ __forceinline__ void tc_commit2_both(uint32_t bar_addr) {
   asm volatile(
       "{\n\t"

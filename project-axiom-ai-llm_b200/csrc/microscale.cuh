@@ -18,6 +18,8 @@
 // runs on the few-rows kernels they have 16, 32 or 64 rows instead, in the same places of 512 bytes.
 #pragma once
 
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace axm {
@@ -28,7 +30,7 @@ __host__ __device__ constexpr int mx4_chunks(int k) { return (k + 255) / 256 * 2
 __host__ __device__ constexpr long long mx4_row_tiles(long long rows, int num_segments, int tile_rows = 128) {
   return rows / tile_rows + num_segments;
 }
-// Room for any tile_rows that mx4_tile_rows chooses, in a workspace made for `rows` or more.
+// Room for any tile_rows that mx4_choose settles on, in a workspace made for `rows` or more.
 __host__ __device__ constexpr long long mx4_row_tiles_most(long long rows, int num_segments) {
   return rows / 128 + 2LL * num_segments;
 }
@@ -76,6 +78,11 @@ int launch_mx4_linear_few(const Mx4Rows& r, const void* a_codes, const void* a_s
 int launch_mx4_gated_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, const AxmMx4Experts* w, int experts,
                          int d, int f, void* h_codes, void* h_scales, cudaStream_t st);
 
+// Tensor maps (mx4_gemm.cu).  Codes: rows of k / 2 bytes, a box of 128 bytes x box_rows rows, 128-byte swizzle.
+int mx4_map_codes(CUtensorMap* m, const void* base, uint64_t experts, uint64_t rows, uint64_t k, uint32_t box_rows);
+// Scale chunks: words [tiles][chunks][128], a box of two chunks of one tile.
+int mx4_map_scales(CUtensorMap* m, const void* base, uint64_t tiles, int k);
+
 #if defined(__CUDACC__)
 
 // Scale byte of a block whose largest magnitude has these fp32 bits (sign cleared).
@@ -109,6 +116,23 @@ __device__ __forceinline__ uint32_t mx4_pack8(const float (&v)[8]) {
       : "=r"(r)
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
+}
+// A row's block of 32 to its codes and scale byte.
+__device__ __forceinline__ uint4 mx4_quantize_block(const float (&h)[32], uint32_t& byte) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) top = max(top, __float_as_uint(h[j]) & 0x7fffffffu);
+  byte = mx_scale_byte<2>(top);
+  const float inv = mx_inverse_scale(byte);
+  uint32_t q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = h[8 * i + j] * inv;
+    q[i] = mx4_pack8(t);
+  }
+  return make_uint4(q[0], q[1], q[2], q[3]);
 }
 // Reading back.  What a block of e2m1 holds is exact in bf16 (two significant bits, 2^-128 the smallest), and
 // what a block of e4m3 holds is too but for the smallest codes under the scale bytes 0 to 2 (steps of 2^-136
@@ -231,6 +255,26 @@ __device__ __forceinline__ AxmSegment product_segment(const AxmSegment* segments
                                                       int experts) {
   if (segments == nullptr) return AxmSegment{0, 0, rows_total, expert_base};
   return kept_inside(segments[s], rows_total, expert_base, experts);
+}
+
+// ---- tcgen05, block-scaled kind::mxf4, one CTA ----
+__device__ __forceinline__ void tc_mma1_mx4(uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                            uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_cp1_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Shared-memory descriptor of a 512-byte scale chunk: no swizzle, 8-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr >> 4) & 0x3fffu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
 }
 
 #endif

@@ -92,23 +92,6 @@ constexpr uint32_t few_instr_desc(uint32_t step) {
   return ((step * 2u) << 4) | (1u << 7) | (1u << 10) | (((uint32_t)N >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24) |
          ((step * 2u) << 29);
 }
-__device__ __forceinline__ void tc_mma1_mx4(uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                            uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
-      "}" ::"r"(d_tmem),
-      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void tc_cp1_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-__device__ __forceinline__ uint64_t few_scale_desc(uint32_t smem_addr) {
-  return (uint64_t)((smem_addr >> 4) & 0x3fffu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
-}
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -177,7 +160,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
   const int k_blocks = (args.k_total + 255) / 256;
 
   // the next kernel may start its own preparations; it waits for this one before it reads
-  asm volatile("griddepcontrol.launch_dependents;");
+  launch_dependents();
 
   // The segment table is older than the kernel before this one (see the launch), so it may be read
   // at once.
@@ -292,7 +275,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         const FewTile t = decode(tile);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!waited && ahead == kStages) {
-            asm volatile("griddepcontrol.wait;" ::: "memory");
+            wait_for_previous();
             waited = true;
             int n = 0;
             long long t2;
@@ -315,7 +298,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         }
       }
       if (!waited) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
+        wait_for_previous();
         int n = 0;
         long long t2;
         int b0, b1;
@@ -329,7 +312,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     // ---- MMA issuer (the whole warp, one elected lane issues) -------------------------------------
     {
       const uint64_t codes0 = make_smem_desc(smem_u32(tiles), 16, 1024);
-      const uint64_t scales0 = few_scale_desc(smem_u32(scales_s));
+      const uint64_t scales0 = scale_desc(smem_u32(scales_s));
       const uint32_t sf_w = tmem_base + Cfg::kSf, sf_a = sf_w + Cfg::kWeights * 8;
       int stage = 0;
       uint32_t phase = 0;
@@ -384,7 +367,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     const int quad = warp & 3;
     float* turn_s = sh->turn[warp - 2];
     const int feature = quad * 32 + lane;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // outputs and partial sums of earlier launches
+    wait_for_previous();  // outputs and partial sums of earlier launches
     Units p = mine;
     long long tile;
     int kb0, kb1;
@@ -477,25 +460,11 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
               uint32_t byte = 0;
               if (f0 < args.n_total) {
                 float h[32];
-                uint32_t top = 0;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  h[j] = turn_s[lane * 33 + j];
-                  top = max(top, __float_as_uint(h[j]) & 0x7fffffffu);
-                }
-                byte = mx_scale_byte<2>(top);
-                const float inv = mx_inverse_scale(byte);
-                uint32_t q[4];
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                  float x[8];
-#pragma unroll
-                  for (int j = 0; j < 8; ++j) x[j] = h[8 * b + j] * inv;
-                  q[b] = mx4_pack8(x);
-                }
+                for (int j = 0; j < 32; ++j) h[j] = turn_s[lane * 33 + j];
                 *reinterpret_cast<uint4*>(static_cast<uint8_t*>(args.out) +
                                           (row0 + n0 + lane) * (size_t)(args.n_total >> 1) + (f0 >> 1)) =
-                    make_uint4(q[0], q[1], q[2], q[3]);
+                    mx4_quantize_block(h, byte);
               }
               sf[quad] = (uint8_t)byte;
               if (quad == 0 && t.f_tile == f_tiles - 1 && f_tiles < chunks) *reinterpret_cast<uint32_t*>(sf + 512) = 0u;
@@ -547,19 +516,6 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
   }
 }
 
-int map_few(CUtensorMap* m, const void* base, uint64_t experts, uint64_t rows, uint64_t k, uint32_t box_rows) {
-  const uint64_t dims[3] = {k / 2, rows, experts};
-  const uint64_t strides[2] = {k / 2, k / 2 * rows};
-  const uint32_t box[3] = {128, box_rows, 1};
-  return encode_tensor_map_bytes(m, base, 3, dims, strides, box);
-}
-int map_few_scales(CUtensorMap* m, const void* base, uint64_t tiles, int k) {
-  const uint64_t dims[3] = {128, (uint64_t)mx4_chunks(k), tiles};
-  const uint64_t strides[2] = {512, 512ull * mx4_chunks(k)};
-  const uint32_t box[3] = {128, 2, 1};
-  return encode_tensor_map_words(m, base, 3, dims, strides, box);
-}
-
 template <bool kGated, int N>
 int launch_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, const void* const (&w)[4], int experts, int k,
                int n, FewArgs ga, cudaStream_t st) {
@@ -572,13 +528,13 @@ int launch_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, cons
   CUtensorMap a, a_sf, w0, w1, w0_sf, w1_sf;
   int rc;
   const int wn = (n + 127) / 128;
-  if ((rc = map_few(&a, a_codes, 1, r.rows, k, N))) return rc;
-  if ((rc = map_few_scales(&a_sf, a_scales, mx4_row_tiles(r.rows, r.table_segments, N), k))) return rc;
-  if ((rc = map_few(&w0, w[0], experts, n, k, 128))) return rc;
-  if ((rc = map_few_scales(&w0_sf, w[1], (uint64_t)experts * wn, k))) return rc;
+  if ((rc = mx4_map_codes(&a, a_codes, 1, r.rows, k, N))) return rc;
+  if ((rc = mx4_map_scales(&a_sf, a_scales, mx4_row_tiles(r.rows, r.table_segments, N), k))) return rc;
+  if ((rc = mx4_map_codes(&w0, w[0], experts, n, k, 128))) return rc;
+  if ((rc = mx4_map_scales(&w0_sf, w[1], (uint64_t)experts * wn, k))) return rc;
   if constexpr (kGated) {
-    if ((rc = map_few(&w1, w[2], experts, n, k, 128))) return rc;
-    if ((rc = map_few_scales(&w1_sf, w[3], (uint64_t)experts * wn, k))) return rc;
+    if ((rc = mx4_map_codes(&w1, w[2], experts, n, k, 128))) return rc;
+    if ((rc = mx4_map_scales(&w1_sf, w[3], (uint64_t)experts * wn, k))) return rc;
   } else {
     w1 = w0;
     w1_sf = w0_sf;
@@ -597,17 +553,8 @@ int launch_few(const Mx4Rows& r, const void* a_codes, const void* a_scales, cons
   ga.counters = r.few_counters;
   // Starts while the kernel before it drains.  That kernel has waited for everything before itself,
   // so what is older (weights, segment table) may be read without waiting.
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)sm_count(), 1, 1);
-  cfg.blockDim = dim3(kThreadsF, 1, 1);
-  cfg.dynamicSmemBytes = smem_bytes;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, mx4_few_kernel<kGated, N>, a, a_sf, w0, w1, w0_sf, w1_sf, ga), "mx4_few_kernel");
+  return launch_overlapping("mx4_few_kernel", mx4_few_kernel<kGated, N>, sm_count(), kThreadsF, smem_bytes, st, a, a_sf, w0, w1,
+                            w0_sf, w1_sf, ga);
 }
 
 template <bool kGated>

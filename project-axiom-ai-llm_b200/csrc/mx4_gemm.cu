@@ -29,8 +29,6 @@
 // Measured: 8192 rows 4096 -> 14336 185 us (5.2 PFLOP/s) in a short run, 8 experts 4096 x 14336 over 16384 rows
 // gated 720 us, linear 344 us (5.4 and 5.6 PFLOP/s); back to back the power cap holds them to 4.0-4.8.  A stage took
 // 630 cycles where its MMAs take 511 (8192 rows, 14336 -> 4096).
-#include <mutex>
-
 #include "gemm_2sm.cuh"
 #include "microscale.cuh"
 
@@ -109,11 +107,6 @@ __device__ __forceinline__ void tc_mma2_mx4(uint32_t d_tmem, uint64_t desc_a, ui
 __device__ __forceinline__ void tc_cp2_scales(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-// Shared-memory descriptor of a 512-byte scale chunk: no swizzle, 8-row groups 128 bytes apart.
-__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
-  return (uint64_t)((smem_addr >> 4) & 0x3fffu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
-}
-
 struct Unit4 {
   int seg, m_tile, n_tile, seg0;
   bool live;  // false: this half of the pair has no rows
@@ -152,24 +145,12 @@ __device__ __forceinline__ Unit4 decode4(const Mx4Shared* sh, int n_tiles, int u
 // silu(g) u, and the block's codes and scale byte
 __device__ __forceinline__ uint4 gate_block(const uint32_t (&g)[32], const uint32_t (&u)[32], uint32_t& byte) {
   float h[32];
-  uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 32; ++j) {
     const float gv = __uint_as_float(g[j]);
     h[j] = __fdividef(gv, 1.0f + __expf(-gv)) * __uint_as_float(u[j]);
-    top = max(top, __float_as_uint(h[j]) & 0x7fffffffu);
   }
-  byte = mx_scale_byte<2>(top);
-  const float inv = mx_inverse_scale(byte);
-  uint32_t q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float t[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = h[8 * i + j] * inv;
-    q[i] = mx4_pack8(t);
-  }
-  return make_uint4(q[0], q[1], q[2], q[3]);
+  return mx4_quantize_block(h, byte);
 }
 
 // The epilogue of one tile by one of four warps: 128 accumulator rows from `acc` on, a row a thread.
@@ -464,21 +445,6 @@ static_assert(kMx4SmemBytes1 <= 227u * 1024u, "shared memory of the 4-bit one-CT
 constexpr uint32_t mx4_instr_desc1(uint32_t step) {  // M = 128 of one CTA
   return (mx4_instr_desc(step) & ~(0x1fu << 24)) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void tc_mma1_mx4(uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                            uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
-      "}" ::"r"(d_tmem),
-      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void tc_cp1_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-
 // Units: expert group by expert group, column tile by column tile, row tiles innermost.
 __device__ __forceinline__ Unit4 decode1(const Mx4Shared* sh, int n_tiles, int unit) {
   int lo = 0, hi = sh->num_groups - 1;
@@ -688,21 +654,6 @@ mx4_gemm_single_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_co
 
 // ---- host side -----------------------------------------------------------------------------
 
-// Codes: rows of k / 2 bytes, a box of 128 bytes x 128 rows, 128-byte swizzle.
-int map_codes(CUtensorMap* m, const void* base, uint64_t experts, uint64_t rows, uint64_t k) {
-  const uint64_t dims[3] = {k / 2, rows, experts};
-  const uint64_t strides[2] = {k / 2, k / 2 * rows};
-  const uint32_t box[3] = {128, 128, 1};
-  return encode_tensor_map_bytes(m, base, 3, dims, strides, box);
-}
-// Scale chunks: words [tiles][chunks][128], a box of two chunks of one tile.
-int map_scales(CUtensorMap* m, const void* base, uint64_t tiles, int k) {
-  const uint64_t dims[3] = {128, (uint64_t)mx4_chunks(k), tiles};
-  const uint64_t strides[2] = {512, 512ull * mx4_chunks(k)};
-  const uint32_t box[3] = {128, 2, 1};
-  return encode_tensor_map_words(m, base, 3, dims, strides, box);
-}
-
 template <int kMode>
 int launch_tiles(const CUtensorMap& a, const CUtensorMap& a_sf, const CUtensorMap& b0, const CUtensorMap& b1,
                 const CUtensorMap& b0_sf, const CUtensorMap& b1_sf, const Mx4Args& args, bool single, cudaStream_t st) {
@@ -728,6 +679,19 @@ int launch_tiles(const CUtensorMap& a, const CUtensorMap& a_sf, const CUtensorMa
 
 }  // namespace
 
+int mx4_map_codes(CUtensorMap* m, const void* base, uint64_t experts, uint64_t rows, uint64_t k, uint32_t box_rows) {
+  const uint64_t dims[3] = {k / 2, rows, experts};
+  const uint64_t strides[2] = {k / 2, k / 2 * rows};
+  const uint32_t box[3] = {128, box_rows, 1};
+  return encode_tensor_map_bytes(m, base, 3, dims, strides, box);
+}
+int mx4_map_scales(CUtensorMap* m, const void* base, uint64_t tiles, int k) {
+  const uint64_t dims[3] = {128, (uint64_t)mx4_chunks(k), tiles};
+  const uint64_t strides[2] = {512, 512ull * mx4_chunks(k)};
+  const uint32_t box[3] = {128, 2, 1};
+  return encode_tensor_map_words(m, base, 3, dims, strides, box);
+}
+
 // The tables' rows are out_row0 .. of A, of its scale tiles and of the output alike.
 static Mx4Args mx4_args(const Mx4Rows& r) {
   Mx4Args ga = {};
@@ -745,10 +709,10 @@ int launch_mx4_linear(const Mx4Rows& r, const void* a_codes, const void* a_scale
   CUtensorMap a, a_sf, b, b_sf;
   int rc;
   const int wn = (n + 127) / 128;
-  if ((rc = map_codes(&a, a_codes, 1, r.rows, k))) return rc;
-  if ((rc = map_scales(&a_sf, a_scales, mx4_row_tiles(r.rows, r.table_segments), k))) return rc;
-  if ((rc = map_codes(&b, w_codes, experts, n, k))) return rc;
-  if ((rc = map_scales(&b_sf, w_scales, (uint64_t)experts * wn, k))) return rc;
+  if ((rc = mx4_map_codes(&a, a_codes, 1, r.rows, k, 128))) return rc;
+  if ((rc = mx4_map_scales(&a_sf, a_scales, mx4_row_tiles(r.rows, r.table_segments), k))) return rc;
+  if ((rc = mx4_map_codes(&b, w_codes, experts, n, k, 128))) return rc;
+  if ((rc = mx4_map_scales(&b_sf, w_scales, (uint64_t)experts * wn, k))) return rc;
   Mx4Args ga = mx4_args(r);
   ga.experts = experts;
   ga.n_total = n;
@@ -764,12 +728,12 @@ int launch_mx4_gated(const Mx4Rows& r, const void* a_codes, const void* a_scales
   CUtensorMap a, a_sf, g, u, g_sf, u_sf;
   int rc;
   const int wn = (f + 127) / 128;
-  if ((rc = map_codes(&a, a_codes, 1, r.rows, d))) return rc;
-  if ((rc = map_scales(&a_sf, a_scales, mx4_row_tiles(r.rows, r.table_segments), d))) return rc;
-  if ((rc = map_codes(&g, w->gate_codes, experts, f, d))) return rc;
-  if ((rc = map_codes(&u, w->up_codes, experts, f, d))) return rc;
-  if ((rc = map_scales(&g_sf, w->gate_scales, (uint64_t)experts * wn, d))) return rc;
-  if ((rc = map_scales(&u_sf, w->up_scales, (uint64_t)experts * wn, d))) return rc;
+  if ((rc = mx4_map_codes(&a, a_codes, 1, r.rows, d, 128))) return rc;
+  if ((rc = mx4_map_scales(&a_sf, a_scales, mx4_row_tiles(r.rows, r.table_segments), d))) return rc;
+  if ((rc = mx4_map_codes(&g, w->gate_codes, experts, f, d, 128))) return rc;
+  if ((rc = mx4_map_codes(&u, w->up_codes, experts, f, d, 128))) return rc;
+  if ((rc = mx4_map_scales(&g_sf, w->gate_scales, (uint64_t)experts * wn, d))) return rc;
+  if ((rc = mx4_map_scales(&u_sf, w->up_scales, (uint64_t)experts * wn, d))) return rc;
   Mx4Args ga = mx4_args(r);
   ga.experts = experts;
   ga.n_total = f;
