@@ -710,7 +710,8 @@ AXM_API int axm_mx4_expert_ffn(const AxmMoeDesc* desc, const void* x, int32_t ro
 /* axm_moe_forward with expert weights in 4 bits (and shared experts', when num_shared > 0):
  * router, permutation and combine are the layer's own, the expert feed-forward is the one above,
  * with the quantisation of x folded into the permutation's row copies.  tensors->w_* and shared_*
- * are not looked at; AXM_FLAG_H_EXACT does not apply.  Workspace: 256-byte aligned, its first word
+ * are not looked at; AXM_FLAG_H_EXACT does not apply.  x, router_w, out and y are 16-byte aligned
+ * (others are refused).  Workspace: 256-byte aligned, its first word
  * the status word. */
 AXM_API int axm_moe_mx4_workspace_bytes(const AxmMoeDesc* desc, size_t* bytes);
 AXM_API int axm_moe_forward_mx4(const AxmMoeDesc* desc, const AxmMoeTensors* tensors,

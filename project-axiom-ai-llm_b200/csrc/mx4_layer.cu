@@ -248,7 +248,8 @@ extern "C" int axm_moe_forward_mx4(const AxmMoeDesc* desc, const AxmMoeTensors* 
   if (t == nullptr) return fail(AXM_ERR_ARGUMENT, "tensors is null");
   if (desc->tokens == 0) return AXM_OK;
   if (!t->x || !t->router_w || !t->out) return fail(AXM_ERR_ARGUMENT, "%s: x, router_w and out are required", what);
-  if (off16(t->x)) return fail(AXM_ERR_ARGUMENT, "%s: x must be 16-byte aligned", what);
+  if (off16(t->x) || off16(t->router_w) || off16(t->out) || off16(t->y))
+    return fail(AXM_ERR_ARGUMENT, "%s: x, router_w, out and y must be 16-byte aligned", what);
   if (int rc = check_experts(experts, what)) return rc;
   if (desc->num_shared > 0)
     if (int rc = check_experts(shared, what)) return rc;

@@ -1,4 +1,6 @@
 """What the Python objects of the microscaled calls refuse before anything reaches the library."""
+import ctypes
+
 import pytest
 import torch
 
@@ -24,3 +26,20 @@ def test_training_scratch_of_another_device_of_the_same_kind(axm):
     axm.MoeTrainLayer(w, 8, 2, device="cpu", save_8bit=True, weight_grads=False, scratch=torch.empty(need, dtype=torch.uint8))
     with pytest.raises(ValueError, match="scratch"):
         axm.MoeTrainLayer(w, 8, 2, device="cpu", save_8bit=True, weight_grads=False, scratch=Elsewhere(need))
+
+
+def test_layer_refuses_matrices_off_16_bytes(axm):
+    """x, the router's weights and both outputs are read and written in 16-byte pieces."""
+    lib, fake = axm.load(), 1 << 20  # never dereferenced
+    desc = axm.make_desc(4, 64, 64, 4, 2)
+    size = ctypes.c_size_t(0)
+    assert lib.axm_moe_mx4_workspace_bytes(ctypes.byref(desc), ctypes.byref(size)) == axm.AXM_OK
+    weights = axm.Mx4ExpertWeights(*[fake] * 6)
+    for field in ("x", "router_w", "out", "y"):
+        for off in (2, 8):
+            t = axm.MoeTensors()
+            t.x = t.router_w = t.out = t.y = fake
+            setattr(t, field, fake + off)
+            assert lib.axm_moe_forward_mx4(ctypes.byref(desc), ctypes.byref(t), ctypes.byref(weights), None, fake, size.value,
+                                           None) == axm.AXM_ERR_ARGUMENT, (field, off)
+            assert b"aligned" in lib.axm_last_error()
