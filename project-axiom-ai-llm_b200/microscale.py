@@ -16,6 +16,7 @@ with fp32 masters (core/src/CUDA/util/gpu_types.cuh:148-168); either is a source
 import ctypes
 import functools
 import importlib
+import inspect
 
 import torch
 
@@ -33,13 +34,16 @@ def _dtype(t):
 def _on_its_device(call):
     """The library enqueues on the current device: makes that the device of the call's first tensor (or of
     the object's)."""
+    name = next(iter(inspect.signature(call).parameters))
+
     @functools.wraps(call)
-    def wrapped(first, *args, **kw):
-        device = first.device
-        if device.index is None or device.index == torch.cuda.current_device():  # host tensors are refused inside
-            return call(first, *args, **kw)
-        with torch.cuda.device(device):
-            return call(first, *args, **kw)
+    def wrapped(*args, **kw):
+        first = args[0] if args else kw.get(name)
+        index = None if first is None else first.device.index
+        if index is None or index == torch.cuda.current_device():  # host tensors are refused inside
+            return call(*args, **kw)
+        with torch.cuda.device(first.device):
+            return call(*args, **kw)
     return wrapped
 
 

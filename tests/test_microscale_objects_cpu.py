@@ -1,5 +1,6 @@
 """What the Python objects of the microscaled calls refuse before anything reaches the library."""
 import ctypes
+import importlib
 
 import pytest
 import torch
@@ -43,3 +44,15 @@ def test_layer_refuses_matrices_off_16_bytes(axm):
             assert lib.axm_moe_forward_mx4(ctypes.byref(desc), ctypes.byref(t), ctypes.byref(weights), None, fake, size.value,
                                            None) == axm.AXM_ERR_ARGUMENT, (field, off)
             assert b"aligned" in lib.axm_last_error()
+
+
+def test_calls_by_keyword(axm):
+    """The documented names of the first arguments: host tensors come as far as the call's own refusal."""
+    ms = importlib.import_module("project_axiom_ai_llm_b200.microscale")
+    x, codes, scales = torch.zeros(4, 64), torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    for call, kw in [(ms.quantize_rows, dict(x=x)), (ms.quantize_rows8, dict(x=x)), (ms.quantize_weights, dict(w=x.view(1, 4, 64))),
+                     (ms.dequantize_rows8, dict(codes=codes, scales=scales)), (ms.dequantize_rows8, dict(scales=scales, codes=codes))]:
+        with pytest.raises(ValueError, match="CUDA"):
+            call(**kw)
+    with pytest.raises(TypeError):
+        ms.quantize_rows()
