@@ -136,7 +136,17 @@ struct Units {
   }
 };
 // Units below which the reduction is cut: fewer with wide row tiles, whose partial sums cost more.
-// A cut call has less than twice as many.
+// A cut call has less than twice as many.  A linear call with its quantisation, weights from HBM, uncut and cut
+// by this rule, us:
+//                 1 row         24 rows       48 rows       112 rows
+//   11008 -> 4096 19.4 -> 12.9  19.6 -> 17.2  19.9 -> 17.1  21.1 -> 22.6
+//    8192 -> 2048 15.8 -> 10.6  15.9 -> 13.4  16.3 -> 14.6  17.5 -> 19.0
+//    4096 -> 4096 11.0 -> 10.0  11.3 -> 14.4  11.3 -> 13.1  12.5 -> 17.6
+//    2048 -> 1024  8.5 ->  7.9   8.9 -> 11.5   9.0 -> 11.9   9.5 -> 14.8
+//    1024 -> 4096  6.6 ->  7.3   6.9 ->  8.9   7.2 -> 10.2   8.3 -> 14.2
+// So it gains where the reduction is long and the row tile narrow, and loses elsewhere: it does not look at the
+// length of the reduction.  (A limit of 148 units: 9.3 and 10.1 for one row 4096 -> 4096 and 8192 -> 2048, but 18.9
+// where 24 rows 2048 -> 8192 take 9.3.)
 constexpr int few_enough(int n) { return n <= 32 ? 96 : n == 64 ? 64 : 48; }
 
 template <bool kGated, int N>
@@ -577,6 +587,19 @@ int launch_few_n(const Mx4Rows& r, const void* a_codes, const void* a_scales, co
 //   8 experts 4096 x 14336, top 2  128 (32)             133  140  180      256 (64)  164  145  195    512 (128)  234  202  199
 //   one matrix 4096 -> 14336        64                   12   14   15      128        14   16   17    256         20   17   18
 //              14336 -> 4096        64                   20   29   28 (few column tiles: the few-rows kernels cut the reduction)
+// Weights of other shapes, us of a feed-forward (rows a segment: few / one CTA / pairs) and of a linear call:
+//   16 experts 1024 x 512    24: 19 / 15 / 21     56: 17 / 15 / 22    144: 24 / 19 / 24    256: 30 / 24 / 30
+//    8 experts 2048 x 5632   24: 35 / 38 / 49     56: 44 / 40 / 50    144: 68 / 48 / 53    256: 86 / 65 / 72
+//   32 experts 512 x 2048    24: 25 / 26 / 42     56: 30 / 28 / 43    144: 55 / 39 / 46    256: 70 / 50 / 64
+//   128 experts 2048 x 768   24: 78 / 72 / 114    56: 92 / 80 / 123   144: 194 / 134 / 157  256: 235 / 174 / 220
+//   16 experts 5120 x 1536   24: 50 / 52 / 62     56: 58 / 55 / 67    144: 87 / 81 / 84    256: 109 / 101 / 107
+//   2048 -> 2048             64: 13.9 / 9.1 / 10.6    128: 16.0 / 10.5 / 12.3    512: 10.8 / 11.2 / 13.3
+//   5120 -> 5120             64: 14.7 / 15.4 / 16.9   128: 20.2 / 17.9 / 19.4    512: 21.9 / 19.4 / 21.0
+//   8192 -> 10240            64: 17.3 / 20.7 / 21.6   128: 19.2 / 23.8 / 24.5    512: 41.4 / 41.7 / 37.5
+//   1024 -> 16384            64:  8.1 / 8.3 / 11.3    128:  9.3 / 9.4 / 12.6     512: 17.6 / 13.6 / 16.2
+// The limit at 40 rows holds within a few per cent but for the smallest experts (24 rows: a fifth lost).  The one
+// at 128 is the wide layer's: all five of these would gain 5 to 24 % from the one-CTA kernel at 144 to 384 rows, and
+// small single matrices up to a third at 64 to 512; the rule does not look at K and N.
 // The few-rows kernels' row tiles are as wide as a segment has rows at most, or on average with room to
 // spare: a wider tile costs epilogue and tensor time, a narrower one reads the weights again (from
 // L2) for every further tile.
