@@ -243,11 +243,14 @@ __device__ __forceinline__ RowSegment segment_of_row(const AxmSegment* segments,
 }
 
 // A table's entry, kept inside the buffers whatever it says: rows beyond `rows_total` are dropped, and a
-// segment that starts outside or whose expert is not one of this launch's has none.
+// segment that starts outside or whose expert is not one of this launch's has none (the id is then 0xffff, which
+// no launch has: experts are read from 16 bits).
 __device__ __forceinline__ AxmSegment kept_inside(AxmSegment sg, int rows_total, int expert_base, int experts) {
-  const int e = (sg.expert & 0xffff) - expert_base;
-  const bool there = sg.out_row0 >= 0 && sg.out_row0 < rows_total && e >= 0 && e < experts;
+  const int e = (sg.expert & ~AXM_SEG_ALT_A) - expert_base;
+  const bool known = e >= 0 && e < experts;
+  const bool there = known && sg.out_row0 >= 0 && sg.out_row0 < rows_total;
   sg.rows = there ? min(max(sg.rows, 0), rows_total - sg.out_row0) : 0;
+  sg.expert = known ? sg.expert : 0xffff;
   return sg;
 }
 // Entry s of a product's segment table (none: one segment of all rows).

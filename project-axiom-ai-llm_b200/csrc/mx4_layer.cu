@@ -44,7 +44,8 @@ int check_ffn_desc(const AxmMoeDesc* d, const char* what) {
   if (d->tokens < 0) return fail(AXM_ERR_ARGUMENT, "%s: tokens %d negative", what, d->tokens);
   if (d->d_model <= 0 || d->d_ff <= 0 || d->d_model % 32 || d->d_ff % 32)
     return fail(AXM_ERR_ARGUMENT, "%s: d_model %d and d_ff %d must be positive multiples of 32", what, d->d_model, d->d_ff);
-  if (d->num_experts <= 0) return fail(AXM_ERR_ARGUMENT, "%s: num_experts must be positive", what);
+  if (d->num_experts <= 0 || d->num_experts > 65535)
+    return fail(AXM_ERR_ARGUMENT, "%s: num_experts %d not in 1..65535", what, d->num_experts);
   return AXM_OK;
 }
 

@@ -16,7 +16,8 @@ int check_call(const AxmMoeDesc* d, int32_t rows, const AxmSegment* segments, in
   if (d == nullptr) return fail(AXM_ERR_ARGUMENT, "desc is null");
   if (d->d_model <= 0 || d->d_ff <= 0 || d->d_model % 8 || d->d_ff % 32)
     return fail(AXM_ERR_ARGUMENT, "%s: d_model %d must be a positive multiple of 8, d_ff %d of 32", what, d->d_model, d->d_ff);
-  if (d->num_experts <= 0) return fail(AXM_ERR_ARGUMENT, "%s: num_experts must be positive", what);
+  if (d->num_experts <= 0 || d->num_experts > 65535)
+    return fail(AXM_ERR_ARGUMENT, "%s: num_experts %d not in 1..65535", what, d->num_experts);
   if (rows < 0) return fail(AXM_ERR_ARGUMENT, "%s: %d rows", what, rows);
   if (num_segments < 0 || num_segments > kMaxSegments)
     return fail(AXM_ERR_ARGUMENT, "%s: num_segments %d not in 0..%d", what, num_segments, kMaxSegments);

@@ -56,3 +56,14 @@ def test_calls_by_keyword(axm):
             call(**kw)
     with pytest.raises(TypeError):
         ms.quantize_rows()
+
+
+def test_more_experts_than_a_table_can_name(axm):
+    """A segment's expert is read from 16 bits."""
+    lib, fake, size = axm.load(), 1 << 20, ctypes.c_size_t(0)
+    keep = axm.Mx8Checkpoint(*[fake] * 4)
+    for experts, status in ((65535, axm.AXM_OK), (65536, axm.AXM_ERR_ARGUMENT), (70000, axm.AXM_ERR_ARGUMENT)):
+        desc = axm.make_desc(4, 64, 64, experts, 1)
+        assert lib.axm_mx4_expert_ffn_workspace_bytes(ctypes.byref(desc), 4, 2, ctypes.byref(size)) == status
+        assert lib.axm_mx8_expert_ffn_train(ctypes.byref(desc), None, 0, None, 0, None, None, None, ctypes.byref(keep), None, None, 0,
+                                            None, None) == status

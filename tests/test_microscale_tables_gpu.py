@@ -122,3 +122,29 @@ def test_training_tables_that_do_not_fit(ms, axm, cuda_device):
             want = got if want is None else want
             assert all(torch.equal(got[n], want[n]) for n in got), (name, [n for n in got if not torch.equal(got[n], want[n])])
             assert torch.isfinite(v["d_x"].float()).all() and (v["dwg"].view(e, d, f)[3] == 0).all()
+
+
+@pytest.mark.parametrize("rows", [40, 250, 700])  # few-rows, one-CTA and pair kernels
+@pytest.mark.parametrize("expert", [1 << 16, (1 << 20) + 1, 1 << 29, -(1 << 31), -65536])
+def test_experts_whose_low_bits_look_right(ms, cuda_device, rows, expert):
+    """An id is compared as a whole: such an entry's rows are left as they are and no other expert's gradient is
+    touched."""
+    d, f, n = 64, 96, rows // 2
+    w = [torch.randn(2, *kn, device=cuda_device).to(BF16) for kn in ((d, f), (d, f), (f, d))]
+    x = torch.randn(rows, d, device=cuda_device).to(BF16)
+    good, odd = entries([(0, n, 1), (n, 0, 0)], cuda_device), entries([(0, n, 1), (n, rows - n, expert)], cuda_device)
+    plan = ms.Mx4ExpertFfn(*(ms.quantize_weights(t) for t in w), rows=rows, tokens=rows)
+    want, got = (plan.forward(x, t, out=torch.full((rows, d), 5.0, dtype=BF16, device=cuda_device)) for t in (good, odd))
+    assert plan.status() == 0 and torch.equal(want, got) and (got[n:] == 5).all()
+    rows, n = -(-rows // 64) * 64, -(-n // 64) * 64  # the training layout
+    x = torch.randn(rows, d, device=cuda_device).to(BF16)
+    good = entries([(0, n, 1), (n, 0, 0)], cuda_device)
+    odd = entries([(0, n, 1), (n, rows - n, expert), (n, 0, 0)], cuda_device)
+    plan = ms.Mx8TrainFfn(*w, rows=rows)
+    outs = []
+    for t in (good, odd):
+        o = plan.forward(x, t, out=torch.full((rows, d), 5.0, dtype=BF16, device=cuda_device))
+        g = plan.backward(x)
+        outs.append([o, g["d_x"][:n], g["d_gate"], g["d_up"], g["d_down"]])
+    assert plan.status() == 0 and all(torch.equal(a, b) for a, b in zip(*outs)) and (outs[1][0][n:] == 5).all()
+    assert (outs[1][2][0] == 0).all() and bool((outs[1][2][1] != 0).any())
