@@ -740,10 +740,9 @@ AXM_API int axm_mx8_checkpoint_bytes(int32_t rows, int32_t d_ff, size_t* code_by
  * the three weight gradients may all be NULL.  h, d_g, d_u [rows][F] bf16 are scratch of the call.
  * Tables as for axm_moe_expert_ffn_backward: a_row0 == out_row0, every expert once, segments
  * padded to multiples of 64 rows with zero rows of x and d_o (the gradients of experts that a
- * table leaves out, and of all with num_segments 0, are not written; rows outside every segment of what
- * has rows are left as they are).  Entries are kept inside `rows`: one that starts outside or names an
- * expert that does not exist has no rows, rows behind the last are cut off.  d_ff is a multiple of 32,
- * d_model of 8.
+ * table leaves out, and of all with num_segments 0, are not written, nor are rows of o and d_x outside
+ * every segment).  Entries are kept inside `rows`: one that starts outside or names an expert that does
+ * not exist has no rows, rows behind the last are cut off.  d_ff is a multiple of 32, d_model of 8.
  * status: an optional int32 device word that receives a non-zero code when a bounded wait gave up. */
 AXM_API int axm_mx8_expert_ffn_train(const AxmMoeDesc* desc, const void* x, int32_t rows,
                                      const AxmSegment* segments, int32_t num_segments, const void* w_gate,

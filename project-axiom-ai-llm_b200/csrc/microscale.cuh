@@ -136,10 +136,10 @@ __device__ __forceinline__ uint4 mx4_quantize_block(const float (&h)[32], uint32
 }
 // Reading back.  What a block of e2m1 holds is exact in bf16 (two significant bits, 2^-128 the smallest), and
 // what a block of e4m3 holds is too but for the smallest codes under the scale bytes 0 to 2 (steps of 2^-136
-// to 2^-134), which round once; to fp32 they are decoded one by one (mx8_unpack2).  So codes are decoded two at a time: their
-// exponent and mantissa bits moved to bf16's places are the value times 2^-126 (e2m1) or 2^-120 (e4m3),
-// subnormal codes included, and two packed multiplications by powers of two put that right; the first is
-// exact.  Half the instructions of decoding one by one in fp32, which is what bounded the kernels that read
+// to 2^-134), which round once; to fp32 they are decoded one by one (mx8_unpack2).  So codes are decoded two at
+// a time: their exponent and mantissa bits moved to bf16's places are the value times 2^-126 (e2m1) or 2^-120
+// (e4m3), subnormal codes included, and two packed multiplications by powers of two put that right; the first
+// is exact.  Half the instructions of decoding one by one in fp32, which is what bounded the kernels that read
 // blocks back.
 __device__ __forceinline__ uint32_t mx_scale_bf16x2(uint32_t s) {  // 2^(s - 127), twice
   const uint32_t h = s == 255u ? 0x7fc0u : (s == 0u ? 0x0040u : s << 7);
